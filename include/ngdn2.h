@@ -23,6 +23,12 @@
  * Layouts are the reference's (chunk.py:184-217): per-token tensors
  * [B, T, H, ...], states [B, H, L, K, V] float32, parameters
  * [L-1, H, ...] contiguous.
+ *
+ * The operators around that path that a language model's training and
+ * decoding also need, without a counterpart in the reference: the scaled
+ * embedding lookup and its gradient (ngdn2_embed*), the gated linear
+ * recurrence (ngdn2_scan*) and the Newton-Schulz orthogonalisation of
+ * weight updates (ngdn2_orth*).
  */
 #ifndef NGDN2_H_
 #define NGDN2_H_
@@ -87,7 +93,8 @@ enum {
   NGDN2_ERR_UNSUPPORTED = -11,  /* requested path cannot run this shape/dtype */
   NGDN2_ERR_CUDA = -12,         /* a CUDA runtime call failed */
   NGDN2_ERR_ABI = -13,          /* abi_version mismatch */
-  NGDN2_ERR_FIRING = -14        /* firing intervals not nested or not >= 1 */
+  NGDN2_ERR_FIRING = -14,       /* firing intervals not nested or not >= 1 */
+  NGDN2_ERR_COEFFICIENTS = -15  /* Newton-Schulz coefficients whose iteration leaves [0, 4] */
 };
 
 /* Arguments of ngdn2_fwd. */
@@ -148,7 +155,9 @@ enum {
   NGDN2_STATUS_WAIT_TIMEOUT = 1, /* a bounded pipeline wait gave up: outputs are not valid, and
                                     the CUDA context should be treated as suspect (an MMA or copy
                                     the wait was for may still have been in flight) */
-  NGDN2_STATUS_GATE_TIMEOUT = 2  /* the start gate stayed zero: nothing was computed */
+  NGDN2_STATUS_GATE_TIMEOUT = 2, /* the start gate stayed zero: nothing was computed */
+  NGDN2_STATUS_BAD_INDEX = 4     /* a token id outside [0, V): its row is NaN, and the gradient
+                                    leaves it out */
 };
 
 /* Arguments of ngdn2_update_state (update_fwd.py:131-204). */
@@ -264,6 +273,112 @@ typedef struct ngdn2_bwd_args {
   size_t workspace_bytes;
 } ngdn2_bwd_args;
 
+/* Arguments of ngdn2_embed: out[n] = scale * weight[ids[n]]. */
+typedef struct ngdn2_embed_args {
+  int32_t abi_version;
+  int32_t dtype;         /* of weight and out */
+  int32_t ids_i32;       /* ids are int32 (else int64) */
+  float scale;
+  int64_t N, V, D;       /* tokens, rows of weight, columns */
+  const void* ids;       /* [N] contiguous */
+  const void* weight;    /* [V, D], unit column stride */
+  int64_t weight_stride; /* elements from one row to the next */
+  void* out;             /* [N, D] contiguous */
+  int32_t* status;       /* required: NGDN2_STATUS_BAD_INDEX */
+} ngdn2_embed_args;
+
+/* Arguments of ngdn2_embed_bwd:
+ * dweight[v] = scale * sum over {n : ids[n] = v} of d_out[n], every row
+ * written (zeros where no token points, and for padding_idx). Summed in
+ * fp32 in the order of n, so the result is reproducible. */
+typedef struct ngdn2_embed_bwd_args {
+  int32_t abi_version;
+  int32_t dtype;         /* of d_out */
+  int32_t out_dtype;     /* of dweight */
+  int32_t ids_i32;
+  float scale;
+  int64_t N, V, D;
+  int64_t padding_idx;   /* its row gets no gradient; -1 for none */
+  const void* ids;       /* [N] contiguous */
+  const void* d_out;     /* [N, D], unit column stride */
+  int64_t d_stride;      /* elements from one row to the next */
+  void* dweight;         /* [V, D] contiguous */
+  void* workspace;       /* >= ngdn2_embed_bwd_workspace_size */
+  size_t workspace_bytes;
+  int32_t* status;       /* required: NGDN2_STATUS_BAD_INDEX */
+} ngdn2_embed_bwd_args;
+
+/* Steps between the states that ngdn2_scan leaves for its backward. */
+#define NGDN2_SCAN_CHUNK 128
+
+/* Arguments of ngdn2_scan: h_t = e^(g_t) h_{t-1} + x_t for each (batch row,
+ * channel), the state in fp32. g = -inf drops the state (a packed sequence
+ * starts); strides are in elements, 0 included. */
+typedef struct ngdn2_scan_args {
+  int32_t abi_version;
+  int32_t B;
+  int64_t T, D;
+  const void* x; int32_t x_dtype; int64_t x_stride[3]; /* [B, T, D] */
+  const void* g; int32_t g_dtype; int64_t g_stride[3]; /* [B, T, D] log-decays */
+  const float* initial_state;  /* [B, D] contiguous, or NULL for zeros */
+  void* h;                     /* [B, T, D] contiguous, x's element type */
+  float* final_state;          /* [B, D] contiguous, or NULL to skip */
+  float* carries;              /* [B, ceil(T / NGDN2_SCAN_CHUNK), D]: the state entering each
+                                  chunk, for ngdn2_scan_bwd; or NULL to skip */
+  void* workspace;             /* >= ngdn2_scan_workspace_size */
+  size_t workspace_bytes;
+  int32_t* status;             /* required: NGDN2_STATUS_WAIT_TIMEOUT */
+} ngdn2_scan_args;
+
+/* Arguments of ngdn2_scan_bwd: the gradients of sum(h * d_h) +
+ * sum(final * d_final): u_t = d_h_t + e^(g_{t+1}) u_{t+1}; dx = u,
+ * dg_t = u_t e^(g_t) h_{t-1}, d_initial = e^(g_1) u_1. */
+typedef struct ngdn2_scan_bwd_args {
+  int32_t abi_version;
+  ngdn2_scan_args fwd;         /* the forward's inputs and carries (required); its h,
+                                  final_state, workspace and status are not used */
+  const void* d_h; int32_t d_h_dtype; int64_t d_h_stride[3]; /* [B, T, D], x's element type */
+  const float* d_final;        /* [B, D] contiguous, or NULL for zeros */
+  void* dx;                    /* [B, T, D] contiguous, x's element type */
+  void* dg;                    /* [B, T, D] contiguous, g's element type */
+  float* d_initial;            /* [B, D] contiguous, or NULL to skip */
+  void* workspace;             /* >= ngdn2_scan_workspace_size of the forward's arguments */
+  size_t workspace_bytes;
+  int32_t* status;             /* required: NGDN2_STATUS_WAIT_TIMEOUT */
+} ngdn2_scan_bwd_args;
+
+/* Arguments of ngdn2_scan_step: one token of ngdn2_scan. */
+typedef struct ngdn2_scan_step_args {
+  int32_t abi_version;
+  int32_t B;
+  int64_t D;
+  const void* x; int32_t x_dtype; int64_t x_stride[2]; /* [B, D] */
+  const void* g; int32_t g_dtype; int64_t g_stride[2]; /* [B, D] */
+  const float* state_in;       /* [B, D] contiguous */
+  float* state_out;            /* [B, D] contiguous; may equal state_in */
+  void* h;                     /* [B, D] contiguous, x's element type */
+} ngdn2_scan_step_args;
+
+/* Arguments of ngdn2_orth: X_0 = G / (|G|_F + eps), then ``steps`` times
+ * X <- a X + (b A + c A A) X with A = X X^T taken over the smaller side,
+ * for each of ``batch`` matrices. Products to fp32's accuracy, whatever the
+ * element types. */
+typedef struct ngdn2_orth_args {
+  int32_t abi_version;
+  int32_t dtype;               /* of update */
+  int32_t out_dtype;
+  int32_t steps;
+  float coef[3];               /* a, b, c */
+  float eps;
+  int64_t batch, rows, cols;
+  const void* update;          /* [batch, rows, cols] */
+  int64_t update_stride[3];    /* elements */
+  void* out;                   /* [batch, rows, cols] contiguous */
+  void* workspace;             /* >= ngdn2_orth_workspace_size */
+  size_t workspace_bytes;
+  int32_t* status;             /* required: NGDN2_STATUS_WAIT_TIMEOUT */
+} ngdn2_orth_args;
+
 NGDN2_API int ngdn2_abi_version(void);
 /* sizeof the argument structs, so bindings can check their layout. */
 NGDN2_API size_t ngdn2_sizeof_fwd_args(void);
@@ -271,6 +386,12 @@ NGDN2_API size_t ngdn2_sizeof_update_args(void);
 NGDN2_API size_t ngdn2_sizeof_step_args(void);
 NGDN2_API size_t ngdn2_sizeof_bwd_args(void);
 NGDN2_API size_t ngdn2_sizeof_update_bwd_args(void);
+NGDN2_API size_t ngdn2_sizeof_embed_args(void);
+NGDN2_API size_t ngdn2_sizeof_embed_bwd_args(void);
+NGDN2_API size_t ngdn2_sizeof_scan_args(void);
+NGDN2_API size_t ngdn2_sizeof_scan_bwd_args(void);
+NGDN2_API size_t ngdn2_sizeof_scan_step_args(void);
+NGDN2_API size_t ngdn2_sizeof_orth_args(void);
 NGDN2_API const char* ngdn2_error_string(int code);
 
 /* Validates *args and returns the workspace ngdn2_fwd needs, in bytes. */
@@ -320,6 +441,21 @@ NGDN2_API int ngdn2_step_workspace_size(const ngdn2_step_args* args, size_t* byt
  * promotes, bottom-up, per batch row (rows may sit at different positions).
  * Reads state_in, writes state_out (in place when they are equal). */
 NGDN2_API int ngdn2_step(const ngdn2_step_args* args, void* stream);
+
+/* The scaled embedding lookup and its gradient. */
+NGDN2_API int ngdn2_embed(const ngdn2_embed_args* args, void* stream);
+NGDN2_API int ngdn2_embed_bwd_workspace_size(const ngdn2_embed_bwd_args* args, size_t* bytes);
+NGDN2_API int ngdn2_embed_bwd(const ngdn2_embed_bwd_args* args, void* stream);
+
+/* The gated linear recurrence, its backward and its one-token step. */
+NGDN2_API int ngdn2_scan_workspace_size(const ngdn2_scan_args* args, size_t* bytes);
+NGDN2_API int ngdn2_scan(const ngdn2_scan_args* args, void* stream);
+NGDN2_API int ngdn2_scan_bwd(const ngdn2_scan_bwd_args* args, void* stream);
+NGDN2_API int ngdn2_scan_step(const ngdn2_scan_step_args* args, void* stream);
+
+/* The Newton-Schulz orthogonalisation of weight updates. */
+NGDN2_API int ngdn2_orth_workspace_size(const ngdn2_orth_args* args, size_t* bytes);
+NGDN2_API int ngdn2_orth(const ngdn2_orth_args* args, void* stream);
 
 /* Capacity of the fixed scratch buffer behind ngdn2_fwd_noalloc. */
 #define NGDN2_NOALLOC_SCRATCH_BYTES ((size_t)64 << 20)

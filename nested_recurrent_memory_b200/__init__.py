@@ -6,6 +6,11 @@ with its backward, ``chunk_nested_gdn2_fwd``, ``chunk_nested_gdn2_bwd``,
 ``naive_step_nested_gdn2`` as ``step_nested_gdn2``), computed by hand-written
 sm_100a CUDA kernels behind the C ABI in ``include/ngdn2.h``. ``HostPipeline``
 runs the op over host-resident batches with their copies overlapped.
+
+Around it, the operators that training and decoding a language model of
+recurrent layers needs: ``embed_tokens`` (scaled embedding lookup and its
+gradient), ``gated_scan`` / ``step_gated_scan`` (the channel-wise gated
+linear recurrence) and ``orthogonalize`` (Newton-Schulz weight updates).
 """
 
 from .ops import (  # noqa: F401
@@ -23,6 +28,14 @@ from .ops import (  # noqa: F401
     update_state,
     update_state_bwd,
 )
+from .embedding import embed_tokens, embed_tokens_bwd, embed_tokens_fwd  # noqa: F401
 from .host import HostPipeline  # noqa: F401
+from .orthogonal import orthogonalize  # noqa: F401
+from .recurrence import (  # noqa: F401
+    gated_scan,
+    gated_scan_bwd,
+    gated_scan_fwd,
+    step_gated_scan,
+)
 
 __version__ = "0.1.0"

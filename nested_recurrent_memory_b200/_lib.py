@@ -1,7 +1,9 @@
 """ctypes binding of ``libngdn2.so`` (the C ABI declared in include/ngdn2.h).
 
 The structs below mirror ``ngdn2_fwd_args``, ``ngdn2_update_args``,
-``ngdn2_step_args``, ``ngdn2_bwd_args`` and ``ngdn2_update_bwd_args`` field
+``ngdn2_step_args``, ``ngdn2_bwd_args``, ``ngdn2_update_bwd_args``,
+``ngdn2_embed_args``, ``ngdn2_embed_bwd_args``, ``ngdn2_scan_args``,
+``ngdn2_scan_bwd_args``, ``ngdn2_scan_step_args`` and ``ngdn2_orth_args`` field
 for field; ``check_layout()`` compares their sizes with the library's own
 ``sizeof``. Loading fails loudly: there is no fallback implementation.
 """
@@ -30,9 +32,13 @@ ERR_BLOCK_V = -3
 ERR_DIVISIBLE = -4
 ERR_UNIT_STRIDE = -5
 ERR_INCONSISTENT = -6
+ERR_COEFFICIENTS = -15
 
 STATUS_WAIT_TIMEOUT = 1
 STATUS_GATE_TIMEOUT = 2
+STATUS_BAD_INDEX = 4
+
+SCAN_CHUNK = 128
 
 c_i32, c_i64, c_ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
 
@@ -111,6 +117,59 @@ class BwdArgs(ctypes.Structure):
     ]
 
 
+class EmbedArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", c_i32), ("dtype", c_i32), ("ids_i32", c_i32), ("scale", ctypes.c_float),
+        ("N", c_i64), ("V", c_i64), ("D", c_i64),
+        ("ids", c_ptr), ("weight", c_ptr), ("weight_stride", c_i64), ("out", c_ptr),
+        ("status", c_ptr),
+    ]
+
+
+class EmbedBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", c_i32), ("dtype", c_i32), ("out_dtype", c_i32), ("ids_i32", c_i32),
+        ("scale", ctypes.c_float),
+        ("N", c_i64), ("V", c_i64), ("D", c_i64), ("padding_idx", c_i64),
+        ("ids", c_ptr), ("d_out", c_ptr), ("d_stride", c_i64), ("dweight", c_ptr),
+        ("workspace", c_ptr), ("workspace_bytes", ctypes.c_size_t), ("status", c_ptr),
+    ]
+
+
+class ScanArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", c_i32), ("B", c_i32), ("T", c_i64), ("D", c_i64),
+        *_tok("x", 3), *_tok("g", 3),
+        ("initial_state", c_ptr), ("h", c_ptr), ("final_state", c_ptr), ("carries", c_ptr),
+        ("workspace", c_ptr), ("workspace_bytes", ctypes.c_size_t), ("status", c_ptr),
+    ]
+
+
+class ScanBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", c_i32), ("fwd", ScanArgs), *_tok("d_h", 3), ("d_final", c_ptr),
+        ("dx", c_ptr), ("dg", c_ptr), ("d_initial", c_ptr),
+        ("workspace", c_ptr), ("workspace_bytes", ctypes.c_size_t), ("status", c_ptr),
+    ]
+
+
+class ScanStepArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", c_i32), ("B", c_i32), ("D", c_i64), *_tok("x", 2), *_tok("g", 2),
+        ("state_in", c_ptr), ("state_out", c_ptr), ("h", c_ptr),
+    ]
+
+
+class OrthArgs(ctypes.Structure):
+    _fields_ = [
+        ("abi_version", c_i32), ("dtype", c_i32), ("out_dtype", c_i32), ("steps", c_i32),
+        ("coef", ctypes.c_float * 3), ("eps", ctypes.c_float),
+        ("batch", c_i64), ("rows", c_i64), ("cols", c_i64),
+        ("update", c_ptr), ("update_stride", c_i64 * 3), ("out", c_ptr),
+        ("workspace", c_ptr), ("workspace_bytes", ctypes.c_size_t), ("status", c_ptr),
+    ]
+
+
 EXPORTS = (
     "ngdn2_abi_version", "ngdn2_sizeof_fwd_args", "ngdn2_sizeof_update_args",
     "ngdn2_error_string", "ngdn2_fwd_workspace_size", "ngdn2_fwd_select_path",
@@ -118,6 +177,11 @@ EXPORTS = (
     "ngdn2_fwd_noalloc", "ngdn2_sizeof_step_args", "ngdn2_step_workspace_size", "ngdn2_step",
     "ngdn2_sizeof_bwd_args", "ngdn2_bwd_workspace_size", "ngdn2_bwd", "ngdn2_bwd_num_launches",
     "ngdn2_sizeof_update_bwd_args", "ngdn2_update_bwd_workspace_size", "ngdn2_update_state_bwd",
+    "ngdn2_sizeof_embed_args", "ngdn2_sizeof_embed_bwd_args", "ngdn2_sizeof_scan_args",
+    "ngdn2_sizeof_scan_bwd_args", "ngdn2_sizeof_scan_step_args", "ngdn2_sizeof_orth_args",
+    "ngdn2_embed", "ngdn2_embed_bwd_workspace_size", "ngdn2_embed_bwd",
+    "ngdn2_scan_workspace_size", "ngdn2_scan", "ngdn2_scan_bwd", "ngdn2_scan_step",
+    "ngdn2_orth_workspace_size", "ngdn2_orth",
 )
 
 _LIB = None
@@ -171,6 +235,16 @@ def load(path: str | os.PathLike | None = None):
     lib.ngdn2_update_bwd_workspace_size.restype = ctypes.c_int
     lib.ngdn2_update_state_bwd.argtypes = [ctypes.POINTER(UpdateBwdArgs), c_ptr]
     lib.ngdn2_update_state_bwd.restype = ctypes.c_int
+    for name, struct in (("embed", EmbedArgs), ("embed_bwd", EmbedBwdArgs), ("scan", ScanArgs),
+                         ("scan_bwd", ScanBwdArgs), ("scan_step", ScanStepArgs),
+                         ("orth", OrthArgs)):
+        getattr(lib, f"ngdn2_sizeof_{name}_args").restype = ctypes.c_size_t
+        fn = getattr(lib, f"ngdn2_{name}")
+        fn.argtypes, fn.restype = [ctypes.POINTER(struct), c_ptr], ctypes.c_int
+    for name, struct in (("embed_bwd", EmbedBwdArgs), ("scan", ScanArgs), ("orth", OrthArgs)):
+        fn = getattr(lib, f"ngdn2_{name}_workspace_size")
+        fn.argtypes = [ctypes.POINTER(struct), ctypes.POINTER(ctypes.c_size_t)]
+        fn.restype = ctypes.c_int
     if path is None:
         _LIB = lib
     return lib
@@ -190,6 +264,11 @@ def check_layout(lib=None) -> None:
         raise RuntimeError("ngdn2_bwd_args layout mismatch")
     if lib.ngdn2_sizeof_update_bwd_args() != ctypes.sizeof(UpdateBwdArgs):
         raise RuntimeError("ngdn2_update_bwd_args layout mismatch")
+    for name, struct in (("embed", EmbedArgs), ("embed_bwd", EmbedBwdArgs), ("scan", ScanArgs),
+                         ("scan_bwd", ScanBwdArgs), ("scan_step", ScanStepArgs),
+                         ("orth", OrthArgs)):
+        if getattr(lib, f"ngdn2_sizeof_{name}_args")() != ctypes.sizeof(struct):
+            raise RuntimeError(f"ngdn2_{name}_args layout mismatch")
 
 
 def error_string(code: int) -> str:

@@ -157,6 +157,8 @@ const char* ngdn2_error_string(int code) {
     case NGDN2_ERR_CUDA: return "CUDA runtime error";
     case NGDN2_ERR_ABI: return "ABI version mismatch";
     case NGDN2_ERR_FIRING: return "firing intervals must be >= 1";
+    case NGDN2_ERR_COEFFICIENTS:
+      return "the iteration with these coefficients leaves [0, 4] for a singular value in [0, 1]";
     default: return "unknown error";
   }
 }

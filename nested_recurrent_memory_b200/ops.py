@@ -46,9 +46,9 @@ _LAST_PATH = [None]
 
 
 class KernelStatusError(RuntimeError):
-    """A forward's kernels reported a device status (include/ngdn2.h
-    NGDN2_STATUS_*): a bounded wait gave up, so that forward's outputs are
-    not valid."""
+    """A call's kernels reported a device status (include/ngdn2.h
+    NGDN2_STATUS_*): a bounded wait gave up, so that call's outputs are not
+    valid, or an embedding met a token id outside its table."""
 
 
 def _status_message(bits: int) -> str:
@@ -58,6 +58,9 @@ def _status_message(bits: int) -> str:
                      "context as suspect)")
     if bits & _lib.STATUS_GATE_TIMEOUT:
         parts.append("the start gate stayed closed (nothing was computed)")
+    if bits & _lib.STATUS_BAD_INDEX:
+        parts.append("embedding: a token id outside [0, V) (its output row is NaN, its gradient "
+                     "left out)")
     return "; ".join(parts) or f"status bits {bits:#x}"
 
 
@@ -96,7 +99,8 @@ class _DeviceStatus:
         if bits:
             self.word.zero_()
             self.host.zero_()
-            raise KernelStatusError(f"nested GDN-2 forward: {_status_message(bits)}")
+            what = "nested GDN-2 forward: " if bits != _lib.STATUS_BAD_INDEX else ""
+            raise KernelStatusError(what + _status_message(bits))
 
     def poll(self):
         """Raise for a status copied back by an earlier launch, if its copy is done."""
@@ -121,6 +125,17 @@ class _DeviceStatus:
             self._raise_if_set(int(self.word.item()))
         else:
             self.poll()
+
+
+    def word_ptr(self) -> int:
+        """Device address of the status word, for calls that poison their
+        outputs with NaN when they set it and so queue no copy of it: it
+        surfaces at ``check_status`` or the next forward's copy."""
+        return self.word.data_ptr()
+
+    def after_poisoning_launch(self):
+        if _SYNC_CHECK and not torch.cuda.is_current_stream_capturing():
+            self.check(sync=True)
 
 
 _SYNC_CHECK = __import__("os").environ.get("NGDN2_SYNC_CHECK", "0") not in ("", "0")
@@ -163,6 +178,31 @@ def _require_cuda(*ts):
             raise RuntimeError(
                 "nested_recurrent_memory_b200 runs on CUDA tensors only (no CPU fallback); "
                 f"got a tensor on {t.device}")
+
+
+class _SameDevice:
+    """No change of device (the tensors' device is already current)."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def _on_device(dev):
+    """The context in which a launch on ``dev`` runs: launches go to the
+    current device, so it is changed when it is another one."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(dev)
+
+
+def _stream(dev):
+    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
 
 
 def _fill_tok(args, name, t, rank):

@@ -1,0 +1,70 @@
+"""Orthogonalising weight updates by Newton-Schulz products, by the kernels
+behind ``ngdn2_orth`` (include/ngdn2.h), as the Muon optimiser does.
+
+    X_0 = G / (|G|_F + eps);   X <- a X + (b A + c A A) X,  A = X X^T
+
+with the products taken over the smaller side of G. After a few steps the
+singular values of X lie around 1 and its singular vectors are G's.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .ops import _code, _DeviceStatus, _on_device, _raise_for, _require_cuda, _stream
+
+__all__ = ["orthogonalize"]
+
+
+def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, dtype=None,
+                  workspace=None):
+    """The orthogonalised update. update [..., rows, cols] in float32,
+    bfloat16 or float16; leading dimensions are a batch of matrices treated
+    each on its own (layers stacked, or promotion parameters
+    [L - 1, H, rows, cols]). Returns the same shape in ``dtype`` (default
+    update's). Products and sums keep fp32's accuracy whatever the types.
+
+    ``coefficients`` (a, b, c) must keep every singular value that starts in
+    [0, 1] within [0, 4] over ``steps`` steps, else ValueError. A zero update
+    gives zeros.
+    """
+    if update.dim() < 2:
+        raise ValueError(f"update must be [..., rows, cols], got {tuple(update.shape)}")
+    _require_cuda(update)
+    rows, cols = update.shape[-2:]
+    dev = update.device
+    out = torch.empty(update.shape, dtype=dtype or update.dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    flat = update if update.dim() == 3 else update.reshape(-1, rows, cols)
+    status = _DeviceStatus.get(dev)
+    a = _lib.OrthArgs()
+    a.abi_version = _lib.ABI_VERSION
+    a.dtype, a.out_dtype = _code(flat), _code(out)
+    a.steps = int(steps)
+    for i, c in enumerate(coefficients):
+        a.coef[i] = c
+    a.eps = eps
+    a.batch, a.rows, a.cols = flat.shape[0], rows, cols
+    a.update, a.out, a.status = flat.data_ptr(), out.data_ptr(), status.word_ptr()
+    for i, st in enumerate(flat.stride()):
+        a.update_stride[i] = st
+    lib = _lib.load()
+    need = ctypes.c_size_t(0)
+    rc = lib.ngdn2_orth_workspace_size(ctypes.byref(a), ctypes.byref(need))
+    if rc == _lib.ERR_COEFFICIENTS:
+        raise ValueError(f"coefficients {tuple(coefficients)} do not keep singular values in "
+                         f"[0, 1] within [0, 4] over {steps} steps")
+    _raise_for(rc, "ngdn2_orth")
+    if need.value and (workspace is None or workspace.numel() < need.value):
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
+    if need.value:
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    with _on_device(dev):
+        rc = lib.ngdn2_orth(ctypes.byref(a), _stream(dev))
+    _raise_for(rc, "ngdn2_orth")
+    status.after_poisoning_launch()
+    return out

@@ -1,0 +1,200 @@
+"""Gated linear recurrence, by the kernels behind ``ngdn2_scan``,
+``ngdn2_scan_bwd`` and ``ngdn2_scan_step`` (include/ngdn2.h).
+
+    h_t = e^{g_t} h_{t-1} + x_t        for every channel, t = 1 .. T
+
+The state is fp32 throughout. ``g`` are log-decays, as in the nested op
+(``<= 0`` for a decay); ``g = -inf`` drops the state, so packed sequences of
+different lengths are one call with -inf at each sequence's first token.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .ops import _code, _DeviceStatus, _fill_tok, _on_device, _raise_for, _require_cuda, _stream
+
+__all__ = ["gated_scan", "gated_scan_fwd", "gated_scan_bwd", "step_gated_scan"]
+
+
+def _check_state(state, B, D, name):
+    if state is None:
+        return None
+    if tuple(state.shape) != (B, D):
+        raise ValueError(f"{name} must be [{B}, {D}], got {tuple(state.shape)}")
+    _require_cuda(state)
+    if state.dtype == torch.float32 and state.is_contiguous():
+        return state
+    return state.to(torch.float32).contiguous()
+
+
+def _scan_args(x, g, init):
+    B, T, D = x.shape
+    a = _lib.ScanArgs()
+    a.abi_version = _lib.ABI_VERSION
+    a.B, a.T, a.D = B, T, D
+    _fill_tok(a, "x", x, 3)
+    _fill_tok(a, "g", g, 3)
+    a.initial_state = init.data_ptr() if init is not None else None
+    return a
+
+
+def _check_inputs(x, g):
+    if x.dim() != 3 or x.shape != g.shape:
+        raise ValueError(f"x and g must both be [B, T, D], got {tuple(x.shape)} and "
+                         f"{tuple(g.shape)}")
+    _require_cuda(x, g)
+
+
+def _workspace(a, workspace, dev):
+    need = ctypes.c_size_t(0)
+    _raise_for(_lib.load().ngdn2_scan_workspace_size(ctypes.byref(a), ctypes.byref(need)),
+               "ngdn2_scan")
+    if need.value and (workspace is None or workspace.numel() < need.value):
+        workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
+    return workspace if need.value else None
+
+
+def gated_scan_fwd(x, g, initial_state=None, output_final_state=False, return_aux=False,
+                   workspace=None):
+    """The recurrence forward. x, g [B, T, D] in float32, bfloat16 or float16
+    (any strides, broadcast views included); initial_state [B, D] or None.
+    Returns ``(h, final_state)``: h [B, T, D] in x's dtype, final_state
+    [B, D] float32 (None unless ``output_final_state``); with ``return_aux``
+    also the dict that ``gated_scan_bwd`` takes (the states entering every
+    128 steps)."""
+    _check_inputs(x, g)
+    B, T, D = x.shape
+    dev = x.device
+    init = _check_state(initial_state, B, D, "initial_state")
+    h = torch.empty(B, T, D, dtype=x.dtype, device=dev)
+    final = torch.empty(B, D, dtype=torch.float32, device=dev) if output_final_state else None
+    carries = None
+    if return_aux:
+        carries = torch.empty(B, -(-T // _lib.SCAN_CHUNK), D, dtype=torch.float32, device=dev)
+    if h.numel() == 0:
+        if final is not None:
+            final.zero_() if init is None else final.copy_(init)
+    else:
+        a = _scan_args(x, g, init)
+        a.h = h.data_ptr()
+        a.final_state = final.data_ptr() if final is not None else None
+        a.carries = carries.data_ptr() if carries is not None else None
+        ws = _workspace(a, workspace, dev)
+        if ws is not None:
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        status = _DeviceStatus.get(dev)
+        a.status = status.word_ptr()
+        with _on_device(dev):
+            rc = _lib.load().ngdn2_scan(ctypes.byref(a), _stream(dev))
+        _raise_for(rc, "ngdn2_scan")
+        status.after_poisoning_launch()
+    return (h, final, dict(carries=carries)) if return_aux else (h, final)
+
+
+def gated_scan_bwd(x, g, dh, d_final=None, initial_state=None, aux=None, workspace=None):
+    """Gradients of ``sum(h * dh) + sum(final_state * d_final)``: returns
+    ``(dx, dg, d_initial)`` in the dtypes of x, g and initial_state
+    (``d_initial`` is None without an initial state). ``aux`` is the
+    forward's; without it the forward runs again."""
+    _check_inputs(x, g)
+    B, T, D = x.shape
+    dev = x.device
+    if dh.shape != x.shape:
+        raise ValueError(f"dh must be {tuple(x.shape)}, got {tuple(dh.shape)}")
+    _require_cuda(dh)
+    init = _check_state(initial_state, B, D, "initial_state")
+    dfin = _check_state(d_final, B, D, "d_final")
+    dx = torch.empty(B, T, D, dtype=x.dtype, device=dev)
+    dg = torch.empty(B, T, D, dtype=g.dtype, device=dev)
+    dinit = torch.empty(B, D, dtype=torch.float32, device=dev) if init is not None else None
+    if dx.numel() == 0:
+        if dinit is not None:
+            dinit.zero_() if dfin is None else dinit.copy_(dfin)
+    else:
+        carries = aux["carries"] if aux is not None else None
+        if carries is None:
+            carries = gated_scan_fwd(x, g, init, return_aux=True, workspace=workspace)[2]["carries"]
+        if (tuple(carries.shape) != (B, -(-T // _lib.SCAN_CHUNK), D)
+                or carries.dtype != torch.float32 or not carries.is_contiguous()):
+            raise ValueError("aux is not that of a forward of these shapes")
+        if dh.dtype != x.dtype:
+            dh = dh.to(x.dtype)
+        a = _lib.ScanBwdArgs()
+        a.abi_version = _lib.ABI_VERSION
+        fwd = _scan_args(x, g, init)
+        fwd.carries = carries.data_ptr()
+        ws = _workspace(fwd, workspace, dev)
+        if ws is not None:
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        a.fwd = fwd
+        _fill_tok(a, "d_h", dh, 3)
+        a.d_final = dfin.data_ptr() if dfin is not None else None
+        a.dx, a.dg = dx.data_ptr(), dg.data_ptr()
+        a.d_initial = dinit.data_ptr() if dinit is not None else None
+        status = _DeviceStatus.get(dev)
+        a.status = status.word_ptr()
+        with _on_device(dev):
+            rc = _lib.load().ngdn2_scan_bwd(ctypes.byref(a), _stream(dev))
+        _raise_for(rc, "ngdn2_scan_bwd")
+        status.after_poisoning_launch()
+    if dinit is not None and initial_state.dtype != torch.float32:
+        dinit = dinit.to(initial_state.dtype)
+    return dx, dg, dinit
+
+
+class GatedScanFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, g, initial_state, output_final_state):
+        h, final, aux = gated_scan_fwd(x, g, initial_state, output_final_state, return_aux=True)
+        ctx.save_for_backward(x, g, initial_state, aux["carries"])
+        return h, final
+
+    @staticmethod
+    def backward(ctx, dh, d_final):
+        x, g, init, carries = ctx.saved_tensors
+        if dh is None:
+            dh = torch.zeros((), dtype=x.dtype, device=x.device).expand(x.shape)
+        dx, dg, dinit = gated_scan_bwd(x, g, dh, d_final, init, dict(carries=carries))
+        return dx, dg, dinit, None
+
+
+def gated_scan(x, g, initial_state=None, output_final_state=False):
+    """``gated_scan_fwd`` with its gradient (``gated_scan_bwd``) in autograd:
+    returns ``(h, final_state)``."""
+    if not torch.is_grad_enabled() or not (
+            x.requires_grad or g.requires_grad
+            or (initial_state is not None and initial_state.requires_grad)):
+        return gated_scan_fwd(x, g, initial_state, output_final_state)
+    return GatedScanFunction.apply(x, g, initial_state, output_final_state)
+
+
+def step_gated_scan(x, g, state, *, out_state=None):
+    """One decode token: x, g [B, D], state [B, D]. Returns ``(h, state)``,
+    h [B, D] in x's dtype and the new state float32; ``out_state`` may be
+    ``state`` itself to update in place."""
+    if x.dim() != 2 or x.shape != g.shape:
+        raise ValueError(f"x and g must both be [B, D], got {tuple(x.shape)} and {tuple(g.shape)}")
+    _require_cuda(x, g, state)
+    B, D = x.shape
+    state = _check_state(state, B, D, "state")
+    new = torch.empty_like(state) if out_state is None else out_state
+    if out_state is not None and (tuple(new.shape) != (B, D) or new.dtype != torch.float32
+                                  or not new.is_contiguous()):
+        raise ValueError(f"out_state must be a contiguous float32 [{B}, {D}]")
+    h = torch.empty(B, D, dtype=x.dtype, device=x.device)
+    if h.numel() == 0:
+        return h, new
+    a = _lib.ScanStepArgs()
+    a.abi_version = _lib.ABI_VERSION
+    a.B, a.D = B, D
+    _fill_tok(a, "x", x, 2)
+    _fill_tok(a, "g", g, 2)
+    a.state_in, a.state_out, a.h = state.data_ptr(), new.data_ptr(), h.data_ptr()
+    with _on_device(x.device):
+        rc = _lib.load().ngdn2_scan_step(ctypes.byref(a), _stream(x.device))
+    _raise_for(rc, "ngdn2_scan_step")
+    return h, new
