@@ -6,8 +6,8 @@
 // the end: c_t = e^{g_t} (dh_t + c_{t+1}), c_{T+1} = d_final. States are fp32.
 //
 // Both are bound by memory: forward x, g -> h, backward x, g, dh -> dx, dg,
-// each byte moved once. A CTA takes a tile of steps x channels: every thread
-// a run of R steps of four channels, which it keeps in registers. A run maps the
+// each byte moved once. A CTA takes a tile of steps x channels into shared
+// memory, every thread a run of R steps of four channels. A run maps the
 // state that enters it to the one that leaves, s -> A s + H; runs are joined
 // within the warp by shuffles, across warps through shared memory, and
 // across tiles by a chain in global memory: a tile publishes its (A, H) as
@@ -37,14 +37,9 @@ constexpr uint32_t kPollLimit = 1u << 21;
 bool dtype_ok(int d) { return d == NGDN2_F32 || d == NGDN2_BF16 || d == NGDN2_F16; }
 
 // ---------------------------------------------------------------------------
-// Tiles: CL lanes of four channels by 256 / CL runs of R steps.
+// The chain of tiles. A tile is CL lanes of four channels by 256 / CL runs of R
+// steps.
 // ---------------------------------------------------------------------------
-
-template <int CL, int R>
-struct Tile {
-  static constexpr int kChannels = 4 * CL;
-  static constexpr int kSteps = kThreads / CL * R;
-};
 
 // Per-tile records of the chain, [strip][position] in chain order: a state
 // word (0 nothing, 1 (A, H) is there, 2 the leaving state too) and the
@@ -168,120 +163,176 @@ __device__ __forceinline__ void chain_state(const Chain& ch, int strip, int pos,
 }
 
 // ---------------------------------------------------------------------------
-// Four channels of one step. VEC: neighbouring, unit stride and aligned, one
-// vector access. Otherwise CL apart (so a warp's accesses stay together), each
-// by its own strides.
+// A tile of one tensor in shared memory, in its own type: runs of R rows (steps)
+// of the tile's channels. Runs are padded apart where rows are half of the
+// 128 bytes that the banks span, so that the two runs of a half warp's 8-byte
+// reads fall on different banks.
 // ---------------------------------------------------------------------------
 
-template <int DT, bool VEC, int CL>
-__device__ __forceinline__ void load4(const void* p, int64_t o, int64_t sd, int left, float* v) {
-  if constexpr (VEC) {
-    if (left <= 0) {
-      v[0] = v[1] = v[2] = v[3] = 0.f;
-    } else if constexpr (DT == NGDN2_F32) {
-      const float4 f = __ldg(reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + o));
-      v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-    } else {
-      const uint2 r = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(p) + o));
-      float2 a, b;
-      if constexpr (DT == NGDN2_BF16) {
-        a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.x));
-        b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.y));
-      } else {
-        a = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
-        b = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
-      }
-      v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = CL * i < left ? load_typed<DT>(p, o + CL * i * sd) : 0.f;
-  }
-}
-
-template <int DT, bool VEC, int CL>
-__device__ __forceinline__ void store4(void* p, int64_t o, int left, const float* v) {
-  if constexpr (VEC) {
-    if (left <= 0) return;
-    if constexpr (DT == NGDN2_F32) {
-      __stcs(reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + o),
-             make_float4(v[0], v[1], v[2], v[3]));
-    } else {
-      uint2 r;
-      if constexpr (DT == NGDN2_BF16) {
-        const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
-        r.x = *reinterpret_cast<const uint32_t*>(&a);
-        r.y = *reinterpret_cast<const uint32_t*>(&b);
-      } else {
-        const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
-        r.x = *reinterpret_cast<const uint32_t*>(&a);
-        r.y = *reinterpret_cast<const uint32_t*>(&b);
-      }
-      __stcs(reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p) + o), r);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (CL * i < left) store_elem(p, o + CL * i, v[i], DT);
-  }
-}
-
-// A thread's place in its tile: lane of channels, run of steps, its first
-// channel d and how many of the row's channels lie from there on, the
-// spacing of its four channels.
-template <int CL, bool VEC>
-struct Place {
-  int cl, run;
-  int64_t d;
-  int left;
-  static constexpr int kGap = VEC ? 1 : CL;
-  __device__ Place(int64_t d0, int64_t D) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    cl = lane % CL;
-    run = warp * (32 / CL) + lane / CL;
-    d = d0 + (VEC ? 4 * cl : cl);
-    left = D - d > 4 * CL ? 4 * CL : int(D - d);
-  }
-  // Tile-local index of channel i.
-  __device__ int ch(int i) const { return (VEC ? 4 * cl : cl) + kGap * i; }
+template <int DT, int CL, int R>
+struct Stage {
+  static constexpr int kEl = DT == NGDN2_F32 ? 4 : 2;
+  static constexpr int kRow = 4 * CL * kEl;
+  static constexpr int kRun = R * kRow + (kRow == 64 ? 64 : 0);
+  static constexpr int kSteps = kThreads / CL * R;
+  static constexpr int kBytes = kThreads / CL * kRun;
+  static __device__ __forceinline__ int at(int t) { return t / R * kRun + t % R * kRow; }
 };
 
+// Copies of G bytes at a time without registers in between (G = 16 or 4), zeros
+// for what lies outside [T, D]; G = 0 moves single elements of any stride.
+template <int G>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool ok) {
+  const uint32_t n = ok ? G : 0;
+  if constexpr (G == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+template <int DT, int CL, int R, int G>
+__device__ __forceinline__ void fill(unsigned char* sm, const void* p, const int64_t* st, int64_t b,
+                                     int64_t t0, int64_t d0, int64_t T, int64_t D) {
+  using S = Stage<DT, CL, R>;
+  const int64_t base = b * st[0] + t0 * st[1] + d0 * st[2];
+  if constexpr (G > 0) {
+    constexpr int kPer = S::kRow / G, kN = S::kSteps * kPer;
+    const char* src = static_cast<const char*>(p) + base * S::kEl;
+    const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(sm));
+#pragma unroll 4
+    for (int q = threadIdx.x; q < kN; q += kThreads) {
+      const int t = q / kPer, c = q % kPer * G;
+      const bool ok = t0 + t < T && d0 + c / S::kEl < D;
+      copy_async<G>(dst + S::at(t) + c, ok ? src + t * st[1] * S::kEl + c : p, ok);
+    }
+  } else {
+    using E = typename std::conditional<S::kEl == 4, uint32_t, uint16_t>::type;
+    const E* src = static_cast<const E*>(p) + base;
+#pragma unroll 8
+    for (int q = threadIdx.x; q < S::kSteps * 4 * CL; q += kThreads) {
+      const int t = q / (4 * CL), c = q % (4 * CL);
+      const bool ok = t0 + t < T && d0 + c < D;
+      *reinterpret_cast<E*>(sm + S::at(t) + c * S::kEl) = ok ? src[t * st[1] + c * st[2]] : E(0);
+    }
+  }
+}
+
+__device__ __forceinline__ void fill_done() {
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+}
+
+// Four neighbouring elements as fp32, and back (rounded once).
+template <int DT>
+__device__ __forceinline__ void get4(const void* p, float* v) {
+  if constexpr (DT == NGDN2_F32) {
+    const float4 f = *reinterpret_cast<const float4*>(p);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  } else {
+    const uint2 r = *reinterpret_cast<const uint2*>(p);
+    float2 a, b;
+    if constexpr (DT == NGDN2_BF16) {
+      a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.x));
+      b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&r.y));
+    } else {
+      a = __half22float2(*reinterpret_cast<const __half2*>(&r.x));
+      b = __half22float2(*reinterpret_cast<const __half2*>(&r.y));
+    }
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void put4(void* p, const float* v) {
+  if constexpr (DT == NGDN2_F32) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    uint2 r;
+    if constexpr (DT == NGDN2_BF16) {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+      r.x = *reinterpret_cast<const uint32_t*>(&a);
+      r.y = *reinterpret_cast<const uint32_t*>(&b);
+    } else {
+      const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+      r.x = *reinterpret_cast<const uint32_t*>(&a);
+      r.y = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    *reinterpret_cast<uint2*>(p) = r;
+  }
+}
+
+// A tile's rows from shared memory to a contiguous [B, T, D] output, element
+// by element with neighbouring threads on neighbouring channels: for widths
+// whose rows four-channel accesses cannot follow.
+template <int DT, int CL, int R>
+__device__ __forceinline__ void drain(const unsigned char* sm, void* out, int64_t b, int64_t t0,
+                                      int64_t d0, int64_t T, int64_t D) {
+  using S = Stage<DT, CL, R>;
+  using E = typename std::conditional<S::kEl == 4, uint32_t, uint16_t>::type;
+  E* dst = static_cast<E*>(out) + (b * T + t0) * D + d0;
+#pragma unroll 8
+  for (int q = threadIdx.x; q < S::kSteps * 4 * CL; q += kThreads) {
+    const int t = q / (4 * CL), c = q % (4 * CL);
+    if (t0 + t < T && d0 + c < D)
+      dst[t * D + c] = *reinterpret_cast<const E*>(sm + S::at(t) + c * S::kEl);
+  }
+}
+
+// Decays of a run's step: e^g, kept in g's place once computed where g is fp32.
+template <int GT>
+__device__ __forceinline__ void decay4(const void* p, bool first, float* e) {
+  get4<GT>(p, e);
+  if (first || GT != NGDN2_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = expf(e[i]);
+  }
+}
+
 // ---------------------------------------------------------------------------
-// Forward
+// Forward. G is the copy size of the fills (see fill); with G = 16 the outputs
+// go straight to memory, four channels at a time, else through the stage.
 // ---------------------------------------------------------------------------
 
-template <int XT, int GT, bool VEC, int CL, int R>
-__global__ void __launch_bounds__(kThreads) scan_kernel(ngdn2_scan_args a, Chain chain, int row_strips) {
-  using TL = Tile<CL, R>;
-  constexpr int kCh = TL::kChannels, NV = kCh / 32;
+template <int XT, int GT, int CL, int R>
+constexpr int fwd_smem() {
+  return Stage<XT, CL, R>::kBytes + Stage<GT, CL, R>::kBytes;
+}
+
+template <int XT, int GT, int G, int CL, int R>
+__global__ void __launch_bounds__(kThreads, 4)
+scan_kernel(const __grid_constant__ ngdn2_scan_args a, Chain chain, int row_strips) {
+  constexpr int kCh = 4 * CL, NV = kCh / 32, kSteps = kThreads / CL * R;
+  using SX = Stage<XT, CL, R>;
+  using SG = Stage<GT, CL, R>;
+  extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float2 part[kWarps][kCh];  // the warps' maps
   __shared__ float enter[kWarps][kCh];  // the state entering each warp's runs
   int strip, pos;
   take_tile(chain, &strip, &pos);
   const int64_t b = strip / row_strips, d0 = int64_t(strip % row_strips) * kCh;
-  const Place<CL, VEC> me(d0, a.D);
+  const int64_t t0 = int64_t(pos) * kSteps;
+  unsigned char *sx = smem, *sg = smem + SX::kBytes;
+  fill<XT, CL, R, G>(sx, a.x, a.x_stride, b, t0, d0, a.T, a.D);
+  fill<GT, CL, R, G>(sg, a.g, a.g_stride, b, t0, d0, a.T, a.D);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t0 = int64_t(pos) * TL::kSteps + me.run * R;
+  const int c = 4 * (lane % CL), run = threadIdx.x / CL;
+  unsigned char *mx = sx + run * SX::kRun + c * SX::kEl, *mg = sg + run * SG::kRun + c * SG::kEl;
+  fill_done();
 
-  float x[R][4], e[R][4];
-  const int64_t xo = b * a.x_stride[0] + t0 * a.x_stride[1] + me.d * a.x_stride[2];
-  const int64_t go = b * a.g_stride[0] + t0 * a.g_stride[1] + me.d * a.g_stride[2];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int left = t0 + r < a.T ? me.left : 0;
-    load4<XT, VEC, CL>(a.x, xo + r * a.x_stride[1], a.x_stride[2], left, x[r]);
-    load4<GT, VEC, CL>(a.g, go + r * a.g_stride[1], a.g_stride[2], left, e[r]);
-  }
-  // Past the end x = g = 0: the identity.
+  // The run's map. Past the end x = g = 0: the identity.
   float A[4] = {1.f, 1.f, 1.f, 1.f}, H[4] = {};
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int r = 0; r < R; ++r) {
+    float x[4], e[4];
+    get4<XT>(mx + r * SX::kRow, x);
+    decay4<GT>(mg + r * SG::kRow, true, e);
+    if (GT == NGDN2_F32) put4<NGDN2_F32>(mg + r * SG::kRow, e);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      e[r][i] = expf(e[r][i]);
-      A[i] *= e[r][i];
-      H[i] = fmaf(e[r][i], H[i], x[r][i]);
+      A[i] *= e[i];
+      H[i] = fmaf(e[i], H[i], x[i]);
     }
+  }
   // Within the warp: the maps of all runs up to this one, then up to the
   // one before.
 #pragma unroll
@@ -296,7 +347,7 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ngdn2_scan_args a, Chain
     }
   if (lane >= 32 - CL) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part[warp][me.ch(i)] = make_float2(A[i], H[i]);
+    for (int i = 0; i < 4; ++i) part[warp][c + i] = make_float2(A[i], H[i]);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -310,13 +361,13 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ngdn2_scan_args a, Chain
     float ta[NV], th[NV], first[NV], s[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = lane + 32 * i;
-      first[i] = a.initial_state && d0 + c < a.D ? a.initial_state[b * a.D + d0 + c] : 0.f;
+      const int ch = lane + 32 * i;
+      first[i] = a.initial_state && d0 + ch < a.D ? a.initial_state[b * a.D + d0 + ch] : 0.f;
       ta[i] = 1.f;
       th[i] = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float2 m = part[w][c];
+        const float2 m = part[w][ch];
         th[i] = fmaf(m.x, th[i], m.y);
         ta[i] *= m.x;
       }
@@ -324,30 +375,42 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ngdn2_scan_args a, Chain
     chain_state<NV>(chain, strip, pos, ta, th, first, s, a.status);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = lane + 32 * i;
+      const int ch = lane + 32 * i;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        enter[w][c] = s[i];
-        s[i] = fmaf(part[w][c].x, s[i], part[w][c].y);
+        enter[w][ch] = s[i];
+        s[i] = fmaf(part[w][ch].x, s[i], part[w][ch].y);
       }
-      if (a.final_state && (int64_t(pos) + 1) * TL::kSteps >= a.T && d0 + c < a.D)
-        a.final_state[b * a.D + d0 + c] = s[i];
+      if (a.final_state && t0 + kSteps >= a.T && d0 + ch < a.D)
+        a.final_state[b * a.D + d0 + ch] = s[i];
     }
   }
   __syncthreads();
   float h[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = fmaf(A[i], enter[warp][me.ch(i)], H[i]);
-  if (a.carries && t0 % NGDN2_SCAN_CHUNK == 0 && t0 < a.T) {
+  for (int i = 0; i < 4; ++i) h[i] = fmaf(A[i], enter[warp][c + i], H[i]);
+  const int64_t t1 = t0 + run * R, d = d0 + c;
+  if (a.carries && t1 % NGDN2_SCAN_CHUNK == 0 && t1 < a.T) {
     const int64_t NC = (a.T + NGDN2_SCAN_CHUNK - 1) / NGDN2_SCAN_CHUNK;
-    store4<NGDN2_F32, VEC, CL>(a.carries, (b * NC + t0 / NGDN2_SCAN_CHUNK) * a.D + me.d, me.left, h);
+    float* to = a.carries + (b * NC + t1 / NGDN2_SCAN_CHUNK) * a.D + d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (d + i < a.D) to[i] = h[i];
   }
-  const int64_t ho = (b * a.T + t0) * a.D + me.d;
+  unsigned char* out = static_cast<unsigned char*>(a.h) + ((b * a.T + t1) * a.D + d) * SX::kEl;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
+    float x[4], e[4];
+    get4<XT>(mx + r * SX::kRow, x);
+    decay4<GT>(mg + r * SG::kRow, false, e);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = fmaf(e[r][i], h[i], x[r][i]);
-    if (t0 + r < a.T) store4<XT, VEC, CL>(a.h, ho + r * a.D, me.left, h);
+    for (int i = 0; i < 4; ++i) h[i] = fmaf(e[i], h[i], x[i]);
+    if (G != 16) put4<XT>(mx + r * SX::kRow, h);
+    else if (t1 + r < a.T && d < a.D) put4<XT>(out + r * a.D * SX::kEl, h);
+  }
+  if (G != 16) {
+    __syncthreads();
+    drain<XT, CL, R>(sx, a.h, b, t0, d0, a.T, a.D);
   }
 }
 
@@ -356,47 +419,59 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(ngdn2_scan_args a, Chain
 // the gradients from the chain that runs from the end.
 // ---------------------------------------------------------------------------
 
-template <int XT, int GT, bool VEC, int CL, int R>
-__global__ void __launch_bounds__(kThreads)
-scan_bwd_kernel(ngdn2_scan_bwd_args p, Chain chain, int row_strips) {
-  using TL = Tile<CL, R>;
-  constexpr int kCh = TL::kChannels, NV = kCh / 32;
-  static_assert(TL::kSteps <= NGDN2_SCAN_CHUNK && NGDN2_SCAN_CHUNK % TL::kSteps == 0, "");
+template <int XT, int GT, int CL, int R>
+constexpr int bwd_smem() {
+  return 2 * Stage<XT, CL, R>::kBytes + Stage<GT, CL, R>::kBytes;
+}
+
+template <int XT, int GT, int G, int CL, int R>
+__global__ void __launch_bounds__(kThreads, 2)
+scan_bwd_kernel(const __grid_constant__ ngdn2_scan_bwd_args p, Chain chain, int row_strips) {
+  constexpr int kCh = 4 * CL, NV = kCh / 32, kSteps = kThreads / CL * R;
+  static_assert(NGDN2_SCAN_CHUNK % kSteps == 0, "a tile starts at a state that the forward left, or within its chunk as the only tile");
+  using SX = Stage<XT, CL, R>;
+  using SG = Stage<GT, CL, R>;
   const ngdn2_scan_args& a = p.fwd;
+  extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float2 part_h[kWarps][kCh], part_c[kWarps][kCh];
   __shared__ float enter_h[kWarps][kCh], enter_c[kWarps][kCh];
   int strip, pos;
   take_tile(chain, &strip, &pos);
   const int64_t b = strip / row_strips, d0 = int64_t(strip % row_strips) * kCh;
-  const int64_t tile = chain.tiles - 1 - pos;
-  const Place<CL, VEC> me(d0, a.D);
+  const int64_t tile = chain.tiles - 1 - pos, t0 = tile * kSteps;
+  unsigned char *sx = smem, *sd = smem + SX::kBytes, *sg = smem + 2 * SX::kBytes;
+  fill<XT, CL, R, G>(sx, a.x, a.x_stride, b, t0, d0, a.T, a.D);
+  fill<GT, CL, R, G>(sg, a.g, a.g_stride, b, t0, d0, a.T, a.D);
+  fill<XT, CL, R, G>(sd, p.d_h, p.d_h_stride, b, t0, d0, a.T, a.D);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t t0 = tile * TL::kSteps + me.run * R;
+  const int c = 4 * (lane % CL), run = threadIdx.x / CL;
+  unsigned char *mx = sx + run * SX::kRun + c * SX::kEl, *md = sd + run * SX::kRun + c * SX::kEl,
+                *mg = sg + run * SG::kRun + c * SG::kEl;
+  fill_done();
 
-  float x[R][4], e[R][4], dh[R][4];
-  const int64_t xo = b * a.x_stride[0] + t0 * a.x_stride[1] + me.d * a.x_stride[2];
-  const int64_t go = b * a.g_stride[0] + t0 * a.g_stride[1] + me.d * a.g_stride[2];
-  const int64_t dho = b * p.d_h_stride[0] + t0 * p.d_h_stride[1] + me.d * p.d_h_stride[2];
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int left = t0 + r < a.T ? me.left : 0;
-    load4<XT, VEC, CL>(a.x, xo + r * a.x_stride[1], a.x_stride[2], left, x[r]);
-    load4<GT, VEC, CL>(a.g, go + r * a.g_stride[1], a.g_stride[2], left, e[r]);
-    load4<XT, VEC, CL>(p.d_h, dho + r * p.d_h_stride[1], p.d_h_stride[2], left, dh[r]);
-  }
   float Ah[4] = {1.f, 1.f, 1.f, 1.f}, H[4] = {}, Ac[4], C[4] = {};
+  {
+    float e[R][4];
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+      float x[4];
+      get4<XT>(mx + r * SX::kRow, x);
+      decay4<GT>(mg + r * SG::kRow, true, e[r]);
+      if (GT == NGDN2_F32) put4<NGDN2_F32>(mg + r * SG::kRow, e[r]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      e[r][i] = expf(e[r][i]);
-      Ah[i] *= e[r][i];
-      H[i] = fmaf(e[r][i], H[i], x[r][i]);
+      for (int i = 0; i < 4; ++i) {
+        Ah[i] *= e[r][i];
+        H[i] = fmaf(e[r][i], H[i], x[i]);
+      }
     }
 #pragma unroll
-  for (int r = R - 1; r >= 0; --r)
+    for (int r = R - 1; r >= 0; --r) {
+      float dh[4];
+      get4<XT>(md + r * SX::kRow, dh);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) C[i] = e[r][i] * (dh[r][i] + C[i]);
+      for (int i = 0; i < 4; ++i) C[i] = e[r][i] * (dh[i] + C[i]);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) Ac[i] = Ah[i];
 #pragma unroll
@@ -416,11 +491,11 @@ scan_bwd_kernel(ngdn2_scan_bwd_args p, Chain chain, int row_strips) {
     }
   if (lane >= 32 - CL) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part_h[warp][me.ch(i)] = make_float2(Ah[i], H[i]);
+    for (int i = 0; i < 4; ++i) part_h[warp][c + i] = make_float2(Ah[i], H[i]);
   }
   if (lane < CL) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part_c[warp][me.ch(i)] = make_float2(Ac[i], C[i]);
+    for (int i = 0; i < 4; ++i) part_c[warp][c + i] = make_float2(Ac[i], C[i]);
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -438,13 +513,13 @@ scan_bwd_kernel(ngdn2_scan_bwd_args p, Chain chain, int row_strips) {
     float ta[NV], tc[NV], first[NV], s[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = lane + 32 * i;
-      first[i] = p.d_final && d0 + c < a.D ? p.d_final[b * a.D + d0 + c] : 0.f;
+      const int ch = lane + 32 * i;
+      first[i] = p.d_final && d0 + ch < a.D ? p.d_final[b * a.D + d0 + ch] : 0.f;
       ta[i] = 1.f;
       tc[i] = 0.f;
 #pragma unroll
       for (int w = kWarps - 1; w >= 0; --w) {
-        const float2 m = part_c[w][c];
+        const float2 m = part_c[w][ch];
         tc[i] = fmaf(m.x, tc[i], m.y);
         ta[i] *= m.x;
       }
@@ -452,58 +527,68 @@ scan_bwd_kernel(ngdn2_scan_bwd_args p, Chain chain, int row_strips) {
     chain_state<NV>(chain, strip, pos, ta, tc, first, s, p.status);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = lane + 32 * i;
+      const int ch = lane + 32 * i;
 #pragma unroll
       for (int w = kWarps - 1; w >= 0; --w) {
-        enter_c[w][c] = s[i];
-        s[i] = fmaf(part_c[w][c].x, s[i], part_c[w][c].y);
+        enter_c[w][ch] = s[i];
+        s[i] = fmaf(part_c[w][ch].x, s[i], part_c[w][ch].y);
       }
-      if (p.d_initial && tile == 0 && d0 + c < a.D) p.d_initial[b * a.D + d0 + c] = s[i];
+      if (p.d_initial && tile == 0 && d0 + ch < a.D) p.d_initial[b * a.D + d0 + ch] = s[i];
     }
   } else if (warp == 1) {
     const int64_t NC = (a.T + NGDN2_SCAN_CHUNK - 1) / NGDN2_SCAN_CHUNK;
-    const int64_t chunk = tile * TL::kSteps / NGDN2_SCAN_CHUNK;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = lane + 32 * i;
-      float s = d0 + c < a.D ? a.carries[(b * NC + chunk) * a.D + d0 + c] : 0.f;
+      const int ch = lane + 32 * i;
+      float s = d0 + ch < a.D ? a.carries[(b * NC + t0 / NGDN2_SCAN_CHUNK) * a.D + d0 + ch] : 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        enter_h[w][c] = s;
-        s = fmaf(part_h[w][c].x, s, part_h[w][c].y);
+        enter_h[w][ch] = s;
+        s = fmaf(part_h[w][ch].x, s, part_h[w][ch].y);
       }
     }
   }
   __syncthreads();
-  float h[4], c[4];
+  float h[R][4], cc[4];  // h[r]: the state before step r
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    h[i] = fmaf(Ah[i], enter_h[warp][me.ch(i)], H[i]);
-    c[i] = fmaf(Ac[i], enter_c[warp][me.ch(i)], C[i]);
+    h[0][i] = fmaf(Ah[i], enter_h[warp][c + i], H[i]);
+    cc[i] = fmaf(Ac[i], enter_c[warp][c + i], C[i]);
   }
-  // x[r] becomes the state before step r.
 #pragma unroll
-  for (int r = 0; r < R; ++r)
+  for (int r = 0; r + 1 < R; ++r) {
+    float x[4], e[4];
+    get4<XT>(mx + r * SX::kRow, x);
+    decay4<GT>(mg + r * SG::kRow, false, e);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float next = fmaf(e[r][i], h[i], x[r][i]);
-      x[r][i] = h[i];
-      h[i] = next;
-    }
-  const int64_t o = (b * a.T + t0) * a.D + me.d;
+    for (int i = 0; i < 4; ++i) h[r + 1][i] = fmaf(e[i], h[r][i], x[i]);
+  }
+  const int64_t t1 = t0 + run * R, d = d0 + c, o = (b * a.T + t1) * a.D + d;
+  unsigned char *ox = static_cast<unsigned char*>(p.dx) + o * SX::kEl,
+                *og = static_cast<unsigned char*>(p.dg) + o * SG::kEl;
 #pragma unroll
   for (int r = R - 1; r >= 0; --r) {
-    float u[4], dg[4];
+    float u[4], e[4], dg[4];
+    get4<XT>(md + r * SX::kRow, u);
+    decay4<GT>(mg + r * SG::kRow, false, e);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      u[i] = dh[r][i] + c[i];
-      c[i] = e[r][i] * u[i];
-      dg[i] = c[i] * x[r][i];
+      u[i] += cc[i];
+      cc[i] = e[i] * u[i];
+      dg[i] = cc[i] * h[r][i];
     }
-    if (t0 + r < a.T) {
-      store4<XT, VEC, CL>(p.dx, o + r * a.D, me.left, u);
-      store4<GT, VEC, CL>(p.dg, o + r * a.D, me.left, dg);
+    if (G != 16) {
+      put4<XT>(md + r * SX::kRow, u);
+      put4<GT>(mg + r * SG::kRow, dg);
+    } else if (t1 + r < a.T && d < a.D) {
+      put4<XT>(ox + r * a.D * SX::kEl, u);
+      put4<GT>(og + r * a.D * SG::kEl, dg);
     }
+  }
+  if (G != 16) {
+    __syncthreads();
+    drain<XT, CL, R>(sd, p.dx, b, t0, d0, a.T, a.D);
+    drain<GT, CL, R>(sg, p.dg, b, t0, d0, a.T, a.D);
   }
 }
 
@@ -522,13 +607,25 @@ __global__ void __launch_bounds__(128) scan_step_kernel(ngdn2_scan_step_args a) 
 // Choice of tile and launch
 // ---------------------------------------------------------------------------
 
-bool vec_ok(const void* p, int dt, const int64_t* st, int64_t D) {
-  const int64_t bytes = dt == NGDN2_F32 ? 16 : 8;
-  return st[2] == 1 && D % 4 == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 &&
-         reinterpret_cast<uintptr_t>(p) % bytes == 0;
+// The largest copy that every row of a [B, T, D] view allows: 16 or 4 bytes,
+// or 0 for element by element.
+int granule(const void* p, int dt, const int64_t* st, int64_t D) {
+  const int64_t el = dt == NGDN2_F32 ? 4 : 2;
+  if (st[2] != 1) return 0;
+  const uintptr_t all = reinterpret_cast<uintptr_t>(p) | uintptr_t(st[0] * el) | uintptr_t(st[1] * el) |
+                        uintptr_t(D * el);
+  return all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 0;
 }
 
-bool out_ok(const void* p, int dt) { return reinterpret_cast<uintptr_t>(p) % (dt == NGDN2_F32 ? 16 : 8) == 0; }
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+template <class K, class... Args>
+cudaError_t launch(K kernel, int64_t grid, int smem, cudaStream_t st, const Args&... args) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
+  kernel<<<unsigned(grid), kThreads, smem, st>>>(args...);
+  return cudaGetLastError();
+}
 
 template <class F>
 cudaError_t by_types(int xt, int gt, F&& f) {
@@ -549,20 +646,34 @@ cudaError_t by_types(int xt, int gt, F&& f) {
 // The narrow tile (32 channels) leaves the long axis in few, long tiles, so
 // that the chain is short; the wide one (128 channels) is for sequences of
 // at most its 32 steps, whose narrow tiles would be mostly empty.
-constexpr int kFwdSteps = Tile<8, 8>::kSteps, kBwdSteps = Tile<8, 4>::kSteps;
-constexpr int kWideSteps = Tile<32, 4>::kSteps;
+constexpr int kNarrowR = 8, kNarrowSteps = kThreads / 8 * kNarrowR;
+constexpr int kWideR = 4, kWideSteps = kThreads / 32 * kWideR;
+
+template <class F>
+cudaError_t by_tile(int channels, int granule, F&& f) {
+  auto g = [&](auto CL, auto R) {
+    switch (granule) {
+      case 16: return f(std::integral_constant<int, 16>{}, CL, R);
+      case 4: return f(std::integral_constant<int, 4>{}, CL, R);
+      default: return f(std::integral_constant<int, 0>{}, CL, R);
+    }
+  };
+  return channels == 128
+             ? g(std::integral_constant<int, 32>{}, std::integral_constant<int, kWideR>{})
+             : g(std::integral_constant<int, 8>{}, std::integral_constant<int, kNarrowR>{});
+}
 
 struct Shape {
   int row_strips, channels;
   int64_t strips, tiles;
 };
 
-Shape shape_of(const ngdn2_scan_args* a, int steps) {
+Shape shape_of(const ngdn2_scan_args* a) {
   Shape s;
   s.channels = a->T <= kWideSteps ? 128 : 32;
   s.row_strips = int((a->D + s.channels - 1) / s.channels);
   s.strips = int64_t(a->B) * s.row_strips;
-  s.tiles = a->T <= kWideSteps ? 1 : (a->T + steps - 1) / steps;
+  s.tiles = a->T <= kWideSteps ? 1 : (a->T + kNarrowSteps - 1) / kNarrowSteps;
   return s;
 }
 
@@ -573,7 +684,7 @@ int validate_scan(const ngdn2_scan_args* a, bool outputs) {
   // The strips of all tiles are counted in 31 bits.
   if (a->B < 1 || a->T < 1 || a->D < 1 || a->T >= (int64_t(1) << 31) ||
       a->D >= (int64_t(1) << 31) ||
-      (a->D + 31) / 32 * ((a->T + kBwdSteps - 1) / kBwdSteps) > ((int64_t(1) << 31) - 1) / a->B)
+      (a->D + 31) / 32 * ((a->T + kNarrowSteps - 1) / kNarrowSteps) > ((int64_t(1) << 31) - 1) / a->B)
     return NGDN2_ERR_SHAPE;
   if (!a->x || !a->g || (outputs && (!a->h || !a->status))) return NGDN2_ERR_NULL;
   return NGDN2_OK;
@@ -587,13 +698,6 @@ int validate_scan_bwd(const ngdn2_scan_bwd_args* a) {
   if (a->d_h_dtype != a->fwd.x_dtype) return NGDN2_ERR_DTYPE;
   if (!a->fwd.carries || !a->d_h || !a->dx || !a->dg || !a->status) return NGDN2_ERR_NULL;
   return NGDN2_OK;
-}
-
-size_t workspace_bytes(const ngdn2_scan_args* a) {
-  const Shape f = shape_of(a, kFwdSteps), b = shape_of(a, kBwdSteps);
-  const size_t x = chain_bytes(f.strips, f.tiles, f.channels),
-               y = chain_bytes(b.strips, b.tiles, b.channels);
-  return x > y ? x : y;
 }
 
 // The chain of one launch, its counter and state words cleared.
@@ -618,7 +722,8 @@ NGDN2_API int ngdn2_scan_workspace_size(const ngdn2_scan_args* a, size_t* bytes)
   const int rc = validate_scan(a, false);
   if (rc != NGDN2_OK) return rc;
   if (!bytes) return NGDN2_ERR_NULL;
-  *bytes = workspace_bytes(a);
+  const Shape s = shape_of(a);
+  *bytes = chain_bytes(s.strips, s.tiles, s.channels);
   return NGDN2_OK;
 }
 
@@ -626,24 +731,21 @@ NGDN2_API int ngdn2_scan(const ngdn2_scan_args* a, void* stream) {
   int rc = validate_scan(a, true);
   if (rc != NGDN2_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const Shape s = shape_of(a, kFwdSteps);
+  const Shape s = shape_of(a);
   Chain chain;
   rc = start_chain(s, a->workspace, a->workspace_bytes, st, &chain);
   if (rc != NGDN2_OK) return rc;
-  const bool vec = vec_ok(a->x, a->x_dtype, a->x_stride, a->D) &&
-                   vec_ok(a->g, a->g_dtype, a->g_stride, a->D) && out_ok(a->h, a->x_dtype) &&
-                   out_ok(a->carries, NGDN2_F32);
-  const unsigned grid = unsigned(s.strips * s.tiles);
-  const cudaError_t err = by_types(a->x_dtype, a->g_dtype, [&](auto X, auto G) {
-    constexpr int XT = decltype(X)::value, GT = decltype(G)::value;
-    if (s.channels == 128) {
-      if (vec) scan_kernel<XT, GT, true, 32, 4><<<grid, kThreads, 0, st>>>(*a, chain, s.row_strips);
-      else scan_kernel<XT, GT, false, 32, 4><<<grid, kThreads, 0, st>>>(*a, chain, s.row_strips);
-    } else {
-      if (vec) scan_kernel<XT, GT, true, 8, 8><<<grid, kThreads, 0, st>>>(*a, chain, s.row_strips);
-      else scan_kernel<XT, GT, false, 8, 8><<<grid, kThreads, 0, st>>>(*a, chain, s.row_strips);
-    }
-    return cudaGetLastError();
+  int g = granule(a->x, a->x_dtype, a->x_stride, a->D);
+  const int g2 = granule(a->g, a->g_dtype, a->g_stride, a->D);
+  g = g2 < g ? g2 : g;
+  if (g == 16 && !aligned16(a->h)) g = 4;
+  const cudaError_t err = by_types(a->x_dtype, a->g_dtype, [&](auto X, auto Gt) {
+    constexpr int XT = decltype(X)::value, GT = decltype(Gt)::value;
+    return by_tile(s.channels, g, [&](auto GR, auto CLc, auto Rc) {
+      constexpr int G = decltype(GR)::value, CL = decltype(CLc)::value, R = decltype(Rc)::value;
+      return launch(scan_kernel<XT, GT, G, CL, R>, s.strips * s.tiles, fwd_smem<XT, GT, CL, R>(), st,
+                    *a, chain, s.row_strips);
+    });
   });
   return err == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
 }
@@ -653,25 +755,22 @@ NGDN2_API int ngdn2_scan_bwd(const ngdn2_scan_bwd_args* p, void* stream) {
   if (rc != NGDN2_OK) return rc;
   const ngdn2_scan_args* a = &p->fwd;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const Shape s = shape_of(a, kBwdSteps);
+  const Shape s = shape_of(a);
   Chain chain;
   rc = start_chain(s, p->workspace, p->workspace_bytes, st, &chain);
   if (rc != NGDN2_OK) return rc;
-  const bool vec = vec_ok(a->x, a->x_dtype, a->x_stride, a->D) &&
-                   vec_ok(a->g, a->g_dtype, a->g_stride, a->D) &&
-                   vec_ok(p->d_h, p->d_h_dtype, p->d_h_stride, a->D) && out_ok(p->dx, a->x_dtype) &&
-                   out_ok(p->dg, a->g_dtype);
-  const unsigned grid = unsigned(s.strips * s.tiles);
-  const cudaError_t err = by_types(a->x_dtype, a->g_dtype, [&](auto X, auto G) {
-    constexpr int XT = decltype(X)::value, GT = decltype(G)::value;
-    if (s.channels == 128) {
-      if (vec) scan_bwd_kernel<XT, GT, true, 32, 4><<<grid, kThreads, 0, st>>>(*p, chain, s.row_strips);
-      else scan_bwd_kernel<XT, GT, false, 32, 4><<<grid, kThreads, 0, st>>>(*p, chain, s.row_strips);
-    } else {
-      if (vec) scan_bwd_kernel<XT, GT, true, 8, 4><<<grid, kThreads, 0, st>>>(*p, chain, s.row_strips);
-      else scan_bwd_kernel<XT, GT, false, 8, 4><<<grid, kThreads, 0, st>>>(*p, chain, s.row_strips);
-    }
-    return cudaGetLastError();
+  int g = granule(a->x, a->x_dtype, a->x_stride, a->D);
+  for (const int o : {granule(a->g, a->g_dtype, a->g_stride, a->D),
+                      granule(p->d_h, p->d_h_dtype, p->d_h_stride, a->D)})
+    g = o < g ? o : g;
+  if (g == 16 && (!aligned16(p->dx) || !aligned16(p->dg))) g = 4;
+  const cudaError_t err = by_types(a->x_dtype, a->g_dtype, [&](auto X, auto Gt) {
+    constexpr int XT = decltype(X)::value, GT = decltype(Gt)::value;
+    return by_tile(s.channels, g, [&](auto GR, auto CLc, auto Rc) {
+      constexpr int G = decltype(GR)::value, CL = decltype(CLc)::value, R = decltype(Rc)::value;
+      return launch(scan_bwd_kernel<XT, GT, G, CL, R>, s.strips * s.tiles,
+                    bwd_smem<XT, GT, CL, R>(), st, *p, chain, s.row_strips);
+    });
   });
   return err == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
 }
