@@ -10,9 +10,9 @@
 // memory, every thread a run of R steps of four channels. A run maps the
 // state that enters it to the one that leaves, s -> A s + H; runs are joined
 // within the warp by shuffles, across warps through shared memory, and
-// across tiles by a chain in global memory: a tile publishes its (A, H) as
-// soon as it has them, then looks back for the nearest tile whose leaving
-// state is known and applies the (A, H) of those in between in order. That is
+// across tiles by a chain in global memory: a tile posts its (A, H), looks
+// back for the nearest tile whose leaving state is there, applies the (A, H) of
+// those in between in order, and posts its own leaving state. That is
 // the same sequence of operations however far it has to look, so the result
 // does not depend on timing. Tiles are handed out in chain order by a
 // counter, so a tile only waits for tiles that already run; the wait is
@@ -41,125 +41,103 @@ bool dtype_ok(int d) { return d == NGDN2_F32 || d == NGDN2_BF16 || d == NGDN2_F1
 // steps.
 // ---------------------------------------------------------------------------
 
-// Per-tile records of the chain, [strip][position] in chain order: a state
-// word (0 nothing, 1 (A, H) is there, 2 the leaving state too) and the
-// values for the tile's channels.
+// Per-tile records of the chain, [strip][position][channel] in chain order: a
+// tile's map (A, H) and the state that leaves it. All bits set means "not
+// there yet": the arithmetic that makes these values never does. So each value
+// tells by itself whether it is there, and needs no flag and no fence.
+constexpr int kChainCh = 32;
+constexpr uint32_t kNotYet = 0xffffffffu;
+
 struct Chain {
-  uint32_t* ticket;
-  uint32_t* flag;
-  float2* agg;
-  float* inc;
+  uint64_t* map;
+  uint32_t* state;
+  uint32_t* ticket;  // one more than the tiles handed out, so that it starts as kNotYet
   int64_t strips;
   int tiles;
 };
 
-size_t chain_flag_bytes(int64_t strips, int64_t tiles) {
-  return size_t((strips * tiles + 1) * 4 + 255) & ~size_t(255);
+size_t chain_words(int64_t strips, int64_t tiles) { return size_t(strips) * tiles * kChainCh; }
+
+size_t chain_bytes(int64_t strips, int64_t tiles) {
+  return tiles < 2 ? 0 : 16 + chain_words(strips, tiles) * 12 + 4;
 }
 
-size_t chain_bytes(int64_t strips, int64_t tiles, int channels) {
-  return tiles < 2 ? 0 : 256 + chain_flag_bytes(strips, tiles) +
-                             size_t(strips) * tiles * channels * (sizeof(float2) + sizeof(float));
-}
-
-Chain make_chain(void* ws, int64_t strips, int64_t tiles, int channels) {
+Chain make_chain(void* ws, int64_t strips, int64_t tiles) {
   Chain c{};
   c.strips = strips;
   c.tiles = int(tiles);
   if (tiles < 2) return c;
-  char* p = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(ws) + 255) & ~uintptr_t(255));
-  c.ticket = reinterpret_cast<uint32_t*>(p);
-  c.flag = c.ticket + 1;
-  p += chain_flag_bytes(strips, tiles);
-  c.agg = reinterpret_cast<float2*>(p);
-  c.inc = reinterpret_cast<float*>(p + size_t(strips) * tiles * channels * sizeof(float2));
+  c.map = reinterpret_cast<uint64_t*>((reinterpret_cast<uintptr_t>(ws) + 15) & ~uintptr_t(15));
+  c.state = reinterpret_cast<uint32_t*>(c.map + chain_words(strips, tiles));
+  c.ticket = c.state + chain_words(strips, tiles);
   return c;
 }
 
-__device__ __forceinline__ uint32_t load_acquire(const uint32_t* p) {
+__device__ __forceinline__ uint32_t peek(const uint32_t* p) {
   uint32_t v;
-  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
   return v;
 }
-__device__ __forceinline__ void store_release(uint32_t* p, uint32_t v) {
-  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+__device__ __forceinline__ uint64_t peek(const uint64_t* p) {
+  uint64_t v;
+  asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void post(uint32_t* p, float v) {
+  asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(__float_as_uint(v)) : "memory");
+}
+__device__ __forceinline__ void post(uint64_t* p, float A, float H) {
+  const uint64_t v = uint64_t(__float_as_uint(H)) << 32 | __float_as_uint(A);
+  asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
 }
 
-// Which tile this CTA takes: position in its chain and strip of channels.
-// Positions of all strips in turn, by the counter (a lone position needs none).
-__device__ __forceinline__ void take_tile(const Chain& ch, int* strip, int* pos) {
-  __shared__ uint32_t ticket;
-  if (ch.tiles < 2) {
-    *strip = int(blockIdx.x);
-    *pos = 0;
-    return;
-  }
-  if (threadIdx.x == 0) ticket = atomicAdd(ch.ticket, 1u);
-  __syncthreads();
-  *strip = int(ticket % uint32_t(ch.strips));
-  *pos = int(ticket / uint32_t(ch.strips));
+// Tiles are handed out in chain order, positions of all strips in turn, to
+// CTAs that stay. A CTA asks for its next tile when the state entering this
+// one is known: earlier, and the tile would hold up its chain until this one
+// is done (1 x 65536 x 1024: 199 us when asked for right after the loads). A lone
+// position needs no counter: its tiles go round.
+__device__ __forceinline__ uint32_t ask_tile(const Chain& ch, uint32_t last) {
+  return ch.tiles < 2 ? last + gridDim.x : atomicAdd(ch.ticket, 1u) + 1u;
 }
 
-// The state entering tile ``pos`` for NV channels a lane (channel lane +
-// 32 i), whose own map is (A, H); publishes the map and the leaving state.
-// ``first`` is the state that enters position 0. One whole warp.
-template <int NV>
-__device__ __forceinline__ void chain_state(const Chain& ch, int strip, int pos, const float* A,
-                                            const float* H, const float* first, float* s,
-                                            int32_t* status) {
-  constexpr int kCh = 32 * NV;
+// The state entering tile ``pos`` > 0 for the lane's channel, whose own map is
+// (A, H). One whole warp. The nearest of the kBack tiles before this one whose
+// leaving state is there, and the maps of those in between, in order.
+constexpr int kBack = 8;
+
+__device__ __forceinline__ float chain_state(const Chain& ch, int64_t at, int pos, float A, float H,
+                                             int32_t* status) {
   const int lane = threadIdx.x & 31;
-  const int64_t at = int64_t(strip) * ch.tiles + pos;
-  if (pos == 0) {
+  const uint64_t* map = ch.map + at * kChainCh + lane;
+  const uint32_t* state = ch.state + at * kChainCh + lane;
+  for (uint32_t poll = 0; poll < kPollLimit; ++poll) {
+    uint32_t st[kBack];
+    uint64_t mp[kBack];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) s[i] = first[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      ch.agg[at * kCh + lane + 32 * i] = make_float2(A[i], H[i]);
-    __syncwarp();
-    if (lane == 0) {
-      __threadfence();
-      store_release(ch.flag + at, 1u);
+    for (int k = 0; k < kBack; ++k) {
+      st[k] = k < pos ? peek(state - (k + 1) * kChainCh) : kNotYet;
+      mp[k] = k + 1 < pos && k + 1 < kBack ? peek(map - (k + 1) * kChainCh) : ~uint64_t(0);
     }
-    int back = -1;  // how many tiles lie between this one and the known state
-    for (uint32_t poll = 0; poll < kPollLimit; ++poll) {
-      const uint32_t f = lane < pos ? load_acquire(ch.flag + at - 1 - lane) : 0u;
-      const unsigned known = __ballot_sync(kAll, f == 2u), there = __ballot_sync(kAll, f >= 1u);
-      const int p = __ffs(known) - 1;
-      const unsigned between = p >= 0 ? (1u << p) - 1u : 0u;
-      if (p >= 0 && (there & between) == between) {
-        back = p;
-        break;
+    if (poll == 0) post(ch.map + at * kChainCh + lane, A, H);
+    int back = -1;
+    bool joined = true;
+#pragma unroll
+    for (int k = 0; k < kBack; ++k) {
+      if (back < 0 && joined && st[k] != kNotYet) back = k;
+      joined = joined && uint32_t(mp[k]) != kNotYet && uint32_t(mp[k] >> 32) != kNotYet;
+    }
+    if (__all_sync(kAll, back >= 0)) {
+      float s = 0.f;
+#pragma unroll
+      for (int k = kBack - 1; k >= 0; --k) {
+        if (k == back) s = __uint_as_float(st[k]);
+        if (k < back) s = fmaf(__uint_as_float(uint32_t(mp[k])), s, __uint_as_float(uint32_t(mp[k] >> 32)));
       }
-    }
-    __syncwarp();
-    if (back < 0) {
-      if (lane == 0) atomicOr(status, NGDN2_STATUS_WAIT_TIMEOUT);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) s[i] = __int_as_float(0x7fc00000);
-    } else {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) s[i] = __ldcg(ch.inc + (at - 1 - back) * kCh + lane + 32 * i);
-#pragma unroll 8
-      for (int k = back; k > 0; --k)
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          const float2 m = __ldcg(ch.agg + (at - k) * kCh + lane + 32 * i);
-          s[i] = fmaf(m.x, s[i], m.y);
-        }
+      return s;
     }
   }
-  if (pos + 1 < ch.tiles) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      ch.inc[at * kCh + lane + 32 * i] = fmaf(A[i], s[i], H[i]);
-    __syncwarp();
-    if (lane == 0) {
-      __threadfence();
-      store_release(ch.flag + at, 2u);
-    }
-  }
+  if (lane == 0) atomicOr(status, NGDN2_STATUS_WAIT_TIMEOUT);
+  return __int_as_float(0x7fc00000);
 }
 
 // ---------------------------------------------------------------------------
@@ -196,14 +174,21 @@ __device__ __forceinline__ void fill(unsigned char* sm, const void* p, const int
   using S = Stage<DT, CL, R>;
   const int64_t base = b * st[0] + t0 * st[1] + d0 * st[2];
   if constexpr (G > 0) {
-    constexpr int kPer = S::kRow / G, kN = S::kSteps * kPer;
-    const char* src = static_cast<const char*>(p) + base * S::kEl;
-    const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(sm));
-#pragma unroll 4
-    for (int q = threadIdx.x; q < kN; q += kThreads) {
-      const int t = q / kPer, c = q % kPer * G;
-      const bool ok = t0 + t < T && d0 + c / S::kEl < D;
-      copy_async<G>(dst + S::at(t) + c, ok ? src + t * st[1] * S::kEl + c : p, ok);
+    // A thread keeps its columns and steps down the rows.
+    constexpr int kPer = S::kRow / G, kHop = kThreads / kPer;
+    static_assert(kThreads % kPer == 0 && S::kSteps % kHop == 0 && (kHop % R == 0 || R % kHop == 0), "");
+    const int t = threadIdx.x / kPer, c = threadIdx.x % kPer * G;
+    const bool in = d0 + c / S::kEl < D;
+    const char* src = static_cast<const char*>(p) + (base + t * st[1]) * S::kEl + c;
+    const int64_t hop = kHop * st[1] * S::kEl;
+    const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(sm)) + c;
+    const int64_t left = T - t0 - t;
+#pragma unroll 8
+    for (int j = 0; j < S::kSteps / kHop; ++j) {
+      const bool ok = in && j * kHop < left;
+      const uint32_t to = kHop % R == 0 ? S::at(t) + j * (kHop / R) * S::kRun : S::at(t + j * kHop);
+      copy_async<G>(dst + to, ok ? src : p, ok);
+      src += hop;
     }
   } else {
     using E = typename std::conditional<S::kEl == 4, uint32_t, uint16_t>::type;
@@ -307,16 +292,21 @@ scan_kernel(const __grid_constant__ ngdn2_scan_args a, Chain chain, int row_stri
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float2 part[kWarps][kCh];  // the warps' maps
   __shared__ float enter[kWarps][kCh];  // the state entering each warp's runs
-  int strip, pos;
-  take_tile(chain, &strip, &pos);
+  __shared__ uint32_t ticket;
+  const uint32_t total = uint32_t(chain.strips * chain.tiles);
+  unsigned char *sx = smem, *sg = smem + SX::kBytes;
+  if (threadIdx.x == 0) ticket = ask_tile(chain, blockIdx.x - gridDim.x);
+  __syncthreads();
+  for (uint32_t mine = ticket; mine < total; mine = ticket) {
+  const int strip = int(mine % uint32_t(chain.strips)), pos = int(mine / uint32_t(chain.strips));
   const int64_t b = strip / row_strips, d0 = int64_t(strip % row_strips) * kCh;
   const int64_t t0 = int64_t(pos) * kSteps;
-  unsigned char *sx = smem, *sg = smem + SX::kBytes;
   fill<XT, CL, R, G>(sx, a.x, a.x_stride, b, t0, d0, a.T, a.D);
   fill<GT, CL, R, G>(sg, a.g, a.g_stride, b, t0, d0, a.T, a.D);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = 4 * (lane % CL), run = threadIdx.x / CL;
   unsigned char *mx = sx + run * SX::kRun + c * SX::kEl, *mg = sg + run * SG::kRun + c * SG::kEl;
+  uint32_t next = 0;
   fill_done();
 
   // The run's map. Past the end x = g = 0: the identity.
@@ -358,11 +348,10 @@ scan_kernel(const __grid_constant__ ngdn2_scan_args a, Chain chain, int row_stri
   }
   __syncthreads();
   if (warp == 0) {
-    float ta[NV], th[NV], first[NV], s[NV];
+    float ta[NV], th[NV], s[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int ch = lane + 32 * i;
-      first[i] = a.initial_state && d0 + ch < a.D ? a.initial_state[b * a.D + d0 + ch] : 0.f;
       ta[i] = 1.f;
       th[i] = 0.f;
 #pragma unroll
@@ -371,8 +360,13 @@ scan_kernel(const __grid_constant__ ngdn2_scan_args a, Chain chain, int row_stri
         th[i] = fmaf(m.x, th[i], m.y);
         ta[i] *= m.x;
       }
+      s[i] = pos == 0 && a.initial_state && d0 + ch < a.D ? a.initial_state[b * a.D + d0 + ch] : 0.f;
     }
-    chain_state<NV>(chain, strip, pos, ta, th, first, s, a.status);
+    const int64_t at = int64_t(strip) * chain.tiles + pos;
+    if (CL == 8 && pos > 0) s[0] = chain_state(chain, at, pos, ta[0], th[0], a.status);
+    if (CL == 8 && pos + 1 < chain.tiles)  // the same by whichever way s came
+      post(chain.state + at * kChainCh + lane, fmaf(ta[0], s[0], th[0]));
+    if (lane == 0) next = ask_tile(chain, mine);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int ch = lane + 32 * i;
@@ -408,9 +402,12 @@ scan_kernel(const __grid_constant__ ngdn2_scan_args a, Chain chain, int row_stri
     if (G != 16) put4<XT>(mx + r * SX::kRow, h);
     else if (t1 + r < a.T && d < a.D) put4<XT>(out + r * a.D * SX::kEl, h);
   }
+  if (threadIdx.x == 0) ticket = next;
+  __syncthreads();
   if (G != 16) {
-    __syncthreads();
     drain<XT, CL, R>(sx, a.h, b, t0, d0, a.T, a.D);
+    __syncthreads();
+  }
   }
 }
 
@@ -425,7 +422,7 @@ constexpr int bwd_smem() {
 }
 
 template <int XT, int GT, int G, int CL, int R>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kThreads, XT == NGDN2_F32 ? 2 : 3)
 scan_bwd_kernel(const __grid_constant__ ngdn2_scan_bwd_args p, Chain chain, int row_strips) {
   constexpr int kCh = 4 * CL, NV = kCh / 32, kSteps = kThreads / CL * R;
   static_assert(NGDN2_SCAN_CHUNK % kSteps == 0, "a tile starts at a state that the forward left, or within its chunk as the only tile");
@@ -435,11 +432,15 @@ scan_bwd_kernel(const __grid_constant__ ngdn2_scan_bwd_args p, Chain chain, int 
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ float2 part_h[kWarps][kCh], part_c[kWarps][kCh];
   __shared__ float enter_h[kWarps][kCh], enter_c[kWarps][kCh];
-  int strip, pos;
-  take_tile(chain, &strip, &pos);
+  __shared__ uint32_t ticket;
+  const uint32_t total = uint32_t(chain.strips * chain.tiles);
+  unsigned char *sx = smem, *sd = smem + SX::kBytes, *sg = smem + 2 * SX::kBytes;
+  if (threadIdx.x == 0) ticket = ask_tile(chain, blockIdx.x - gridDim.x);
+  __syncthreads();
+  for (uint32_t mine = ticket; mine < total; mine = ticket) {
+  const int strip = int(mine % uint32_t(chain.strips)), pos = int(mine / uint32_t(chain.strips));
   const int64_t b = strip / row_strips, d0 = int64_t(strip % row_strips) * kCh;
   const int64_t tile = chain.tiles - 1 - pos, t0 = tile * kSteps;
-  unsigned char *sx = smem, *sd = smem + SX::kBytes, *sg = smem + 2 * SX::kBytes;
   fill<XT, CL, R, G>(sx, a.x, a.x_stride, b, t0, d0, a.T, a.D);
   fill<GT, CL, R, G>(sg, a.g, a.g_stride, b, t0, d0, a.T, a.D);
   fill<XT, CL, R, G>(sd, p.d_h, p.d_h_stride, b, t0, d0, a.T, a.D);
@@ -447,6 +448,7 @@ scan_bwd_kernel(const __grid_constant__ ngdn2_scan_bwd_args p, Chain chain, int 
   const int c = 4 * (lane % CL), run = threadIdx.x / CL;
   unsigned char *mx = sx + run * SX::kRun + c * SX::kEl, *md = sd + run * SX::kRun + c * SX::kEl,
                 *mg = sg + run * SG::kRun + c * SG::kEl;
+  uint32_t next = 0;
   fill_done();
 
   float Ah[4] = {1.f, 1.f, 1.f, 1.f}, H[4] = {}, Ac[4], C[4] = {};
@@ -510,11 +512,10 @@ scan_bwd_kernel(const __grid_constant__ ngdn2_scan_bwd_args p, Chain chain, int 
   }
   __syncthreads();
   if (warp == 0) {
-    float ta[NV], tc[NV], first[NV], s[NV];
+    float ta[NV], tc[NV], s[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int ch = lane + 32 * i;
-      first[i] = p.d_final && d0 + ch < a.D ? p.d_final[b * a.D + d0 + ch] : 0.f;
       ta[i] = 1.f;
       tc[i] = 0.f;
 #pragma unroll
@@ -523,8 +524,13 @@ scan_bwd_kernel(const __grid_constant__ ngdn2_scan_bwd_args p, Chain chain, int 
         tc[i] = fmaf(m.x, tc[i], m.y);
         ta[i] *= m.x;
       }
+      s[i] = pos == 0 && p.d_final && d0 + ch < a.D ? p.d_final[b * a.D + d0 + ch] : 0.f;
     }
-    chain_state<NV>(chain, strip, pos, ta, tc, first, s, p.status);
+    const int64_t at = int64_t(strip) * chain.tiles + pos;
+    if (CL == 8 && pos > 0) s[0] = chain_state(chain, at, pos, ta[0], tc[0], p.status);
+    if (CL == 8 && pos + 1 < chain.tiles)
+      post(chain.state + at * kChainCh + lane, fmaf(ta[0], s[0], tc[0]));
+    if (lane == 0) next = ask_tile(chain, mine);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int ch = lane + 32 * i;
@@ -585,10 +591,13 @@ scan_bwd_kernel(const __grid_constant__ ngdn2_scan_bwd_args p, Chain chain, int 
       put4<GT>(og + r * a.D * SG::kEl, dg);
     }
   }
+  if (threadIdx.x == 0) ticket = next;
+  __syncthreads();
   if (G != 16) {
-    __syncthreads();
     drain<XT, CL, R>(sd, p.dx, b, t0, d0, a.T, a.D);
     drain<GT, CL, R>(sg, p.dg, b, t0, d0, a.T, a.D);
+    __syncthreads();
+  }
   }
 }
 
@@ -619,11 +628,18 @@ int granule(const void* p, int dt, const int64_t* st, int64_t D) {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// At most as many CTAs as the GPU holds at once.
 template <class K, class... Args>
-cudaError_t launch(K kernel, int64_t grid, int smem, cudaStream_t st, const Args&... args) {
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+cudaError_t launch(K kernel, int64_t tiles, int smem, cudaStream_t st, const Args&... args) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  int dev = 0, sms = 0, per_sm = 0;
+  if (e == cudaSuccess) e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess)
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, smem);
   if (e != cudaSuccess) return e;
-  kernel<<<unsigned(grid), kThreads, smem, st>>>(args...);
+  const int64_t fit = int64_t(sms) * (per_sm > 0 ? per_sm : 1);
+  kernel<<<unsigned(tiles < fit ? tiles : fit), kThreads, smem, st>>>(args...);
   return cudaGetLastError();
 }
 
@@ -700,12 +716,12 @@ int validate_scan_bwd(const ngdn2_scan_bwd_args* a) {
   return NGDN2_OK;
 }
 
-// The chain of one launch, its counter and state words cleared.
+// The chain of one launch, with nothing there yet.
 int start_chain(const Shape& s, void* ws, size_t ws_bytes, cudaStream_t st, Chain* c) {
-  const size_t need = chain_bytes(s.strips, s.tiles, s.channels);
+  const size_t need = chain_bytes(s.strips, s.tiles);
   if (need && (!ws || ws_bytes < need)) return NGDN2_ERR_WORKSPACE;
-  *c = make_chain(ws, s.strips, s.tiles, s.channels);
-  if (need && cudaMemsetAsync(c->ticket, 0, chain_flag_bytes(s.strips, s.tiles), st) != cudaSuccess)
+  *c = make_chain(ws, s.strips, s.tiles);
+  if (need && cudaMemsetAsync(c->map, 0xff, need - 16, st) != cudaSuccess)
     return NGDN2_ERR_CUDA;
   return NGDN2_OK;
 }
@@ -723,7 +739,7 @@ NGDN2_API int ngdn2_scan_workspace_size(const ngdn2_scan_args* a, size_t* bytes)
   if (rc != NGDN2_OK) return rc;
   if (!bytes) return NGDN2_ERR_NULL;
   const Shape s = shape_of(a);
-  *bytes = chain_bytes(s.strips, s.tiles, s.channels);
+  *bytes = chain_bytes(s.strips, s.tiles);
   return NGDN2_OK;
 }
 
