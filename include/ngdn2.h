@@ -309,7 +309,7 @@ typedef struct ngdn2_embed_bwd_args {
 } ngdn2_embed_bwd_args;
 
 /* Steps between the states that ngdn2_scan leaves for its backward. */
-#define NGDN2_SCAN_CHUNK 256
+#define NGDN2_SCAN_CHUNK 128
 
 /* Arguments of ngdn2_scan: h_t = e^(g_t) h_{t-1} + x_t for each (batch row,
  * channel), the state in fp32. g = -inf drops the state (a packed sequence

@@ -38,7 +38,7 @@ STATUS_WAIT_TIMEOUT = 1
 STATUS_GATE_TIMEOUT = 2
 STATUS_BAD_INDEX = 4
 
-SCAN_CHUNK = 256
+SCAN_CHUNK = 128
 
 c_i32, c_i64, c_ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
 

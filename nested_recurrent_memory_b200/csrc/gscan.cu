@@ -29,7 +29,7 @@ using namespace ngdn2;
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr unsigned kAll = 0xffffffffu;
 constexpr uint32_t kPollLimit = 1u << 21;
@@ -37,7 +37,7 @@ constexpr uint32_t kPollLimit = 1u << 21;
 bool dtype_ok(int d) { return d == NGDN2_F32 || d == NGDN2_BF16 || d == NGDN2_F16; }
 
 // ---------------------------------------------------------------------------
-// The chain of tiles. A tile is CL lanes of four channels by 256 / CL runs of R
+// The chain of tiles. A tile is CL lanes of four channels by 128 / CL runs of R
 // steps.
 // ---------------------------------------------------------------------------
 
@@ -284,7 +284,7 @@ constexpr int fwd_smem() {
 }
 
 template <int XT, int GT, int G, int CL, int R>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, 8)
 scan_kernel(const __grid_constant__ ngdn2_scan_args a, Chain chain, int row_strips) {
   constexpr int kCh = 4 * CL, NV = kCh / 32, kSteps = kThreads / CL * R;
   using SX = Stage<XT, CL, R>;
@@ -422,7 +422,7 @@ constexpr int bwd_smem() {
 }
 
 template <int XT, int GT, int G, int CL, int R>
-__global__ void __launch_bounds__(kThreads, XT == NGDN2_F32 ? 2 : 3)
+__global__ void __launch_bounds__(kThreads, XT == NGDN2_F32 ? 4 : 6)
 scan_bwd_kernel(const __grid_constant__ ngdn2_scan_bwd_args p, Chain chain, int row_strips) {
   constexpr int kCh = 4 * CL, NV = kCh / 32, kSteps = kThreads / CL * R;
   static_assert(NGDN2_SCAN_CHUNK % kSteps == 0, "a tile starts at a state that the forward left, or within its chunk as the only tile");
@@ -663,7 +663,7 @@ cudaError_t by_types(int xt, int gt, F&& f) {
 // that the chain is short; the wide one (128 channels) is for sequences of
 // at most its 32 steps, whose narrow tiles would be mostly empty.
 constexpr int kNarrowR = 8, kNarrowSteps = kThreads / 8 * kNarrowR;
-constexpr int kWideR = 4, kWideSteps = kThreads / 32 * kWideR;
+constexpr int kWideR = 8, kWideSteps = kThreads / 32 * kWideR;
 
 template <class F>
 cudaError_t by_tile(int channels, int granule, F&& f) {

@@ -65,7 +65,7 @@ def gated_scan_fwd(x, g, initial_state=None, output_final_state=False, return_au
     Returns ``(h, final_state)``: h [B, T, D] in x's dtype, final_state
     [B, D] float32 (None unless ``output_final_state``); with ``return_aux``
     also the dict that ``gated_scan_bwd`` takes (the states entering every
-    256 steps)."""
+    128 steps)."""
     _check_inputs(x, g)
     B, T, D = x.shape
     dev = x.device
