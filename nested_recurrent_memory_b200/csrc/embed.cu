@@ -7,7 +7,7 @@
 //
 // The gradient sorts (token, position) pairs by token with a stable radix
 // sort, so that a row's terms are added in the order of their positions and
-// the result is reproducible (in one launch by a cluster up to 8192 tokens). The
+// the result is reproducible (in one launch by a cluster up to 16384 tokens). The
 // sorted list is then cut into chunks of
 // equal length, however often a token occurs: a CTA adds up the runs of
 // equal tokens in its chunk; a run that lies within the chunk is its row's
@@ -147,8 +147,7 @@ embed_kernel(const __grid_constant__ ngdn2_embed_args a, int rows) {
 
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 // Pairs a thread has of its tile. One up to kFewTokens: small tiles spread the
-// scattered stores, which bound a pass, over the GPU; beyond, eight keep the
-// table of the tiles' counts, which every tile reads, small.
+// scattered stores over the GPU; beyond, eight keep the tiles' counts few.
 constexpr int kManyEach = 8;
 constexpr int64_t kFewTokens = 256 * kSortThreads;
 constexpr int kDigitMost = 9, kBinsMost = 1 << kDigitMost;
@@ -158,8 +157,7 @@ struct SortArgs {
   int ids_i32, bits;     // bits of a digit
   int64_t N, V, pad, tiles;
   uint2 *a, *b;          // pairs: sorted ones end in a
-  uint32_t* count;       // [tiles][bins]
-  uint8_t* present;      // [V + 1]: the token occurs
+  uint32_t* count;       // [bins][tiles], then [bins]: the tiles' digit counts, all tiles'
   uint32_t* crossing;    // how many runs cross chunks, then their first chunks
   char* zero;            // the part of dweight to be zeroed beside the sort
   int64_t zero_bytes;
@@ -188,7 +186,7 @@ __device__ __forceinline__ uint2 load_pair(const SortArgs& s, const uint2* src, 
   return src[n];
 }
 
-// Digit counts of every tile; the first pass also clears ``present``.
+// Digit counts of every tile.
 template <bool FIRST, int EACH>
 __global__ void __launch_bounds__(kSortThreads)
 sort_count_kernel(const __grid_constant__ SortArgs s, const uint2* src, int shift) {
@@ -207,13 +205,40 @@ sort_count_kernel(const __grid_constant__ SortArgs s, const uint2* src, int shif
   for (int k = 0; k < EACH; ++k)
     if (d[k] < uint32_t(nb)) atomicAdd(bins + d[k], 1u);
   __syncthreads();
-  for (int i = tid; i < nb; i += kSortThreads) s.count[int64_t(blockIdx.x) * nb + i] = bins[i];
+  for (int i = tid; i < nb; i += kSortThreads) s.count[int64_t(i) * s.tiles + blockIdx.x] = bins[i];
   if (FIRST && blockIdx.x == 0 && tid == 0) s.crossing[0] = 0;
-  if (FIRST)
-    for (int64_t v = int64_t(blockIdx.x) * kSortThreads + tid; v <= s.V / 16;
-         v += s.tiles * kSortThreads)  // (its room is a multiple of 256 bytes)
-      reinterpret_cast<uint4*>(s.present)[v] = make_uint4(0, 0, 0, 0);
   let_next_start();
+}
+
+// Each digit's counts become the counts of the tiles before; a warp a digit.
+constexpr int kPrefixThreads = 128;
+
+__global__ void __launch_bounds__(kPrefixThreads) sort_prefix_kernel(const __grid_constant__ SortArgs s) {
+  const int lane = threadIdx.x & 31, d = blockIdx.x * (kPrefixThreads / 32) + (threadIdx.x >> 5);
+  const int nb = 1 << s.bits;
+  after_previous();
+  let_next_start();
+  if (d >= nb) return;
+  uint32_t* row = s.count + int64_t(d) * s.tiles;
+  uint32_t sum = 0;
+  for (int64_t t0 = 0; t0 < s.tiles; t0 += 128) {
+    uint32_t c[4], x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = x[i] = t0 + 32 * i + lane < s.tiles ? row[t0 + 32 * i + lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x[i], o);
+        if (lane >= o) x[i] += y;
+      }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (t0 + 32 * i + lane < s.tiles) row[t0 + 32 * i + lane] = sum + x[i] - c[i];
+      sum += __shfl_sync(0xffffffffu, x[i], 31);
+    }
+  }
+  if (lane == 0) s.count[nb * s.tiles + d] = sum;
 }
 
 // The lanes whose digit equals this lane's: one vote a bit.
@@ -279,11 +304,11 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* part) {
   return before + x - v;
 }
 
-template <bool FIRST, bool LAST, int EACH>
+template <bool FIRST, int EACH>
 __global__ void __launch_bounds__(kSortThreads)
 sort_place_kernel(const __grid_constant__ SortArgs s, const uint2* src, uint2* dst, int shift) {
   __shared__ uint16_t warp_bins[kSortWarps][kBinsMost];
-  __shared__ uint32_t total[kSortThreads], before[kSortThreads], part[kSortWarps], base[kBinsMost];
+  __shared__ uint32_t part[kSortWarps], base[kBinsMost];
   const int nb = 1 << s.bits, tid = threadIdx.x;
   after_previous();
   uint2 p[EACH];
@@ -294,45 +319,33 @@ sort_place_kernel(const __grid_constant__ SortArgs s, const uint2* src, uint2* d
     p[k] = n < s.N ? load_pair<FIRST>(s, src, n) : make_uint2(0, 0);
     digit[k] = n < s.N ? p[k].x >> shift & (nb - 1) : uint32_t(nb);
   }
-  // Pairs of smaller digits, and of this digit in earlier tiles: threads of
-  // one digit share the tiles.
-  const int d = tid & (nb - 1), share = kSortThreads / nb, first = tid / nb;
-  uint32_t all = 0, earlier = 0;
-#pragma unroll 8
-  for (int64_t t = first; t < s.tiles; t += share) {
-    const uint32_t c = s.count[t * nb + d];
-    all += c;
-    earlier += t < blockIdx.x ? c : 0;
-  }
-  total[tid] = all;
-  before[tid] = earlier;
+  // Pairs of smaller digits, and of this digit in earlier tiles.
+  const uint32_t all = tid < nb ? s.count[nb * s.tiles + tid] : 0;
+  const uint32_t earlier = tid < nb ? s.count[tid * s.tiles + blockIdx.x] : 0;
   rank_pairs<EACH>(s.bits, digit, at, warp_bins, nullptr);
-  __syncthreads();
-  all = earlier = 0;
-  if (tid < nb)
-    for (int i = 0; i < share; ++i) {
-      all += total[tid + i * nb];
-      earlier += before[tid + i * nb];
-    }
-  const uint32_t smaller = block_prefix(tid < nb ? all : 0, part);
+  const uint32_t smaller = block_prefix(all, part);
   if (tid < nb) base[tid] = smaller + earlier;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < EACH; ++k)
-    if (digit[k] < uint32_t(nb)) {
+    if (digit[k] < uint32_t(nb))
       dst[base[digit[k]] + warp_bins[tid >> 5][digit[k]] + at[k]] = p[k];
-      if (LAST) s.present[p[k].x] = 1;
-    }
   let_next_start();
 }
 
-// All passes in one launch for up to 8192 pairs, one a thread: a cluster of eight
-// CTAs exchanges the digits' totals and the pairs themselves through distributed
-// shared memory. (With 16 pairs a thread, for up to 131072, its scattered
-// stores took 68 us.) The CTAs after the cluster zero their part of dweight.
-constexpr int kCluster = 8, kClusterTokens = kCluster * kSortThreads;
-constexpr size_t kClusterSmem = sizeof(uint16_t) * kSortWarps * kBinsMost + sizeof(uint2) * kSortThreads;
+// All passes in one launch for up to 8192 EACH pairs: a cluster of eight CTAs
+// exchanges the digits' totals and the pairs themselves through distributed
+// shared memory. (With EACH = 16, for 131072 pairs, its scattered stores took
+// 68 us.) The CTAs after the cluster zero their part of dweight.
+constexpr int kCluster = 8, kClusterEach = 2;
+constexpr int64_t kClusterTokens = kCluster * kSortThreads * kClusterEach;
 
+template <int EACH>
+constexpr size_t cluster_smem() {
+  return sizeof(uint16_t) * kSortWarps * kBinsMost + sizeof(uint2) * kSortThreads * EACH;
+}
+
+template <int EACH>
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kSortThreads)
 sort_cluster_kernel(const __grid_constant__ SortArgs s, int passes) {
   namespace cg = cooperative_groups;
@@ -353,14 +366,19 @@ sort_cluster_kernel(const __grid_constant__ SortArgs s, int passes) {
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t mine = blockIdx.x;  // (one cluster)
   if (mine == 0 && tid == 0) s.crossing[0] = 0;
-  for (int64_t v = mine * kSortThreads + tid; v <= s.V / 16; v += kCluster * kSortThreads)
-    reinterpret_cast<uint4*>(s.present)[v] = make_uint4(0, 0, 0, 0);  // (room for a multiple of 256 bytes)
-  const int64_t n = int64_t(mine) * kSortThreads + tid;
-  uint2 p = n < s.N ? load_pair<true>(s, nullptr, n) : make_uint2(0, 0);
+  constexpr uint32_t kRoom = kSortThreads * EACH;
+  uint2 p[EACH];
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    const int64_t n = pair_index<EACH>(mine, k);
+    p[k] = n < s.N ? load_pair<true>(s, nullptr, n) : make_uint2(0, 0);
+  }
   for (int pass = 0; pass < passes; ++pass) {
-    const uint32_t digit = n < s.N ? p.x >> (pass * s.bits) & (nb - 1) : uint32_t(nb);
-    uint32_t at;
-    rank_pairs<1>(s.bits, &digit, &at, warp_bins, totals);
+    uint32_t digit[EACH], at[EACH];
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+      digit[k] = pair_index<EACH>(mine, k) < s.N ? p[k].x >> (pass * s.bits) & (nb - 1) : uint32_t(nb);
+    rank_pairs<EACH>(s.bits, digit, at, warp_bins, totals);
     cluster.sync();  // all totals are there, and all pairs in registers
     const int d = tid & (nb - 1), share = kSortThreads / nb;
     uint32_t all = 0, earlier = 0;
@@ -382,18 +400,21 @@ sort_cluster_kernel(const __grid_constant__ SortArgs s, int passes) {
     if (tid < nb) base[tid] = smaller + earlier;
     __syncthreads();
     const bool last = pass + 1 == passes;
-    if (digit < uint32_t(nb)) {
-      const uint32_t to = base[digit] + warp_bins[warp][digit] + at;
-      if (last) {
-        s.a[to] = p;
-        s.present[p.x] = 1;
-      } else {
-        *cluster.map_shared_rank(buf + to % kSortThreads, to / kSortThreads) = p;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+      if (digit[k] < uint32_t(nb)) {
+        const uint32_t to = base[digit[k]] + warp_bins[warp][digit[k]] + at[k];
+        if (last) s.a[to] = p[k];
+        else *cluster.map_shared_rank(buf + to % kRoom, to / kRoom) = p[k];
       }
-    }
     if (last) let_next_start();
     cluster.sync();  // the pairs have arrived; nobody reads these totals any more
-    if (!last && n < s.N) p = buf[tid];
+    if (!last)
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        const int64_t n = pair_index<EACH>(mine, k);
+        if (n < s.N) p[k] = buf[n - int64_t(mine) * kRoom];
+      }
   }
 }
 
@@ -402,11 +423,10 @@ sort_cluster_kernel(const __grid_constant__ SortArgs s, int passes) {
 // ---------------------------------------------------------------------------
 
 constexpr int kSumThreads = 128, kSumAhead = 8;
-constexpr int kChunkMost = 128, kZeroRows = 16;
+constexpr int kChunkMost = 128, kZeroRows = 64, kLookThrough = 2048;
 
 struct SumArgs {
   const uint2* pairs;
-  const uint8_t* present;
   const void* d_out;
   void* dweight;
   uint32_t* crossing;
@@ -416,6 +436,25 @@ struct SumArgs {
   int chunk;
   float scale;
 };
+
+// The first of the sorted pairs [lo, hi) that is not less than v, left in lo,
+// for M values at once. One whole warp.
+template <int M>
+__device__ __forceinline__ void lower_bounds(const uint2* pairs, int64_t* lo, int64_t* hi, const uint32_t* v) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t span = hi[0] - lo[0]; span > 0; span = span > 1 ? (span + 31) / 32 : 0) {
+    const int64_t step = (span + 31) / 32;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const int64_t at = lo[m] + lane * step;
+      const bool less = at < hi[m] && pairs[at].x < v[m];
+      const int n = __popc(__ballot_sync(0xffffffffu, less));
+      // It lies after the last probe that was less and not after the next one.
+      hi[m] = lo[m] + n * step < hi[m] ? lo[m] + n * step : hi[m];
+      lo[m] = n == 0 ? lo[m] : lo[m] + (n - 1) * step + 1;
+    }
+  }
+}
 
 // Column blocks of kSumThreads * W in grid.y; in grid.x the chunks, then the
 // rows to be zeroed.
@@ -437,13 +476,33 @@ __global__ void __launch_bounds__(kSumThreads) sum_kernel(const __grid_constant_
   };
   after_previous();
   if (blockIdx.x >= s.chunks) {
+    // Which of kZeroRows rows have a token: the rows' part of the sorted list is
+    // searched for, 32 ways a step, and then looked through, or searched row by
+    // row where it is long.
     const int64_t v0 = (int64_t(blockIdx.x) - s.chunks) * kZeroRows;
+    const int lane = tid & 31;
+    int64_t lo[2] = {0, 0}, hi[2] = {s.N, s.N};
+    const uint32_t ends[2] = {uint32_t(v0), uint32_t(v0 + kZeroRows)};
+    lower_bounds<2>(s.pairs, lo, hi, ends);
+    if (tid < kZeroRows) list[tid].x = 0;
+    __syncthreads();
+    if (lo[1] - lo[0] <= kLookThrough) {
+      for (int64_t i = lo[0] + tid; i < lo[1]; i += kSumThreads) list[s.pairs[i].x - ends[0]].x = 1;
+    } else {
+      for (int r = tid / 32; r < kZeroRows; r += kSumThreads / 32) {
+        int64_t l = lo[0], h = lo[1];
+        const uint32_t v = uint32_t(v0 + r);
+        lower_bounds<1>(s.pairs, &l, &h, &v);
+        if (lane == 0 && l < s.N && s.pairs[l].x == v) list[r].x = 1;
+      }
+    }
+    __syncthreads();
+    let_next_start();
     if (col < s.D) {
       float zero[W] = {};
       for (int r = 0; r < kZeroRows; ++r)
-        if (v0 + r < s.zero_rows && !s.present[v0 + r]) write(v0 + r, zero);
+        if (v0 + r < s.zero_rows && !list[r].x) write(v0 + r, zero);
     }
-    let_next_start();
     return;
   }
   const int64_t i0 = int64_t(blockIdx.x) * s.chunk;
@@ -589,7 +648,7 @@ constexpr int64_t kZeroBytes = int64_t(64) << 20;
 struct BwdPlan {
   int bits, passes, chunk;
   int64_t tiles, chunks;
-  size_t a, b, count, present, crossing, part, total;
+  size_t a, b, count, crossing, part, total;
 };
 
 BwdPlan plan_bwd(const ngdn2_embed_bwd_args* a) {
@@ -614,8 +673,7 @@ BwdPlan plan_bwd(const ngdn2_embed_bwd_args* a) {
   p.a = take(size_t(a->N) * 8);
   const bool clustered = a->N <= kClusterTokens;
   p.b = take(clustered ? 0 : size_t(a->N) * 8);
-  p.count = take(clustered ? 0 : size_t(p.tiles) << p.bits << 2);
-  p.present = take(size_t(a->V) + 1);
+  p.count = take(clustered ? 0 : size_t(p.tiles + 1) << p.bits << 2);
   p.crossing = take(size_t(p.chunks + 1) * 4);
   p.part = take(size_t(p.chunks) * 2 * size_t(a->D) * 4);
   p.total = at + 256;
@@ -631,25 +689,33 @@ cudaError_t sort_in_tiles(const SortArgs& s, int passes, cudaStream_t st) {
     uint2* dst = (passes - 1 - pass) % 2 == 0 ? s.a : s.b;
     const uint2* src = dst == s.a ? s.b : s.a;
     const int shift = pass * s.bits;
-    const bool last = pass + 1 == passes;
     e = pass == 0 ? launch_next(sort_count_kernel<true, EACH>, grid, block, 0, st, false, s, src, shift)
                   : launch_next(sort_count_kernel<false, EACH>, grid, block, 0, st, true, s, src, shift);
     if (e != cudaSuccess) break;
-    auto* place = pass == 0 ? (last ? sort_place_kernel<true, true, EACH> : sort_place_kernel<true, false, EACH>)
-                            : (last ? sort_place_kernel<false, true, EACH> : sort_place_kernel<false, false, EACH>);
+    constexpr int kDigits = kPrefixThreads / 32;
+    e = launch_next(sort_prefix_kernel, dim3(((1u << s.bits) + kDigits - 1) / kDigits), dim3(kPrefixThreads), 0,
+                    st, true, s);
+    if (e != cudaSuccess) break;
+    auto* place = pass == 0 ? sort_place_kernel<true, EACH> : sort_place_kernel<false, EACH>;
     e = launch_next(place, grid, block, 0, st, true, s, src, dst, shift);
   }
   return e;
 }
 
-cudaError_t sort_pairs(const SortArgs& s, int passes, cudaStream_t st) {
-  if (s.N > kClusterTokens)
-    return s.N <= kFewTokens ? sort_in_tiles<1>(s, passes, st) : sort_in_tiles<kManyEach>(s, passes, st);
-  const cudaError_t e = cudaFuncSetAttribute(sort_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             int(kClusterSmem));
+template <int EACH>
+cudaError_t sort_in_cluster(const SortArgs& s, int passes, cudaStream_t st) {
+  constexpr size_t smem = cluster_smem<EACH>();
+  const cudaError_t e = cudaFuncSetAttribute(sort_cluster_kernel<EACH>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return e;
-  return launch_next(sort_cluster_kernel, dim3(kCluster + (s.zero_bytes ? kZeroCtas : 0)),
-                     dim3(kSortThreads), kClusterSmem, st, false, s, passes);
+  return launch_next(sort_cluster_kernel<EACH>, dim3(kCluster + (s.zero_bytes ? kZeroCtas : 0)),
+                     dim3(kSortThreads), smem, st, false, s, passes);
+}
+
+cudaError_t sort_pairs(const SortArgs& s, int passes, cudaStream_t st) {
+  if (s.N <= kCluster * kSortThreads) return sort_in_cluster<1>(s, passes, st);
+  if (s.N <= kClusterTokens) return sort_in_cluster<kClusterEach>(s, passes, st);
+  return s.N <= kFewTokens ? sort_in_tiles<1>(s, passes, st) : sort_in_tiles<kManyEach>(s, passes, st);
 }
 
 template <class F>
@@ -726,12 +792,10 @@ NGDN2_API int ngdn2_embed_bwd(const ngdn2_embed_bwd_args* a, void* stream) {
   so.a = reinterpret_cast<uint2*>(ws + p.a);
   so.b = reinterpret_cast<uint2*>(ws + p.b);
   so.count = reinterpret_cast<uint32_t*>(ws + p.count);
-  so.present = reinterpret_cast<uint8_t*>(ws + p.present);
   so.crossing = reinterpret_cast<uint32_t*>(ws + p.crossing);
   so.status = a->status;
   SumArgs su;
   su.pairs = so.a;
-  su.present = so.present;
   su.d_out = a->d_out;
   su.dweight = a->dweight;
   su.crossing = so.crossing;
