@@ -13,7 +13,8 @@
 // tensor cores' rate. A 16-bit update fits its hi plane, so the first step
 // needs one product for A and two for X.
 //
-// Kernels: the squared norm (partial sums in 64 bits), the conversion to
+// Matrices of up to 128 x 256 take one CTA and one launch (orth_small_kernel).
+// Kernels for larger ones: the squared norm (partial sums in 64 bits), the conversion to
 // planes, then per step three products: A = X X^T, B = a I + b A + c A A
 // (both symmetric: tiles on and above the diagonal only, written twice) and
 // X' = B X, which reads X as it lies, rows along the reduction.
@@ -29,6 +30,8 @@
 #include <cudaTypedefs.h>
 #include <cuda_fp16.h>
 #include <math.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.cuh"
@@ -56,40 +59,76 @@ __device__ __forceinline__ void split(float x, __half& hi, __half& lo) {
 // Norm and conversion
 // ---------------------------------------------------------------------------
 
-constexpr int kPrepThreads = 256, kNormParts = 64;
+constexpr int kPrepThreads = 256, kNormPartsMost = 256;
 
 struct PrepArgs {
   const void* g;
-  int dtype;
   int64_t batch, m, n;     // X is m x n
   int64_t sb, sr, sc;      // element strides of the update by matrix, row and column of X
   float eps;
-  double* part;            // [batch][kNormParts]
+  int parts;               // of a matrix's sum of squares, a multiple of 32
+  double* part;            // [batch][parts]
   float* sigma;            // [batch]: X_0 = sigma * planes
-  __half* x;               // [batch][2][m][ld]
+  __half* x;               // [batch][2][m][ld]; the lo plane only where lo is set
   int64_t ld;
+  bool lo;
 };
 
+// Sixteen bytes as fp32.
+template <int DT>
+__device__ __forceinline__ void unpack16(const uint4& t, float* v) {
+  const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == NGDN2_F32) {
+      v[i] = __uint_as_float(w[i]);
+    } else {
+      const float2 f = DT == NGDN2_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]))
+                                        : __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+}
+
 // Squares are summed in 64 bits, so neither large nor small updates leave
-// the range.
+// the range. FLAT: each matrix lies in one piece on 16-byte boundaries.
+template <int DT, bool FLAT>
 __global__ void __launch_bounds__(kPrepThreads) orth_norm_kernel(const __grid_constant__ PrepArgs p) {
   __shared__ double red[kPrepThreads / 32];
-  const int64_t b = blockIdx.x / kNormParts, part = blockIdx.x % kNormParts;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // Lanes along the dimension with the smaller stride.
-  const bool along_c = p.sc <= p.sr;
-  const int64_t outer = along_c ? p.m : p.n, inner = along_c ? p.n : p.m;
-  const int64_t so = along_c ? p.sr : p.sc, si = along_c ? p.sc : p.sr;
+  const int64_t b = blockIdx.x / p.parts;
+  const int part = int(blockIdx.x % p.parts), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double s = 0.0;
-  for (int64_t r = part * (kPrepThreads / 32) + warp; r < outer; r += int64_t(kNormParts) * (kPrepThreads / 32)) {
-    const int64_t base = b * p.sb + r * so;
-    double row = 0.0;
-#pragma unroll 8
-    for (int64_t c = lane; c < inner; c += 32) {
-      const double x = load_elem(p.g, base + c * si, p.dtype);
-      row = fma(x, x, row);
+  if constexpr (FLAT) {
+    constexpr int kPer = DT == NGDN2_F32 ? 4 : 8;
+    const int64_t pieces = p.m * p.n / kPer;
+    const char* g = static_cast<const char*>(p.g) + b * p.sb * (16 / kPer);
+    const int64_t hop = int64_t(p.parts) * kPrepThreads;
+#pragma unroll 4
+    for (int64_t i = int64_t(part) * kPrepThreads + threadIdx.x; i < pieces; i += hop) {
+      float v[8];
+      unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(g) + i), v);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) s = fma(double(v[j]), double(v[j]), s);
     }
-    s += row;
+    for (int64_t i = pieces * kPer + threadIdx.x; part == 0 && i < p.m * p.n; i += kPrepThreads) {
+      const double x = load_typed<DT>(g, i);
+      s = fma(x, x, s);
+    }
+  } else {
+    // Lanes along the dimension with the smaller stride.
+    const bool along_c = p.sc <= p.sr;
+    const int64_t outer = along_c ? p.m : p.n, inner = along_c ? p.n : p.m;
+    const int64_t so = along_c ? p.sr : p.sc, si = along_c ? p.sc : p.sr;
+    constexpr int kWarps = kPrepThreads / 32;
+    for (int64_t r = int64_t(part) * kWarps + warp; r < outer; r += int64_t(p.parts) * kWarps) {
+      const int64_t base = b * p.sb + r * so;
+#pragma unroll 8
+      for (int64_t c = lane; c < inner; c += 32) {
+        const double x = load_typed<DT>(p.g, base + c * si);
+        s = fma(x, x, s);
+      }
+    }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -97,58 +136,95 @@ __global__ void __launch_bounds__(kPrepThreads) orth_norm_kernel(const __grid_co
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < kPrepThreads / 32; ++w) s += red[w];
-    p.part[b * kNormParts + part] = s;
+    p.part[b * p.parts + part] = s;
   }
   let_next_start();
 }
 
-// The power of two that brings the norm into [2^11, 2^12), and sigma.
-__device__ __forceinline__ void norm_scale(const PrepArgs& p, int64_t b, int* k, float* sigma) {
-  double s = p.part[b * kNormParts + (threadIdx.x & 31)] + p.part[b * kNormParts + 32 + (threadIdx.x & 31)];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  const double norm = sqrt(s);
-  int e = 0;
-  if (norm > 0.0 && norm < 1e300) frexp(norm, &e);
-  *k = (norm > 0.0 && norm < 1e300) ? 12 - e : 0;
-  *sigma = float(1.0 / (norm + double(p.eps)) / scalbn(1.0, *k));
+// For a sum of squares: the power of two that brings the norm into [2^11, 2^12),
+// and sigma.
+__device__ __forceinline__ void scale_of(double sum, float eps, int* k, float* sigma) {
+  const double norm = sqrt(sum);
+  const bool finite = norm > 0.0 && norm < 1e300;
+  int e = 12;
+  if (finite) frexp(norm, &e);
+  *k = 12 - e;
+  *sigma = float(1.0 / (norm + double(eps)) / scalbn(1.0, *k));
 }
 
-constexpr int kConvTile = 64;
+__device__ __forceinline__ void norm_scale(const PrepArgs& p, int64_t b, int* k, float* sigma) {
+  double s = 0.0;
+  for (int i = threadIdx.x & 31; i < p.parts; i += 32) s += p.part[b * p.parts + i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  scale_of(s, p.eps, k, sigma);
+}
 
+// The planes of X_0 / sigma. ROWS: X's rows lie on 16-byte boundaries in the
+// update, and a CTA takes kConvRows of them in pieces of eight; otherwise it
+// takes a tile, read along the update's dimension with the smaller stride.
+constexpr int kConvTile = 64, kConvRows = 4;
+
+template <int DT, bool ROWS>
 __global__ void __launch_bounds__(kPrepThreads) orth_convert_kernel(const __grid_constant__ PrepArgs p) {
-  __shared__ float tile[kConvTile][kConvTile + 1];
+  __shared__ float tile[ROWS ? 1 : kConvTile][kConvTile + 1];
   after_previous();
-  const int64_t tc = (p.n + kConvTile - 1) / kConvTile, tr = (p.m + kConvTile - 1) / kConvTile;
+  const int64_t tc = ROWS ? 1 : (p.n + kConvTile - 1) / kConvTile;
+  const int64_t tr = ROWS ? (p.m + kConvRows - 1) / kConvRows : (p.m + kConvTile - 1) / kConvTile;
   const int64_t b = blockIdx.x / (tc * tr), q = blockIdx.x % (tc * tr);
-  const int64_t r0 = q / tc * kConvTile, c0 = q % tc * kConvTile;
   int k;
   float sigma;
   norm_scale(p, b, &k, &sigma);
   if (q == 0 && threadIdx.x == 0) p.sigma[b] = sigma;
   const float s1 = scalbnf(1.f, k / 2), s2 = scalbnf(1.f, k - k / 2);
-  const bool along_c = p.sc <= p.sr;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < kConvTile * kConvTile; e += kPrepThreads) {
-    const int i = e / kConvTile, j = e % kConvTile;
-    const int r = along_c ? i : j, c = along_c ? j : i;
-    float x = 0.f;
-    if (r0 + r < p.m && c0 + c < p.n)
-      x = load_elem(p.g, b * p.sb + (r0 + r) * p.sr + (c0 + c) * p.sc, p.dtype) * s1 * s2;
-    tile[r][c] = x;
-  }
-  __syncthreads();
   __half* hi = p.x + b * 2 * p.m * p.ld;
   __half* lo = hi + p.m * p.ld;
-  for (int e = threadIdx.x; e < kConvTile * kConvTile / 4; e += kPrepThreads) {
-    const int r = e / (kConvTile / 4), c = e % (kConvTile / 4) * 4;
-    if (r0 + r >= p.m || c0 + c >= p.ld) continue;  // (ld is a multiple of 8)
-    __half h[4], l[4];
+  if constexpr (ROWS) {
+    const int64_t r0 = q * kConvRows;
+    const int per = int(p.n / 8), rows = int(p.m - r0 < kConvRows ? p.m - r0 : kConvRows);
+#pragma unroll 2
+    for (int e = threadIdx.x; e < rows * per; e += kPrepThreads) {
+      const int r = e / per, c = e % per * 8;
+      const int64_t at = b * p.sb + (r0 + r) * p.sr + c;
+      float v[8];
+      if constexpr (DT == NGDN2_F32) {
+        const uint4* g = reinterpret_cast<const uint4*>(static_cast<const float*>(p.g) + at);
+        const uint4 t0 = __ldg(g), t1 = __ldg(g + 1);
+        unpack16<DT>(t0, v);
+        unpack16<DT>(t1, v + 4);
+      } else {
+        unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.g) + at)), v);
+      }
+      alignas(16) __half h[8], l[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) split(tile[r][c + i], h[i], l[i]);
-    const int64_t o = (r0 + r) * p.ld + c0 + c;
-    *reinterpret_cast<uint2*>(hi + o) = *reinterpret_cast<const uint2*>(h);
-    *reinterpret_cast<uint2*>(lo + o) = *reinterpret_cast<const uint2*>(l);
+      for (int i = 0; i < 8; ++i) split(v[i] * s1 * s2, h[i], l[i]);
+      const int64_t o = (r0 + r) * p.ld + c;
+      *reinterpret_cast<uint4*>(hi + o) = *reinterpret_cast<const uint4*>(h);
+      if (p.lo) *reinterpret_cast<uint4*>(lo + o) = *reinterpret_cast<const uint4*>(l);
+    }
+  } else {
+    const int64_t r0 = q / tc * kConvTile, c0 = q % tc * kConvTile;
+    const bool along_c = p.sc <= p.sr;
+#pragma unroll 8
+    for (int e = threadIdx.x; e < kConvTile * kConvTile; e += kPrepThreads) {
+      const int i = e / kConvTile, j = e % kConvTile;
+      const int r = along_c ? i : j, c = along_c ? j : i;
+      float x = 0.f;
+      if (r0 + r < p.m && c0 + c < p.n)
+        x = load_typed<DT>(p.g, b * p.sb + (r0 + r) * p.sr + (c0 + c) * p.sc);
+      tile[r][c] = x;
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < kConvTile * kConvTile / 4; e += kPrepThreads) {
+      const int r = e / (kConvTile / 4), c = e % (kConvTile / 4) * 4;
+      if (r0 + r >= p.m || c0 + c >= p.ld) continue;  // (ld is a multiple of 8)
+      __half h[4], l[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) split(tile[r][c + i] * s1 * s2, h[i], l[i]);
+      const int64_t o = (r0 + r) * p.ld + c0 + c;
+      *reinterpret_cast<uint2*>(hi + o) = *reinterpret_cast<const uint2*>(h);
+      if (p.lo) *reinterpret_cast<uint2*>(lo + o) = *reinterpret_cast<const uint2*>(l);
+    }
   }
   let_next_start();
 }
@@ -165,7 +241,10 @@ constexpr int kPlane = 128 * kDepth * 2;  // bytes of one operand's plane in one
 constexpr int kStages = 3, kStageBytes = 4 * kPlane;
 constexpr int kMulThreads = 384;      // load, multiply, 2 idle warps, 8 that write results
 constexpr int kWriters = 8;
-constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
+// A writing warp's stage: 32 x 32 results, hi and lo, rows of 64 bytes (64-byte
+// swizzle), stored by TMA, which leaves out what lies past the matrix.
+constexpr int kOutPlane = 32 * 64, kOutBytes = kWriters * 2 * kOutPlane;
+constexpr int kSmem = kStages * kStageBytes + kOutBytes + 1024 + 256;
 
 struct MulArgs {
   int64_t batch, m, n;   // X is m x n
@@ -175,10 +254,10 @@ struct MulArgs {
   float a, b, c;
   const float* sigma;    // [batch], or NULL for 1 / kScale
   const __half* old;     // kPoly: the planes of A
-  __half* out;           // [batch][2][m][ld], or
-  void* final_out;       // the result (kApply)
+  __half* mirror;        // kGram, kPoly: the planes of the result, for direct stores
+  int64_t ld;            // of A and B
+  void* final_out;       // the result of the last kApply; others go to the planes of ``out``
   int out_dtype, transposed;
-  int64_t ld;
   int32_t* status;
 };
 
@@ -249,9 +328,10 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
       : "memory");
 }
 // Descriptor of a right operand that lies rows along the reduction: blocks of 64
-// columns (8 KB: 64 rows of 128 bytes, 128-byte swizzle), 8-row groups of 1 KB.
-__device__ __forceinline__ uint64_t desc_sw128_mn(uint32_t saddr) {
-  return (desc_sw128(saddr, 1024) & ~(uint64_t(0x3FFF) << 16)) | uint64_t(8192 >> 4) << 16;
+// columns (rows of 128 bytes, 128-byte swizzle) ``block`` bytes apart, 8-row groups
+// of 1 KB.
+__device__ __forceinline__ uint64_t desc_sw128_mn(uint32_t saddr, uint32_t block) {
+  return (desc_sw128(saddr, 1024) & ~(uint64_t(0x3FFF) << 16)) | uint64_t(block >> 4) << 16;
 }
 
 // A bounded wait that gives up for the whole CTA.
@@ -265,94 +345,71 @@ __device__ __forceinline__ bool wait_or_die(Barriers* s, uint64_t* bar, uint32_t
   return false;
 }
 
-// 32 neighbouring results of one row, from the accumulator's values v.
-template <int MODE>
-__device__ __forceinline__ void write32(const MulArgs& p, int64_t b, int64_t r, int64_t c, bool mirror,
-                                        float sigma, const float* v) {
-  const int64_t cols = MODE == kApply ? p.n : p.m;
-  const int left = int(cols - c < 32 ? cols - c : 32);
-  if (MODE == kApply && p.final_out) {
-    const float s = sigma / kScale;
-    if (p.transposed) {
+// The result's 32 neighbouring values of one row.
+__device__ __forceinline__ void write_final(const MulArgs& p, int64_t b, int64_t r, int64_t c, float s,
+                                            const float* v) {
+  const int left = int(p.n - c < 32 ? p.n - c : 32);
+  if (p.transposed) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (i < left) store_elem(p.final_out, (b * p.n + c + i) * p.m + r, s * v[i], p.out_dtype);
-    } else {
-      const int64_t o = (b * p.m + r) * p.n + c;
-      const int el = p.out_dtype == NGDN2_F32 ? 4 : 2;
-      char* to = static_cast<char*>(p.final_out) + o * el;
-      if (left == 32 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          alignas(16) unsigned char w[32];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) store_elem(w, j, s * v[i + j], p.out_dtype);
-          reinterpret_cast<uint4*>(to)[i * el / 16] = *reinterpret_cast<const uint4*>(w);
-          if (el == 4) reinterpret_cast<uint4*>(to)[i * el / 16 + 1] = *reinterpret_cast<const uint4*>(w + 16);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < left) store_elem(p.final_out, o + i, s * v[i], p.out_dtype);
-      }
-    }
+    for (int i = 0; i < 32; ++i)
+      if (i < left) store_elem(p.final_out, (b * p.n + c + i) * p.m + r, s * v[i], p.out_dtype);
     return;
   }
-  const int64_t rows = p.m, plane = rows * p.ld, at = r * p.ld + c;
-  const __half* old = p.old + b * 2 * plane;
-  __half* out = p.out + b * 2 * plane;
+  const int64_t o = (b * p.m + r) * p.n + c;
+  const int el = p.out_dtype == NGDN2_F32 ? 4 : 2;
+  char* to = static_cast<char*>(p.final_out) + o * el;
+  if (left == 32 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
 #pragma unroll
-  for (int i0 = 0; i0 < 32; i0 += 8) {
-    alignas(16) __half h[8], l[8], oh[8], ol[8];
-    const bool whole = i0 + 8 <= left;  // (rows are multiples of 8 apart)
-    if (MODE == kPoly) {
-      if (i0 < left) {  // (what lies past the row's end is not used)
-        *reinterpret_cast<uint4*>(oh) = *reinterpret_cast<const uint4*>(old + at + i0);
-        *reinterpret_cast<uint4*>(ol) = *reinterpret_cast<const uint4*>(old + plane + at + i0);
-      }
-    }
+    for (int i = 0; i < 32; i += 8) {
+      alignas(16) unsigned char w[32];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float x;
-      if (MODE == kGram) {
-        x = v[i0 + j] * sigma * sigma * kScale;
-      } else if (MODE == kPoly) {
-        x = p.c * (v[i0 + j] / kScale) + p.b * (__half2float(oh[j]) + __half2float(ol[j])) +
-            (c + i0 + j == r ? p.a * kScale : 0.f);
-      } else {
-        x = v[i0 + j] * sigma;  // sigma X^ B^ / kScale, times kScale
-      }
-      split(x, h[j], l[j]);
+      for (int j = 0; j < 8; ++j) store_elem(w, j, s * v[i + j], p.out_dtype);
+      reinterpret_cast<uint4*>(to)[i * el / 16] = *reinterpret_cast<const uint4*>(w);
+      if (el == 4) reinterpret_cast<uint4*>(to)[i * el / 16 + 1] = *reinterpret_cast<const uint4*>(w + 16);
     }
-    if (whole) {
-      *reinterpret_cast<uint4*>(out + at + i0) = *reinterpret_cast<const uint4*>(h);
-      *reinterpret_cast<uint4*>(out + plane + at + i0) = *reinterpret_cast<const uint4*>(l);
-    } else {
+  } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (i0 + j < left) {
-          out[at + i0 + j] = h[j];
-          out[plane + at + i0 + j] = l[j];
-        }
-    }
-    if (MODE != kApply && mirror) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (i0 + j < left) {
-          out[(c + i0 + j) * p.ld + r] = h[j];
-          out[plane + (c + i0 + j) * p.ld + r] = l[j];
-        }
-    }
+    for (int i = 0; i < 32; ++i)
+      if (i < left) store_elem(p.final_out, o + i, s * v[i], p.out_dtype);
   }
+}
+
+// Byte of element (row, col) in a writing warp's stage plane.
+__device__ __forceinline__ uint32_t out_at(int row, int col) {
+  return row * 64 + (((col >> 3) ^ (row >> 1 & 3)) << 4) + (col & 7) * 2;
+}
+
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int c0, int c1, int c2, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(c2), "r"(src)
+               : "memory");
+}
+
+// The stage's two planes to the matrix, from row r0 and column c0 on.
+__device__ __forceinline__ void store_stage(const CUtensorMap* map, int c0, int r0, int z, uint32_t stage) {
+  fence_proxy_async();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    store_box(map, c0, r0, z, stage);
+    store_box(map, c0, r0, z + 1, stage + kOutPlane);
+    bulk_commit();
+  }
+}
+
+// Before the stage is written again.
+__device__ __forceinline__ void stage_free() {
+  if ((threadIdx.x & 31) == 0) bulk_wait_read0();
+  __syncwarp();
 }
 
 template <int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMulThreads, 1)
 orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUtensorMap left,
-                const __grid_constant__ CUtensorMap right) {
+                const __grid_constant__ CUtensorMap right, const __grid_constant__ CUtensorMap out) {
   extern __shared__ unsigned char raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-  Barriers* s = reinterpret_cast<Barriers*>(raw + (base - smem_u32(raw)) + kStages * kStageBytes);
+  Barriers* s = reinterpret_cast<Barriers*>(raw + (base - smem_u32(raw)) + kStages * kStageBytes + kOutBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int64_t first = blockIdx.x / 2, step = gridDim.x / 2, total = p.batch * p.per;
@@ -437,7 +494,7 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
           auto L = [&](int pl) { return desc_sw128(at + pl * kPlane + kk * 32, 1024); };
           auto R = [&](int pl) {
             const uint32_t r = at + (2 + pl) * kPlane;
-            return MODE == kApply ? desc_sw128_mn(r + kk * 2048) : desc_sw128(r + kk * 32, 1024);
+            return MODE == kApply ? desc_sw128_mn(r + kk * 2048, kPlane / 2) : desc_sw128(r + kk * 32, 1024);
           };
           mma_pair(d, L(0), R(0), idesc, (k | kk) != 0);
           if (p.lo_right) mma_pair(d, L(0), R(1), idesc, 1);
@@ -456,23 +513,80 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
   } else if (warp >= 4) {
     uint32_t buf = 0, acc_phase = 0;
     const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t own = kStages * kStageBytes + (warp - 4) * 2 * kOutPlane, stage = base + own;
+    unsigned char* mem = raw + (base - smem_u32(raw)) + own;
     for (int64_t t = first; t < total; t += step) {
       int64_t b, tm, tn;
       tile_at<MODE>(p, t, &b, &tm, &tn);
-      if (!wait_or_die(s, &s->acc_full[buf], acc_phase, p.status)) break;
-      __syncwarp();
-      fence_after_sync();
-      const float sigma = p.sigma ? p.sigma[b] : 1.f / kScale;
-      const int64_t r = tm * kTile + rank * 128 + quarter * 32 + lane;
+      const int64_t r0 = tm * kTile + rank * 128 + quarter * 32, r = r0 + lane;
       const int64_t cols = MODE == kApply ? p.n : p.m;
+      const int z = int(b * 2);
+      const float sigma = p.sigma ? p.sigma[b] : 1.f / kScale;
+      // A's own values for 32 columns from c on; asked for ahead of the product.
+      uint4 oh[4], ol[4];
+      auto ask = [&](int64_t c) {
+        const __half* old = p.old + (int64_t(z) * p.m + r) * p.ld + c;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = r < p.m && c + 8 * i < cols;  // (a row has room for a multiple of 8)
+          oh[i] = in ? __ldg(reinterpret_cast<const uint4*>(old) + i) : make_uint4(0, 0, 0, 0);
+          ol[i] = in ? __ldg(reinterpret_cast<const uint4*>(old + p.m * p.ld) + i) : make_uint4(0, 0, 0, 0);
+        }
+      };
+      if (MODE == kPoly) ask(tn * kTile + half * (kTile / 2));
+      bool ready = false;
 #pragma unroll 1
       for (int c0 = half * (kTile / 2); c0 < (half + 1) * (kTile / 2); c0 += 32) {
         const int64_t c = tn * kTile + c0;
-        if (c >= cols) break;
+        if (c >= cols || r0 >= p.m) break;
+        if (!ready) {
+          if (!wait_or_die(s, &s->acc_full[buf], acc_phase, p.status)) goto done;
+          __syncwarp();
+          fence_after_sync();
+          ready = true;
+        }
         float v[32];
         tmem_ld32(taddr(tmem, quarter * 32, buf * kTile + c0), v);
-        if (r < p.m) write32<MODE>(p, b, r, c, tm != tn, sigma, v);
+        if (MODE == kApply && p.final_out) {
+          if (r < p.m) write_final(p, b, r, c, sigma / kScale, v);
+          continue;
+        }
+        __half h[32], l[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float x;
+          if (MODE == kGram) {
+            x = v[i] * sigma * sigma * kScale;
+          } else if (MODE == kPoly) {
+            const __half *ph = reinterpret_cast<const __half*>(oh), *pl = reinterpret_cast<const __half*>(ol);
+            x = p.c * (v[i] / kScale) + p.b * (__half2float(ph[i]) + __half2float(pl[i])) +
+                (c + i == r ? p.a * kScale : 0.f);
+          } else {
+            x = v[i] * sigma;  // (sigma X^) (B^ / kScale), times kScale
+          }
+          split(x, h[i], l[i]);
+        }
+        if (MODE == kPoly) ask(c + 32);
+        stage_free();
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          *reinterpret_cast<uint4*>(mem + out_at(lane, i)) = *reinterpret_cast<const uint4*>(h + i);
+          *reinterpret_cast<uint4*>(mem + kOutPlane + out_at(lane, i)) = *reinterpret_cast<const uint4*>(l + i);
+        }
+        store_stage(&out, int(c), int(r0), z, stage);
+        if (MODE != kApply && tm != tn && r < p.m) {
+          // The same below the diagonal: lanes are neighbours there. (Through the
+          // stage as well, each store would wait for the one before.)
+          __half* to = p.mirror + (int64_t(z) * p.m + c) * p.ld + r;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c + i < cols) {
+              to[i * p.ld] = h[i];
+              to[(p.m + i) * p.ld] = l[i];
+            }
+        }
       }
+      if (!ready && !wait_or_die(s, &s->acc_full[buf], acc_phase, p.status)) goto done;
       fence_before_sync();
       __syncwarp();
       if (lane == 0) arrive_at(in_first(&s->acc_empty[buf]));
@@ -481,6 +595,7 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
     }
   }
 done:
+  if (warp >= 4 && lane == 0) bulk_wait0();
   __syncwarp();
   fence_before_sync();
   __syncthreads();
@@ -488,6 +603,190 @@ done:
   if (warp == 2) {
     fence_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kTile) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Small matrices (m <= 128, n <= 256): the whole iteration in one CTA. X and A (then B
+// in its place) stay in shared memory as hi and lo planes in blocks of 64
+// columns, 128 rows of 128 bytes, 128-byte swizzled: as they lie they are left
+// and right operands with the reduction along the rows, and X is the right
+// operand with the reduction down the columns.
+// ---------------------------------------------------------------------------
+
+constexpr int kSmallM = 128, kSmallN = 256, kSmallThreads = 512;
+constexpr int kBlock = 128 * 128;  // bytes of one plane's 64 columns
+
+int small_smem(int64_t m, int64_t n) {
+  return int(2 * kBlock * ((n + 63) / 64 + (m + 63) / 64)) + 1024;
+}
+
+__device__ __forceinline__ uint32_t block_at(int r, int c) {
+  return (c >> 6) * kBlock + (r >> 3) * 1024 + (r & 7) * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4) + (c & 7) * 2;
+}
+
+struct SmallArgs {
+  PrepArgs in;
+  MulArgs out;
+  int steps;
+};
+
+template <int DT>
+__global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __grid_constant__ SmallArgs q) {
+  extern __shared__ unsigned char raw[];
+  __shared__ double red[kSmallThreads / 32];
+  __shared__ uint64_t bar;
+  __shared__ uint32_t tmem_at;
+  const PrepArgs& p = q.in;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int m = int(p.m), n = int(p.n);
+  const int64_t b = blockIdx.x;
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  unsigned char* mem = raw + (base - smem_u32(raw));
+  const int xp = kBlock * ((n + 63) / 64), ap = kBlock * ((m + 63) / 64);  // bytes of a plane
+  unsigned char *mx = mem, *ma = mem + 2 * xp;
+  const uint32_t ax = base, aa = base + 2 * xp;
+  if (tid == 0) {
+    mbar_init(&bar, 1);
+    fence_mbar_init();
+  }
+  if (warp == 0) tmem_alloc(&tmem_at, 256);
+  for (int i = tid * 16; i < 2 * (xp + ap); i += kSmallThreads * 16)
+    *reinterpret_cast<uint4*>(mem + i) = make_uint4(0, 0, 0, 0);
+  // The norm, then the planes of the scaled update. Threads along the
+  // dimension with the smaller stride.
+  const bool along_c = p.sc <= p.sr;
+  const int outer = along_c ? m : n, inner = along_c ? n : m;
+  const int64_t so = along_c ? p.sr : p.sc, si = along_c ? p.sc : p.sr;
+  auto each = [&](auto&& f) {  // a warp takes four rows at a time, their loads in flight together
+    constexpr int kWarps = kSmallThreads / 32;
+    for (int i0 = warp; i0 < outer; i0 += 4 * kWarps)
+#pragma unroll 4
+      for (int j = lane; j < inner; j += 32) {
+        float x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          x[u] = i0 + u * kWarps < outer ? load_typed<DT>(p.g, b * p.sb + (i0 + u * kWarps) * so + j * si) : 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int i = i0 + u * kWarps;
+          if (i < outer) f(along_c ? i : j, along_c ? j : i, x[u]);
+        }
+      }
+  };
+  double sum = 0.0;
+  each([&](int, int, float x) { sum = fma(double(x), double(x), sum); });
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) red[warp] = sum;
+  fence_before_sync();
+  __syncthreads();
+  fence_after_sync();
+  sum = 0.0;
+  for (int w = 0; w < kSmallThreads / 32; ++w) sum += red[w];
+  int k2;
+  float sigma;
+  scale_of(sum, p.eps, &k2, &sigma);
+  const float s1 = scalbnf(1.f, k2 / 2), s2 = scalbnf(1.f, k2 - k2 / 2);
+  each([&](int r, int c, float x) {
+    __half h, l;
+    split(x * s1 * s2, h, l);
+    *reinterpret_cast<__half*>(mx + block_at(r, c)) = h;
+    *reinterpret_cast<__half*>(mx + xp + block_at(r, c)) = l;
+  });
+  const uint32_t tmem = tmem_at;
+  const int quarter = warp & 3, c1 = (warp >> 2) * 32, row = quarter * 32 + lane;
+  const int mn = (m + 15) & ~15, nn = (n + 15) & ~15;
+  uint32_t phase = 0;
+  bool alive = true;
+
+  // D[128 x cols] = L R, reduction over ``depth`` (multiples of 16).
+  auto product = [&](uint32_t L, int lp, uint32_t R, int rp, int depth, int cols, bool down) {
+    fence_proxy_async();
+    fence_before_sync();
+    __syncthreads();
+    if (tid == 0) {
+      fence_after_sync();
+      const uint32_t idesc = idesc_f16(128, cols, false, false, down);
+      for (int kk = 0; kk < depth / 16; ++kk) {
+        auto dl = [&](int pl) { return desc_sw128(L + pl * lp + (kk >> 2) * kBlock + (kk & 3) * 32, 1024); };
+        auto dr = [&](int pl) {
+          return down ? desc_sw128_mn(R + pl * rp + kk * 2048, kBlock)
+                      : desc_sw128(R + pl * rp + (kk >> 2) * kBlock + (kk & 3) * 32, 1024);
+        };
+        mma_f16(tmem, dl(0), dr(0), idesc, kk > 0);
+        mma_f16(tmem, dl(0), dr(1), idesc, 1);
+        mma_f16(tmem, dl(1), dr(0), idesc, 1);
+      }
+      mma_commit(&bar);
+    }
+    const bool ok = mbar_wait(&bar, phase, 1u << 20);
+    phase ^= 1;
+    fence_after_sync();
+    if (!ok) atomicOr(q.out.status, NGDN2_STATUS_WAIT_TIMEOUT);
+    return !__syncthreads_or(!ok);
+  };
+  // Eight results as planes.
+  auto put8 = [&](unsigned char* to, int plane, int c, const float* x) {
+    alignas(16) __half h[8], l[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) split(x[j], h[j], l[j]);
+    *reinterpret_cast<uint4*>(to + block_at(row, c)) = *reinterpret_cast<const uint4*>(h);
+    *reinterpret_cast<uint4*>(to + plane + block_at(row, c)) = *reinterpret_cast<const uint4*>(l);
+  };
+
+  for (int step = 0; step < q.steps && alive; ++step, sigma = 1.f / kScale) {
+    float v[32];
+    alive = product(ax, xp, ax, xp, nn, mn, false);
+    if (!alive) break;
+    for (int c = c1; c < m; c += 128) {
+      tmem_ld32(taddr(tmem, quarter * 32, c), v);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = c + i < m ? v[i] * sigma * sigma * kScale : 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) put8(ma, ap, c + i, v + i);
+    }
+    alive = product(aa, ap, aa, ap, mn, mn, false);
+    if (!alive) break;
+    for (int c = c1; c < m; c += 128) {
+      tmem_ld32(taddr(tmem, quarter * 32, c), v);
+#pragma unroll
+      for (int i = 0; i < 32; i += 8) {
+        alignas(16) __half h[8], l[8];
+        *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(ma + block_at(row, c + i));
+        *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(ma + ap + block_at(row, c + i));
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          v[i + j] = c + i + j < m ? q.out.c * (v[i + j] / kScale) +
+                                         q.out.b * (__half2float(h[j]) + __half2float(l[j])) +
+                                         (c + i + j == row ? q.out.a * kScale : 0.f)
+                                   : 0.f;
+        put8(ma, ap, c + i, v + i);
+      }
+    }
+    alive = product(aa, ap, ax, xp, mn, nn, true);
+    if (!alive) break;
+    for (int c = c1; c < n; c += 128) {
+      tmem_ld32(taddr(tmem, quarter * 32, c), v);
+      if (step + 1 == q.steps) {
+        if (row < m) write_final(q.out, b, row, c, sigma / kScale, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = c + i < n ? v[i] * sigma : 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) put8(mx, xp, c + i, v + i);
+      }
+    }
+  }
+  if (!alive) {  // nothing that was not computed passes as a result
+    for (int e = tid; e < m * n; e += kSmallThreads)
+      store_elem(q.out.final_out, b * m * n + e, __int_as_float(0x7fc00000), q.out.out_dtype);
+  }
+  fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    fence_after_sync();
+    tmem_dealloc(tmem, 256);
   }
 }
 
@@ -499,7 +798,7 @@ orth_scale_kernel(const __grid_constant__ PrepArgs p, void* out, int out_dtype, 
   if (i >= p.batch * p.m * p.n) return;
   const int64_t b = i / (p.m * p.n), r = i / p.n % p.m, c = i % p.n;
   const __half* hi = p.x + b * 2 * p.m * p.ld + r * p.ld + c;
-  const float x = (__half2float(hi[0]) + __half2float(hi[p.m * p.ld])) * p.sigma[b];
+  const float x = (__half2float(hi[0]) + (p.lo ? __half2float(hi[p.m * p.ld]) : 0.f)) * p.sigma[b];
   store_elem(out, b * p.m * p.n + (transposed ? c * p.m + r : r * p.n + c), x, out_dtype);
 }
 
@@ -507,8 +806,18 @@ orth_scale_kernel(const __grid_constant__ PrepArgs p, void* out, int out_dtype, 
 // Host
 // ---------------------------------------------------------------------------
 
+template <class F>
+cudaError_t by_type(int dt, F&& f) {
+  switch (dt) {
+    case NGDN2_BF16: return f(std::integral_constant<int, NGDN2_BF16>{});
+    case NGDN2_F16: return f(std::integral_constant<int, NGDN2_F16>{});
+    default: return f(std::integral_constant<int, NGDN2_F32>{});
+  }
+}
+
 struct OrthLayout {
   int64_t m, n, ldx, lda;
+  int parts;
   size_t x, y, A, B, part, sigma, total;
 };
 
@@ -518,6 +827,7 @@ OrthLayout layout(const ngdn2_orth_args* a) {
   L.n = a->rows < a->cols ? a->cols : a->rows;
   L.ldx = (L.n + 7) / 8 * 8;
   L.lda = (L.m + 7) / 8 * 8;
+  L.parts = a->batch >= 8 ? 64 : kNormPartsMost;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
@@ -528,7 +838,7 @@ OrthLayout layout(const ngdn2_orth_args* a) {
   L.y = take(size_t(a->batch) * 2 * L.m * L.ldx * 2);
   L.A = take(size_t(a->batch) * 2 * L.m * L.lda * 2);
   L.B = take(size_t(a->batch) * 2 * L.m * L.lda * 2);
-  L.part = take(size_t(a->batch) * kNormParts * sizeof(double));
+  L.part = take(size_t(a->batch) * L.parts * sizeof(double));
   L.sigma = take(size_t(a->batch) * sizeof(float));
   L.total = at + 256;
   return L;
@@ -546,20 +856,24 @@ PFN_cuTensorMapEncodeTiled encoder() {
   return fn;
 }
 
-// Planes [batch][2][rows][ld] as boxes of 64 columns by ``box`` rows, 128-byte
-// swizzled; zeros outside [rows, cols].
-bool make_map(CUtensorMap* map, const __half* p, int64_t batch, int64_t rows, int64_t cols, int64_t ld, int box) {
+// Planes [batch][2][rows][ld] as boxes of ``width`` columns by ``box`` rows,
+// swizzled over the box's rows (64 columns: 128 bytes, 32: 64); zeros outside
+// [rows, cols].
+bool make_map(CUtensorMap* map, const __half* p, int64_t batch, int64_t rows, int64_t cols, int64_t ld, int box,
+              int width = kDepth) {
   const cuuint64_t dims[3] = {cuuint64_t(cols), cuuint64_t(rows), cuuint64_t(batch) * 2};
   const cuuint64_t strides[2] = {cuuint64_t(ld) * 2, cuuint64_t(rows) * ld * 2};
-  const cuuint32_t boxes[3] = {kDepth, cuuint32_t(box), 1}, ones[3] = {1, 1, 1};
+  const cuuint32_t boxes[3] = {cuuint32_t(width), cuuint32_t(box), 1}, ones[3] = {1, 1, 1};
   return encoder() &&
          encoder()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(p), dims, strides, boxes, ones,
-                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   width == kDepth ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int MODE>
-cudaError_t multiply(MulArgs p, const CUtensorMap& left, const CUtensorMap& right, int sms, cudaStream_t st) {
+cudaError_t multiply(MulArgs p, const CUtensorMap& left, const CUtensorMap& right, const CUtensorMap& out, int sms,
+                     cudaStream_t st) {
   p.nt = (p.m + kTile - 1) / kTile;
   p.tiles_n = MODE == kApply ? (p.n + kTile - 1) / kTile : p.nt;
   p.per = MODE == kApply ? p.nt * p.tiles_n : p.nt * (p.nt + 1) / 2;
@@ -567,7 +881,7 @@ cudaError_t multiply(MulArgs p, const CUtensorMap& left, const CUtensorMap& righ
   if (e != cudaSuccess) return e;
   const int64_t total = p.batch * p.per, pairs = sms / 2;
   return launch_next(orth_mul_kernel<MODE>, dim3(unsigned(2 * (total < pairs ? total : pairs))), dim3(kMulThreads),
-                     kSmem, st, true, p, left, right);
+                     kSmem, st, true, p, left, right, out);
 }
 
 // The scalar iteration s <- s (a + b s^2 + c s^4) from every start in [0, 1]
@@ -622,7 +936,6 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
   const bool tall = a->rows > a->cols;
   PrepArgs pr;
   pr.g = a->update;
-  pr.dtype = a->dtype;
   pr.batch = a->batch;
   pr.m = L.m;
   pr.n = L.n;
@@ -634,11 +947,45 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
   pr.sigma = reinterpret_cast<float*>(ws + L.sigma);
   pr.x = x;
   pr.ld = L.ldx;
-  const int64_t conv = a->batch * ((L.m + kConvTile - 1) / kConvTile) * ((L.n + kConvTile - 1) / kConvTile);
+  pr.parts = L.parts;
+  pr.lo = a->dtype == NGDN2_F32;  // 16-bit updates fit their hi plane
+  if (a->steps > 0 && L.m <= kSmallM && L.n <= kSmallN) {
+    SmallArgs q{};
+    q.in = pr;
+    q.out.m = L.m;
+    q.out.n = L.n;
+    q.out.a = a->coef[0];
+    q.out.b = a->coef[1];
+    q.out.c = a->coef[2];
+    q.out.final_out = a->out;
+    q.out.out_dtype = a->out_dtype;
+    q.out.transposed = tall;
+    q.out.status = a->status;
+    q.steps = a->steps;
+    const int smem = small_smem(L.m, L.n);
+    const cudaError_t e = by_type(a->dtype, [&](auto T) {
+      auto* kernel = orth_small_kernel<decltype(T)::value>;
+      const cudaError_t f = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      return f != cudaSuccess ? f
+                              : launch_next(kernel, dim3(unsigned(a->batch)), dim3(kSmallThreads), smem, st, false, q);
+    });
+    return e == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
+  }
+  const int64_t el = a->dtype == NGDN2_F32 ? 4 : 2;
+  const bool on16 = reinterpret_cast<uintptr_t>(a->update) % 16 == 0 && pr.sb * el % 16 == 0;
+  const bool flat = on16 && a->update_stride[2] == 1 && a->update_stride[1] == a->cols;
+  const bool rows = on16 && pr.sc == 1 && pr.sr * el % 16 == 0 && L.n % 8 == 0;
+  const int64_t conv = a->batch * (rows ? (L.m + kConvRows - 1) / kConvRows
+                                        : (L.m + kConvTile - 1) / kConvTile * ((L.n + kConvTile - 1) / kConvTile));
   if (conv >= (int64_t(1) << 31)) return NGDN2_ERR_SHAPE;
-  cudaError_t e = launch_next(orth_norm_kernel, dim3(unsigned(a->batch * kNormParts)), dim3(kPrepThreads), 0, st, false, pr);
-  if (e == cudaSuccess)
-    e = launch_next(orth_convert_kernel, dim3(unsigned(conv)), dim3(kPrepThreads), 0, st, true, pr);
+  cudaError_t e = by_type(a->dtype, [&](auto T) {
+    constexpr int DT = decltype(T)::value;
+    const dim3 grid(unsigned(a->batch * L.parts)), block(kPrepThreads);
+    const cudaError_t f = launch_next(flat ? orth_norm_kernel<DT, true> : orth_norm_kernel<DT, false>, grid, block, 0, st, false, pr);
+    return f != cudaSuccess ? f
+                            : launch_next(rows ? orth_convert_kernel<DT, true> : orth_convert_kernel<DT, false>,
+                                          dim3(unsigned(conv)), block, 0, st, true, pr);
+  });
   if (e != cudaSuccess) return NGDN2_ERR_CUDA;
   if (a->steps == 0) {
     const int64_t n = (a->batch * L.m * L.n + kPrepThreads - 1) / kPrepThreads;
@@ -646,11 +993,15 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
                     a->out_dtype, int(tall));
     return e == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
   }
-  // Operands: rows of X, A or B (128 rows a box), and X rows along the reduction (64).
-  CUtensorMap mx[2], mxr[2], mA, mB;
+  // Operands: rows of X, A or B (128 rows a box), and X rows along the reduction
+  // (64); results (32 x 32).
+  CUtensorMap mx[2], mxr[2], mxo[2], mA, mB, mAo, mBo;
   if (!make_map(&mx[0], x, a->batch, L.m, L.n, L.ldx, 128) || !make_map(&mx[1], y, a->batch, L.m, L.n, L.ldx, 128) ||
       !make_map(&mxr[0], x, a->batch, L.m, L.n, L.ldx, 64) || !make_map(&mxr[1], y, a->batch, L.m, L.n, L.ldx, 64) ||
-      !make_map(&mA, A, a->batch, L.m, L.m, L.lda, 128) || !make_map(&mB, B, a->batch, L.m, L.m, L.lda, 128))
+      !make_map(&mA, A, a->batch, L.m, L.m, L.lda, 128) || !make_map(&mB, B, a->batch, L.m, L.m, L.lda, 128) ||
+      !make_map(&mxo[0], x, a->batch, L.m, L.n, L.ldx, 32, 32) ||
+      !make_map(&mxo[1], y, a->batch, L.m, L.n, L.ldx, 32, 32) ||
+      !make_map(&mAo, A, a->batch, L.m, L.m, L.lda, 32, 32) || !make_map(&mBo, B, a->batch, L.m, L.m, L.lda, 32, 32))
     return NGDN2_ERR_CUDA;
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -674,22 +1025,20 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
     p.final_out = nullptr;
     p.depth = L.n;
     p.lo_left = p.lo_right = lo;
-    p.out = A;
     p.ld = L.lda;
-    e = multiply<kGram>(p, mx[in], mx[in], sms, st);
+    p.mirror = A;
+    e = multiply<kGram>(p, mx[in], mx[in], mAo, sms, st);
     if (e != cudaSuccess) break;
     p.depth = L.m;
     p.lo_left = p.lo_right = true;
     p.old = A;
-    p.out = B;
-    e = multiply<kPoly>(p, mA, mA, sms, st);
+    p.mirror = B;
+    e = multiply<kPoly>(p, mA, mA, mBo, sms, st);
     if (e != cudaSuccess) break;
     p.old = nullptr;
     p.lo_right = lo;
-    p.out = in ? x : y;
-    p.ld = L.ldx;
     p.final_out = k + 1 == a->steps ? a->out : nullptr;
-    e = multiply<kApply>(p, mB, mxr[in], sms, st);
+    e = multiply<kApply>(p, mB, mxr[in], mxo[1 - in], sms, st);
   }
   return e == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
 }
