@@ -19,12 +19,14 @@
 // (both symmetric: tiles on and above the diagonal only, written twice) and
 // X' = B X, which reads X as it lies, rows along the reduction.
 //
-// Products: a pair of CTAs computes 256 x 256 tiles (tcgen05, cta_group::2; each
-// CTA holds its 128 rows of the left operand and half of the right one), fed
-// by a thread that issues TMA loads three 64-deep stages ahead, with two
-// accumulators in tensor memory so that one tile's results are written while
-// the next is multiplied. The pair tile halves what each multiprocessor must
-// read: 64 KB a stage for 12 MMAs.
+// Products: a pair of CTAs computes tiles of 256 rows by 256 or 128 columns
+// (tcgen05, cta_group::2; each CTA holds its 128 rows of the left operand and
+// half of the right one), fed by a thread that issues TMA loads of 64-deep
+// stages ahead, with two accumulators in tensor memory so that one tile's
+// results are written while the next is multiplied. The pair tile halves what
+// each multiprocessor must read: 64 KB a stage for 12 MMAs of 256 columns. The
+// narrower tile reads more for each MMA, but few tiles finish sooner. Either
+// sums in the same order, so a matrix has the same bits in any batch.
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -59,7 +61,7 @@ __device__ __forceinline__ void split(float x, __half& hi, __half& lo) {
 // Norm and conversion
 // ---------------------------------------------------------------------------
 
-constexpr int kPrepThreads = 256, kNormPartsMost = 256;
+constexpr int kPrepThreads = 256, kNormParts = 128;
 
 struct PrepArgs {
   const void* g;
@@ -235,21 +237,33 @@ __global__ void __launch_bounds__(kPrepThreads) orth_convert_kernel(const __grid
 
 enum { kGram = 0, kPoly = 1, kApply = 2 };  // A = X X^T; B = a I + b A + c A A; X' = B X
 
-constexpr int kTile = 256;            // rows and columns of a pair's tile
+constexpr int kRows = 256;            // of a pair's tile
 constexpr int kDepth = 64;            // reduction elements of a stage
-constexpr int kPlane = 128 * kDepth * 2;  // bytes of one operand's plane in one CTA, a stage
-constexpr int kStages = 3, kStageBytes = 4 * kPlane;
+constexpr int kLeft = 128 * kDepth * 2;  // bytes of the left operand's plane in one CTA, a stage
+constexpr int kBox = 64 * kDepth * 2;    // of 64 of the right operand's columns
+
+// Tiles of BN columns: a stage holds both operands' planes; as many stages as
+// fit beside the results' stage.
+template <int BN>
+struct Shape {
+  static constexpr int kRight = BN / 128 * kBox;
+  static constexpr int kStage = 2 * (kLeft + kRight);
+  static constexpr int kStages = BN == 256 ? 3 : 4;
+};
+constexpr int kStagesMost = 4;
 constexpr int kMulThreads = 384;      // load, multiply, 2 idle warps, 8 that write results
 constexpr int kWriters = 8;
 // A writing warp's stage: 32 x 32 results, hi and lo, rows of 64 bytes (64-byte
 // swizzle), stored by TMA, which leaves out what lies past the matrix.
 constexpr int kOutPlane = 32 * 64, kOutBytes = kWriters * 2 * kOutPlane;
-constexpr int kSmem = kStages * kStageBytes + kOutBytes + 1024 + 256;
+constexpr int kSmem = 3 * 65536 + kOutBytes + 1024 + 256;
+static_assert(Shape<256>::kStages * Shape<256>::kStage == 3 * 65536, "");
+static_assert(Shape<128>::kStages * Shape<128>::kStage == 3 * 65536, "");
 
 struct MulArgs {
   int64_t batch, m, n;   // X is m x n
   int64_t depth;         // of the reduction
-  int64_t nt, tiles_n, per;  // row tiles, column tiles, tiles of a matrix
+  int64_t tiles_n, per;  // column tiles, tiles of a matrix
   bool lo_left, lo_right;    // whether the operands' lo planes are read
   float a, b, c;
   const float* sigma;    // [batch], or NULL for 1 / kScale
@@ -262,13 +276,13 @@ struct MulArgs {
 };
 
 struct Barriers {
-  uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+  uint64_t full[kStagesMost], empty[kStagesMost], acc_full[2], acc_empty[2];
   uint32_t tmem;
   int dead;
 };
 
-// Tile number t of a matrix: all of them, or those on and above the diagonal.
-template <int MODE>
+// Tile number t: all of a matrix's, or those that reach the diagonal or lie above it.
+template <int MODE, int BN>
 __device__ __forceinline__ void tile_at(const MulArgs& p, int64_t t, int64_t* b, int64_t* tm, int64_t* tn) {
   *b = t / p.per;
   int64_t q = t % p.per;
@@ -276,14 +290,14 @@ __device__ __forceinline__ void tile_at(const MulArgs& p, int64_t t, int64_t* b,
     *tm = q / p.tiles_n;
     *tn = q % p.tiles_n;
   } else {
-    int64_t r = 0, len = p.nt;
+    int64_t r = 0, len = p.tiles_n;
     while (q >= len) {
       q -= len;
-      --len;
+      len -= kRows / BN;
       ++r;
     }
     *tm = r;
-    *tn = r + q;
+    *tn = r * (kRows / BN) + q;
   }
 }
 
@@ -403,13 +417,62 @@ __device__ __forceinline__ void stage_free() {
   __syncwarp();
 }
 
+// A row's 32 neighbouring results, from the sums v: to the planes by way of the
+// warp's stage, or the final values. Whole warps; r0 is lane 0's row.
 template <int MODE>
+__device__ __forceinline__ void emit32(const MulArgs& p, const CUtensorMap* out, unsigned char* mem, int64_t b,
+                                       int64_t r0, int64_t c, bool mirror, float sigma, const float* v,
+                                       const uint4* oh, const uint4* ol) {
+  const int lane = threadIdx.x & 31, z = int(b * 2);
+  const int64_t r = r0 + lane, cols = MODE == kApply ? p.n : p.m;
+  if (MODE == kApply && p.final_out) {
+    if (r < p.m) write_final(p, b, r, c, sigma / kScale, v);
+    return;
+  }
+  __half h[32], l[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    float x;
+    if (MODE == kGram) {
+      x = v[i] * sigma * sigma * kScale;
+    } else if (MODE == kPoly) {
+      const __half *ph = reinterpret_cast<const __half*>(oh), *pl = reinterpret_cast<const __half*>(ol);
+      x = p.c * (v[i] / kScale) + p.b * (__half2float(ph[i]) + __half2float(pl[i])) +
+          (c + i == r ? p.a * kScale : 0.f);
+    } else {
+      x = v[i] * sigma;  // (sigma X^) (B^ / kScale), times kScale
+    }
+    split(x, h[i], l[i]);
+  }
+  stage_free();
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    *reinterpret_cast<uint4*>(mem + out_at(lane, i)) = *reinterpret_cast<const uint4*>(h + i);
+    *reinterpret_cast<uint4*>(mem + kOutPlane + out_at(lane, i)) = *reinterpret_cast<const uint4*>(l + i);
+  }
+  store_stage(out, int(c), int(r0), z, smem_u32(mem));
+  if (MODE != kApply && mirror && r < p.m) {
+    // The same below the diagonal: lanes are neighbours there. (Through the
+    // stage as well, each store would wait for the one before.)
+    __half* to = p.mirror + (int64_t(z) * p.m + c) * p.ld + r;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (c + i < cols) {
+        to[i * p.ld] = h[i];
+        to[(p.m + i) * p.ld] = l[i];
+      }
+  }
+}
+
+template <int MODE, int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMulThreads, 1)
 orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUtensorMap left,
                 const __grid_constant__ CUtensorMap right, const __grid_constant__ CUtensorMap out) {
+  constexpr int kStages = Shape<BN>::kStages, kStage = Shape<BN>::kStage, kRight = Shape<BN>::kRight;
   extern __shared__ unsigned char raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
-  Barriers* s = reinterpret_cast<Barriers*>(raw + (base - smem_u32(raw)) + kStages * kStageBytes + kOutBytes);
+  unsigned char* const smem = raw + (base - smem_u32(raw));
+  Barriers* s = reinterpret_cast<Barriers*>(smem + kStages * kStage + kOutBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int64_t first = blockIdx.x / 2, step = gridDim.x / 2, total = p.batch * p.per;
@@ -428,7 +491,7 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
   }
   if (warp == 2) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s->tmem)),
-                 "r"(2 * kTile)
+                 "r"(2 * BN)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
@@ -440,30 +503,43 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
   after_previous();
   let_next_start();
 
+  // A writing warp's rows and columns, its stage, and A's own values for 32
+  // columns from c on, asked for ahead of the product.
+  const int quarter = warp & 3, half = (warp >> 2) - 1;
+  unsigned char* const mem = smem + kStages * kStage + (warp - 4) * 2 * kOutPlane;
+  uint4 oh[4], ol[4];
+  auto ask = [&](int64_t b, int64_t r, int64_t c) {
+    const __half* old = p.old + (b * 2 * p.m + r) * p.ld + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = r < p.m && c + 8 * i < p.m;  // (a row has room for a multiple of 8)
+      oh[i] = in ? __ldg(reinterpret_cast<const uint4*>(old) + i) : make_uint4(0, 0, 0, 0);
+      ol[i] = in ? __ldg(reinterpret_cast<const uint4*>(old + p.m * p.ld) + i) : make_uint4(0, 0, 0, 0);
+    }
+  };
+
   if (warp == 0 && lane == 0) {
     // Loads of this CTA's halves: 128 rows of the left operand, 128 rows (or
     // columns, kApply) of the right one, hi and lo.
     uint32_t st = 0, phase = 0;
-    const uint32_t bytes = 2 * kPlane * (2 + (p.lo_left ? 1 : 0) + (p.lo_right ? 1 : 0));
+    const uint32_t bytes = 2 * (kLeft * (p.lo_left ? 2 : 1) + kRight * (p.lo_right ? 2 : 1));
     for (int64_t t = first; t < total; t += step) {
       int64_t b, tm, tn;
-      tile_at<MODE>(p, t, &b, &tm, &tn);
-      const int row = int(tm * kTile + rank * 128), col = int(tn * kTile + rank * 128), z = int(b * 2);
+      tile_at<MODE, BN>(p, t, &b, &tm, &tn);
+      const int row = int(tm * kRows + rank * 128), col = int(tn * BN + rank * (BN / 2)), z = int(b * 2);
       for (int k = 0; k < blocks; ++k) {
         if (!wait_or_die(s, &s->empty[st], phase ^ 1, p.status)) goto done;
-        const uint32_t at = base + st * kStageBytes, bar = in_first(&s->full[st]);
+        const uint32_t at = base + st * kStage, bar = in_first(&s->full[st]);
         if (rank == 0) mbar_arrive_expect_tx(&s->full[st], bytes);
         for (int pl = 0; pl < 2; ++pl) {
-          if (pl == 0 || p.lo_left) load_box(at + pl * kPlane, &left, k * kDepth, row, z + pl, bar);
-          if (pl == 0 || p.lo_right) {
-            const uint32_t to = at + (2 + pl) * kPlane;
-            if (MODE == kApply) {
-              load_box(to, &right, col, k * kDepth, z + pl, bar);
-              load_box(to + kPlane / 2, &right, col + 64, k * kDepth, z + pl, bar);
-            } else {
-              load_box(to, &right, k * kDepth, col, z + pl, bar);
+          if (pl == 0 || p.lo_left) load_box(at + pl * kLeft, &left, k * kDepth, row, z + pl, bar);
+          if (pl == 0 || p.lo_right)
+#pragma unroll
+            for (int i = 0; i < BN / 128; ++i) {
+              const uint32_t to = at + 2 * kLeft + pl * kRight + i * kBox;
+              if (MODE == kApply) load_box(to, &right, col + 64 * i, k * kDepth, z + pl, bar);
+              else load_box(to, &right, k * kDepth, col + 64 * i, z + pl, bar);
             }
-          }
         }
         if (++st == kStages) {
           st = 0;
@@ -480,21 +556,21 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
       }
     }
   } else if (warp == 1 && lane == 0 && rank == 0) {
-    const uint32_t idesc = idesc_f16(256, kTile, false, false, MODE == kApply);
+    const uint32_t idesc = idesc_f16(kRows, BN, false, false, MODE == kApply);
     uint32_t st = 0, phase = 0, buf = 0, acc_phase = 0;
     for (int64_t t = first; t < total; t += step) {
       if (!wait_or_die(s, &s->acc_empty[buf], acc_phase ^ 1, p.status)) goto done;
-      const uint32_t d = tmem + buf * kTile;
+      const uint32_t d = tmem + buf * BN;
       for (int k = 0; k < blocks; ++k) {
         if (!wait_or_die(s, &s->full[st], phase, p.status)) goto done;
         fence_after_sync();
-        const uint32_t at = base + st * kStageBytes;
+        const uint32_t at = base + st * kStage;
 #pragma unroll
         for (int kk = 0; kk < kDepth / 16; ++kk) {
-          auto L = [&](int pl) { return desc_sw128(at + pl * kPlane + kk * 32, 1024); };
+          auto L = [&](int pl) { return desc_sw128(at + pl * kLeft + kk * 32, 1024); };
           auto R = [&](int pl) {
-            const uint32_t r = at + (2 + pl) * kPlane;
-            return MODE == kApply ? desc_sw128_mn(r + kk * 2048, kPlane / 2) : desc_sw128(r + kk * 32, 1024);
+            const uint32_t r = at + 2 * kLeft + pl * kRight;
+            return MODE == kApply ? desc_sw128_mn(r + kk * 2048, kBox) : desc_sw128(r + kk * 32, 1024);
           };
           mma_pair(d, L(0), R(0), idesc, (k | kk) != 0);
           if (p.lo_right) mma_pair(d, L(0), R(1), idesc, 1);
@@ -512,81 +588,25 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
     }
   } else if (warp >= 4) {
     uint32_t buf = 0, acc_phase = 0;
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
-    const uint32_t own = kStages * kStageBytes + (warp - 4) * 2 * kOutPlane, stage = base + own;
-    unsigned char* mem = raw + (base - smem_u32(raw)) + own;
     for (int64_t t = first; t < total; t += step) {
       int64_t b, tm, tn;
-      tile_at<MODE>(p, t, &b, &tm, &tn);
-      const int64_t r0 = tm * kTile + rank * 128 + quarter * 32, r = r0 + lane;
-      const int64_t cols = MODE == kApply ? p.n : p.m;
-      const int z = int(b * 2);
+      tile_at<MODE, BN>(p, t, &b, &tm, &tn);
+      const int64_t r0 = tm * kRows + rank * 128 + quarter * 32, cols = MODE == kApply ? p.n : p.m;
+      const bool mirror = tn / (kRows / BN) != tm;
       const float sigma = p.sigma ? p.sigma[b] : 1.f / kScale;
-      // A's own values for 32 columns from c on; asked for ahead of the product.
-      uint4 oh[4], ol[4];
-      auto ask = [&](int64_t c) {
-        const __half* old = p.old + (int64_t(z) * p.m + r) * p.ld + c;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool in = r < p.m && c + 8 * i < cols;  // (a row has room for a multiple of 8)
-          oh[i] = in ? __ldg(reinterpret_cast<const uint4*>(old) + i) : make_uint4(0, 0, 0, 0);
-          ol[i] = in ? __ldg(reinterpret_cast<const uint4*>(old + p.m * p.ld) + i) : make_uint4(0, 0, 0, 0);
-        }
-      };
-      if (MODE == kPoly) ask(tn * kTile + half * (kTile / 2));
-      bool ready = false;
+      if (MODE == kPoly) ask(b, r0 + lane, tn * BN + half * (BN / 2));
+      if (!wait_or_die(s, &s->acc_full[buf], acc_phase, p.status)) goto done;
+      __syncwarp();
+      fence_after_sync();
 #pragma unroll 1
-      for (int c0 = half * (kTile / 2); c0 < (half + 1) * (kTile / 2); c0 += 32) {
-        const int64_t c = tn * kTile + c0;
+      for (int c0 = half * (BN / 2); c0 < (half + 1) * (BN / 2); c0 += 32) {
+        const int64_t c = tn * BN + c0;
         if (c >= cols || r0 >= p.m) break;
-        if (!ready) {
-          if (!wait_or_die(s, &s->acc_full[buf], acc_phase, p.status)) goto done;
-          __syncwarp();
-          fence_after_sync();
-          ready = true;
-        }
         float v[32];
-        tmem_ld32(taddr(tmem, quarter * 32, buf * kTile + c0), v);
-        if (MODE == kApply && p.final_out) {
-          if (r < p.m) write_final(p, b, r, c, sigma / kScale, v);
-          continue;
-        }
-        __half h[32], l[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          float x;
-          if (MODE == kGram) {
-            x = v[i] * sigma * sigma * kScale;
-          } else if (MODE == kPoly) {
-            const __half *ph = reinterpret_cast<const __half*>(oh), *pl = reinterpret_cast<const __half*>(ol);
-            x = p.c * (v[i] / kScale) + p.b * (__half2float(ph[i]) + __half2float(pl[i])) +
-                (c + i == r ? p.a * kScale : 0.f);
-          } else {
-            x = v[i] * sigma;  // (sigma X^) (B^ / kScale), times kScale
-          }
-          split(x, h[i], l[i]);
-        }
-        if (MODE == kPoly) ask(c + 32);
-        stage_free();
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          *reinterpret_cast<uint4*>(mem + out_at(lane, i)) = *reinterpret_cast<const uint4*>(h + i);
-          *reinterpret_cast<uint4*>(mem + kOutPlane + out_at(lane, i)) = *reinterpret_cast<const uint4*>(l + i);
-        }
-        store_stage(&out, int(c), int(r0), z, stage);
-        if (MODE != kApply && tm != tn && r < p.m) {
-          // The same below the diagonal: lanes are neighbours there. (Through the
-          // stage as well, each store would wait for the one before.)
-          __half* to = p.mirror + (int64_t(z) * p.m + c) * p.ld + r;
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c + i < cols) {
-              to[i * p.ld] = h[i];
-              to[(p.m + i) * p.ld] = l[i];
-            }
-        }
+        tmem_ld32(taddr(tmem, quarter * 32, buf * BN + c0), v);
+        emit32<MODE>(p, &out, mem, b, r0, c, mirror, sigma, v, oh, ol);
+        if (MODE == kPoly) ask(b, r0 + lane, c + 32);
       }
-      if (!ready && !wait_or_die(s, &s->acc_full[buf], acc_phase, p.status)) goto done;
       fence_before_sync();
       __syncwarp();
       if (lane == 0) arrive_at(in_first(&s->acc_empty[buf]));
@@ -602,7 +622,7 @@ done:
   cluster_barrier();
   if (warp == 2) {
     fence_after_sync();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kTile) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
   }
 }
 
@@ -827,7 +847,7 @@ OrthLayout layout(const ngdn2_orth_args* a) {
   L.n = a->rows < a->cols ? a->cols : a->rows;
   L.ldx = (L.n + 7) / 8 * 8;
   L.lda = (L.m + 7) / 8 * 8;
-  L.parts = a->batch >= 8 ? 64 : kNormPartsMost;
+  L.parts = kNormParts;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
@@ -871,17 +891,38 @@ bool make_map(CUtensorMap* map, const __half* p, int64_t batch, int64_t rows, in
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int MODE>
-cudaError_t multiply(MulArgs p, const CUtensorMap& left, const CUtensorMap& right, const CUtensorMap& out, int sms,
-                     cudaStream_t st) {
-  p.nt = (p.m + kTile - 1) / kTile;
-  p.tiles_n = MODE == kApply ? (p.n + kTile - 1) / kTile : p.nt;
-  p.per = MODE == kApply ? p.nt * p.tiles_n : p.nt * (p.nt + 1) / 2;
-  const cudaError_t e = cudaFuncSetAttribute(orth_mul_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+// Tiles of one matrix.
+template <int MODE, int BN>
+int64_t tiles_of(const MulArgs& p) {
+  const int64_t rows = (p.m + kRows - 1) / kRows, cols = ((MODE == kApply ? p.n : p.m) + BN - 1) / BN;
+  return MODE == kApply ? rows * cols : rows * cols - rows * (rows - 1) / 2 * (kRows / BN);
+}
+
+template <int MODE, int BN>
+cudaError_t launch_mul(MulArgs p, const CUtensorMap& left, const CUtensorMap& right, const CUtensorMap& out,
+                       int pairs, cudaStream_t st) {
+  p.tiles_n = ((MODE == kApply ? p.n : p.m) + BN - 1) / BN;
+  p.per = tiles_of<MODE, BN>(p);
+  auto* kernel = orth_mul_kernel<MODE, BN>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  const int64_t total = p.batch * p.per, pairs = sms / 2;
-  return launch_next(orth_mul_kernel<MODE>, dim3(unsigned(2 * (total < pairs ? total : pairs))), dim3(kMulThreads),
-                     kSmem, st, true, p, left, right, out);
+  const int64_t total = p.batch * p.per;
+  return launch_next(kernel, dim3(unsigned(2 * (total < pairs ? total : pairs))), dim3(kMulThreads), kSmem, st, true,
+                     p, left, right, out);
+}
+
+// Wide or narrow tiles, by the rounds of tiles that the pairs of CTAs go through:
+// a round of narrow tiles takes 0.6 of one of wide ones (12 x 1024 x 2816, all
+// products narrow: 2114 us against 1729; 1024 x 2816: 419 against 508). An
+// element's sum has the same order either way.
+template <int MODE>
+cudaError_t multiply(const MulArgs& p, const CUtensorMap& left, const CUtensorMap& right, const CUtensorMap& out,
+                     int sms, cudaStream_t st) {
+  const int pairs = sms / 2;
+  const int64_t wide = (p.batch * tiles_of<MODE, 256>(p) + pairs - 1) / pairs;
+  const int64_t narrow = (p.batch * tiles_of<MODE, 128>(p) + pairs - 1) / pairs;
+  return 6 * narrow < 10 * wide ? launch_mul<MODE, 128>(p, left, right, out, pairs, st)
+                                : launch_mul<MODE, 256>(p, left, right, out, pairs, st);
 }
 
 // The scalar iteration s <- s (a + b s^2 + c s^4) from every start in [0, 1]
@@ -993,12 +1034,12 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
                     a->out_dtype, int(tall));
     return e == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
   }
-  // Operands: rows of X, A or B (128 rows a box), and X rows along the reduction
-  // (64); results (32 x 32).
-  CUtensorMap mx[2], mxr[2], mxo[2], mA, mB, mAo, mBo;
+  // Left operands (128 rows a box), right ones (64), results (32 x 32).
+  CUtensorMap mx[2], mxr[2], mxo[2], mA, mAr, mB, mAo, mBo;
   if (!make_map(&mx[0], x, a->batch, L.m, L.n, L.ldx, 128) || !make_map(&mx[1], y, a->batch, L.m, L.n, L.ldx, 128) ||
       !make_map(&mxr[0], x, a->batch, L.m, L.n, L.ldx, 64) || !make_map(&mxr[1], y, a->batch, L.m, L.n, L.ldx, 64) ||
       !make_map(&mA, A, a->batch, L.m, L.m, L.lda, 128) || !make_map(&mB, B, a->batch, L.m, L.m, L.lda, 128) ||
+      !make_map(&mAr, A, a->batch, L.m, L.m, L.lda, 64) ||
       !make_map(&mxo[0], x, a->batch, L.m, L.n, L.ldx, 32, 32) ||
       !make_map(&mxo[1], y, a->batch, L.m, L.n, L.ldx, 32, 32) ||
       !make_map(&mAo, A, a->batch, L.m, L.m, L.lda, 32, 32) || !make_map(&mBo, B, a->batch, L.m, L.m, L.lda, 32, 32))
@@ -1027,13 +1068,13 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
     p.lo_left = p.lo_right = lo;
     p.ld = L.lda;
     p.mirror = A;
-    e = multiply<kGram>(p, mx[in], mx[in], mAo, sms, st);
+    e = multiply<kGram>(p, mx[in], mxr[in], mAo, sms, st);
     if (e != cudaSuccess) break;
     p.depth = L.m;
     p.lo_left = p.lo_right = true;
     p.old = A;
     p.mirror = B;
-    e = multiply<kPoly>(p, mA, mA, mBo, sms, st);
+    e = multiply<kPoly>(p, mA, mAr, mBo, sms, st);
     if (e != cudaSuccess) break;
     p.old = nullptr;
     p.lo_right = lo;
