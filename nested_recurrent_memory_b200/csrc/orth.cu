@@ -11,7 +11,11 @@
 // hi hi + hi lo + lo hi, summed in fp32 in tensor memory: the accuracy of fp32
 // arithmetic (about 1e-6 .. 1e-5 on the same updates) at a third of the
 // tensor cores' rate. A 16-bit update fits its hi plane, so the first step
-// needs one product for A and two for X.
+// needs one product for A and two for X. The last step's roundings are not
+// stretched any more: where the result is bf16 (unit 2^-8) it uses the hi
+// planes alone (2^-11), which leaves the result's error within 1.13 times that
+// of rounding the exact one to bf16 (simulated on full-rank, decaying and
+// low-rank spectra; the last two steps would leave 1.8 times).
 //
 // Matrices of up to 128 x 256 take one CTA and one launch (orth_small_kernel).
 // Kernels for larger ones: the squared norm (partial sums in 64 bits), the conversion to
@@ -265,6 +269,7 @@ struct MulArgs {
   int64_t depth;         // of the reduction
   int64_t tiles_n, per;  // column tiles, tiles of a matrix
   bool lo_left, lo_right;    // whether the operands' lo planes are read
+  bool lo_out;               // whether the result (and, kPoly, A) has a lo plane
   float a, b, c;
   const float* sigma;    // [batch], or NULL for 1 / kScale
   const __half* old;     // kPoly: the planes of A
@@ -400,13 +405,13 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, int c0, int c1
                : "memory");
 }
 
-// The stage's two planes to the matrix, from row r0 and column c0 on.
-__device__ __forceinline__ void store_stage(const CUtensorMap* map, int c0, int r0, int z, uint32_t stage) {
+// The stage's planes to the matrix, from row r0 and column c0 on.
+__device__ __forceinline__ void store_stage(const CUtensorMap* map, int c0, int r0, int z, uint32_t stage, bool lo) {
   fence_proxy_async();
   __syncwarp();
   if ((threadIdx.x & 31) == 0) {
     store_box(map, c0, r0, z, stage);
-    store_box(map, c0, r0, z + 1, stage + kOutPlane);
+    if (lo) store_box(map, c0, r0, z + 1, stage + kOutPlane);
     bulk_commit();
   }
 }
@@ -450,7 +455,7 @@ __device__ __forceinline__ void emit32(const MulArgs& p, const CUtensorMap* out,
     *reinterpret_cast<uint4*>(mem + out_at(lane, i)) = *reinterpret_cast<const uint4*>(h + i);
     *reinterpret_cast<uint4*>(mem + kOutPlane + out_at(lane, i)) = *reinterpret_cast<const uint4*>(l + i);
   }
-  store_stage(out, int(c), int(r0), z, smem_u32(mem));
+  store_stage(out, int(c), int(r0), z, smem_u32(mem), p.lo_out);
   if (MODE != kApply && mirror && r < p.m) {
     // The same below the diagonal: lanes are neighbours there. (Through the
     // stage as well, each store would wait for the one before.)
@@ -459,7 +464,7 @@ __device__ __forceinline__ void emit32(const MulArgs& p, const CUtensorMap* out,
     for (int i = 0; i < 32; ++i)
       if (c + i < cols) {
         to[i * p.ld] = h[i];
-        to[(p.m + i) * p.ld] = l[i];
+        if (p.lo_out) to[(p.m + i) * p.ld] = l[i];
       }
   }
 }
@@ -514,7 +519,7 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
     for (int i = 0; i < 4; ++i) {
       const bool in = r < p.m && c + 8 * i < p.m;  // (a row has room for a multiple of 8)
       oh[i] = in ? __ldg(reinterpret_cast<const uint4*>(old) + i) : make_uint4(0, 0, 0, 0);
-      ol[i] = in ? __ldg(reinterpret_cast<const uint4*>(old + p.m * p.ld) + i) : make_uint4(0, 0, 0, 0);
+      ol[i] = in && p.lo_out ? __ldg(reinterpret_cast<const uint4*>(old + p.m * p.ld) + i) : make_uint4(0, 0, 0, 0);
     }
   };
 
@@ -721,7 +726,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   bool alive = true;
 
   // D[128 x cols] = L R, reduction over ``depth`` (multiples of 16).
-  auto product = [&](uint32_t L, int lp, uint32_t R, int rp, int depth, int cols, bool down) {
+  auto product = [&](uint32_t L, int lp, uint32_t R, int rp, int depth, int cols, bool down, bool full) {
     fence_proxy_async();
     fence_before_sync();
     __syncthreads();
@@ -735,8 +740,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
                       : desc_sw128(R + pl * rp + (kk >> 2) * kBlock + (kk & 3) * 32, 1024);
         };
         mma_f16(tmem, dl(0), dr(0), idesc, kk > 0);
-        mma_f16(tmem, dl(0), dr(1), idesc, 1);
-        mma_f16(tmem, dl(1), dr(0), idesc, 1);
+        if (full) {
+          mma_f16(tmem, dl(0), dr(1), idesc, 1);
+          mma_f16(tmem, dl(1), dr(0), idesc, 1);
+        }
       }
       mma_commit(&bar);
     }
@@ -756,8 +763,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   };
 
   for (int step = 0; step < q.steps && alive; ++step, sigma = 1.f / kScale) {
+    const bool full = !(step + 1 == q.steps && q.out.out_dtype == NGDN2_BF16);
     float v[32];
-    alive = product(ax, xp, ax, xp, nn, mn, false);
+    alive = product(ax, xp, ax, xp, nn, mn, false, full);
     if (!alive) break;
     for (int c = c1; c < m; c += 128) {
       tmem_ld32(taddr(tmem, quarter * 32, c), v);
@@ -766,7 +774,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
 #pragma unroll
       for (int i = 0; i < 32; i += 8) put8(ma, ap, c + i, v + i);
     }
-    alive = product(aa, ap, aa, ap, mn, mn, false);
+    alive = product(aa, ap, aa, ap, mn, mn, false, full);
     if (!alive) break;
     for (int c = c1; c < m; c += 128) {
       tmem_ld32(taddr(tmem, quarter * 32, c), v);
@@ -784,7 +792,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
         put8(ma, ap, c + i, v + i);
       }
     }
-    alive = product(aa, ap, ax, xp, mn, nn, true);
+    alive = product(aa, ap, ax, xp, mn, nn, true, full);
     if (!alive) break;
     for (int c = c1; c < n; c += 128) {
       tmem_ld32(taddr(tmem, quarter * 32, c), v);
@@ -1060,25 +1068,28 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
   p.status = a->status;
   for (int k = 0; k < a->steps && e == cudaSuccess; ++k) {
     const int in = k & 1;
-    const bool lo = k > 0 || a->dtype == NGDN2_F32;  // whether X has a lo plane
+    const bool last = k + 1 == a->steps, full = !(last && a->out_dtype == NGDN2_BF16);
+    const bool lo = full && (k > 0 || a->dtype == NGDN2_F32);  // whether X's lo plane counts
     p.sigma = k == 0 ? pr.sigma : nullptr;
     p.old = nullptr;
     p.final_out = nullptr;
     p.depth = L.n;
     p.lo_left = p.lo_right = lo;
+    p.lo_out = full;
     p.ld = L.lda;
     p.mirror = A;
     e = multiply<kGram>(p, mx[in], mxr[in], mAo, sms, st);
     if (e != cudaSuccess) break;
     p.depth = L.m;
-    p.lo_left = p.lo_right = true;
+    p.lo_left = p.lo_right = full;
     p.old = A;
     p.mirror = B;
     e = multiply<kPoly>(p, mA, mAr, mBo, sms, st);
     if (e != cudaSuccess) break;
     p.old = nullptr;
     p.lo_right = lo;
-    p.final_out = k + 1 == a->steps ? a->out : nullptr;
+    p.lo_out = true;
+    p.final_out = last ? a->out : nullptr;
     e = multiply<kApply>(p, mB, mxr[in], mxo[1 - in], sms, st);
   }
   return e == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
