@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _code, _DeviceStatus, _on_device, _raise_for, _require_cuda, _stream
+from .ops import _code, _launch, _raise_for, _require_same_device, _status_ptr
 
 __all__ = ["embed_tokens", "embed_tokens_fwd", "embed_tokens_bwd"]
 
@@ -46,15 +46,14 @@ def embed_tokens_fwd(ids, weight, scale=1.0):
     """
     if weight.dim() != 2:
         raise ValueError(f"weight must be [V, D], got {tuple(weight.shape)}")
-    _require_cuda(ids, weight)
+    dev = _require_same_device(weight, ids)
     ids = _ids(ids)
     if weight.stride(1) != 1:
         weight = weight.contiguous()
     V, D = weight.shape
-    out = torch.empty(*ids.shape, D, dtype=weight.dtype, device=weight.device)
+    out = weight.new_empty((*ids.shape, D))
     if out.numel() == 0:
         return out
-    status = _DeviceStatus.get(weight.device)
     a = _lib.EmbedArgs()
     a.abi_version = _lib.ABI_VERSION
     a.dtype = _code(weight)
@@ -62,11 +61,8 @@ def embed_tokens_fwd(ids, weight, scale=1.0):
     a.scale = scale
     a.N, a.V, a.D = ids.numel(), V, D
     a.ids, a.weight, a.weight_stride = ids.data_ptr(), weight.data_ptr(), weight.stride(0)
-    a.out, a.status = out.data_ptr(), status.word_ptr()
-    with _on_device(weight.device):
-        rc = _lib.load().ngdn2_embed(ctypes.byref(a), _stream(weight.device))
-    _raise_for(rc, "ngdn2_embed")
-    status.after_poisoning_launch()
+    a.out, a.status = out.data_ptr(), _status_ptr(dev)
+    _launch(_lib.load().ngdn2_embed, a, dev, "ngdn2_embed")
     return out
 
 
@@ -81,7 +77,7 @@ def embed_tokens_bwd(ids, d_out, num_embeddings, scale=1.0, padding_idx=None, dt
     if d_out.shape[:-1] != ids.shape:
         raise ValueError(f"d_out must be [*ids.shape, D], got {tuple(d_out.shape)} for ids "
                          f"{tuple(ids.shape)}")
-    _require_cuda(ids, d_out)
+    dev = _require_same_device(d_out, ids)
     V, D = int(num_embeddings), d_out.shape[-1]
     pad = _padding(padding_idx, V)
     ids = _ids(ids)
@@ -89,11 +85,9 @@ def embed_tokens_bwd(ids, d_out, num_embeddings, scale=1.0, padding_idx=None, dt
         d_out = d_out.reshape(ids.numel(), D)
     if d_out.stride(1) != 1:
         d_out = d_out.contiguous()
-    dev = d_out.device
-    dweight = torch.empty(V, D, dtype=dtype or d_out.dtype, device=dev)
+    dweight = d_out.new_empty((V, D), dtype=dtype)
     if dweight.numel() == 0:
         return dweight
-    status = _DeviceStatus.get(dev)
     a = _lib.EmbedBwdArgs()
     a.abi_version = _lib.ABI_VERSION
     a.dtype, a.out_dtype = _code(d_out), _code(dweight)
@@ -101,7 +95,7 @@ def embed_tokens_bwd(ids, d_out, num_embeddings, scale=1.0, padding_idx=None, dt
     a.scale = scale
     a.N, a.V, a.D, a.padding_idx = ids.numel(), V, D, pad
     a.ids, a.d_out, a.d_stride = ids.data_ptr(), d_out.data_ptr(), d_out.stride(0)
-    a.dweight, a.status = dweight.data_ptr(), status.word_ptr()
+    a.dweight, a.status = dweight.data_ptr(), _status_ptr(dev)
     lib = _lib.load()
     need = ctypes.c_size_t(0)
     _raise_for(lib.ngdn2_embed_bwd_workspace_size(ctypes.byref(a), ctypes.byref(need)),
@@ -110,10 +104,7 @@ def embed_tokens_bwd(ids, d_out, num_embeddings, scale=1.0, padding_idx=None, dt
         workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
     if need.value:
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    with _on_device(dev):
-        rc = lib.ngdn2_embed_bwd(ctypes.byref(a), _stream(dev))
-    _raise_for(rc, "ngdn2_embed_bwd")
-    status.after_poisoning_launch()
+    _launch(lib.ngdn2_embed_bwd, a, dev, "ngdn2_embed_bwd")
     return dweight
 
 

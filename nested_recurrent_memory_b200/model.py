@@ -12,7 +12,13 @@ sigmoid gate) and ``GatedMLP`` (SwiGLU, intermediate size
 256 * ceil(hidden * ratio * 2/3 / 256)). Dense layers run as torch (cuBLAS)
 GEMMs; the token mixer's op is ``chunk_nested_gdn2`` from this package
 (hand-written sm_100a kernels) unless another op with the same signature is
-passed in. Forward only, no decode cache.
+passed in. No decode cache for the nested layers.
+
+Beyond the reference, the embedding may scale its rows (``embed_tokens``), and
+the layers named in ``recurrent_layers`` mix tokens with the channel-wise
+gated recurrence (``gated_scan``) instead of the nested op. A model of such
+layers only decodes token by token (``NestedGDN2ForCausalLM.step``). Everything
+is differentiable, so the same module trains (see ``optim.Muon``).
 """
 
 from __future__ import annotations
@@ -24,9 +30,12 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .embedding import embed_tokens
 from .ops import chunk_nested_gdn2
+from .recurrence import gated_scan, step_gated_scan
 
-__all__ = ["ModelConfig", "NestedGDN2Attention", "NestedGDN2Block", "NestedGDN2ForCausalLM"]
+__all__ = ["ModelConfig", "NestedGDN2Attention", "GatedRecurrence", "ScaledEmbedding",
+           "NestedGDN2Block", "NestedGDN2ForCausalLM"]
 
 
 @dataclass
@@ -50,6 +59,8 @@ class ModelConfig:
     promotion: str = "learned"
     read_mix: str = "softmax"
     max_horizon: int | None = None
+    embed_scale: float = 1.0
+    recurrent_layers: tuple = ()  # indices of the layers that mix by GatedRecurrence
 
 
 class ShortConvolution(nn.Module):
@@ -174,20 +185,80 @@ class NestedGDN2Attention(nn.Module):
         return self.o_proj(o.reshape(B, T, H * V)), state
 
 
+class GatedRecurrence(nn.Module):
+    """A token mixer of one gated linear recurrence a channel,
+    h_t = e^{g_t} h_{t-1} + sqrt(1 - e^{2 g_t}) v_t, with the nested layer's
+    decay parameterisation and gated output norm. Its state is [B, value_dim]
+    float32."""
+
+    def __init__(self, cfg: ModelConfig):
+        super().__init__()
+        d, self.H, self.V = cfg.hidden_size, cfg.num_heads, int(cfg.head_dim * cfg.expand_v)
+        width = self.H * self.V
+        self.v_proj = nn.Linear(d, width, bias=False)
+        self.f_proj = nn.Sequential(nn.Linear(d, self.V, bias=False), nn.Linear(self.V, width, bias=False))
+        self.A_log = nn.Parameter(torch.log(torch.empty(width, dtype=torch.float32).uniform_(1, 16)))
+        dt = torch.exp(torch.rand(width) * (math.log(0.1) - math.log(0.001)) + math.log(0.001))
+        self.dt_bias = nn.Parameter(dt + torch.log(-torch.expm1(-dt)))
+        self.g_proj = nn.Sequential(nn.Linear(d, self.V, bias=False), nn.Linear(self.V, width, bias=True))
+        self.o_norm = GatedRMSNorm(self.V, cfg.norm_eps)
+        self.o_proj = nn.Linear(width, d, bias=False)
+
+    def _inputs(self, x):
+        g = -self.A_log.float().exp() * F.softplus(self.f_proj(x).float() + self.dt_bias)
+        v = self.v_proj(x)
+        return (v * torch.sqrt(-torch.expm1(2.0 * g))).to(v.dtype), g
+
+    def _output(self, h, x):
+        heads = (*h.shape[:-1], self.H, self.V)
+        return self.o_proj(self.o_norm(h.reshape(heads), self.g_proj(x).reshape(heads)).flatten(-2))
+
+    def forward(self, x, initial_state=None):
+        """x [B, T, d] -> (output [B, T, d], final state [B, value_dim])."""
+        v, g = self._inputs(x)
+        h, state = gated_scan(v, g, initial_state, output_final_state=True)
+        return self._output(h, x), state
+
+    def step(self, x, state):
+        """One token: x [B, d], state [B, value_dim] (updated in place) -> [B, d]."""
+        v, g = self._inputs(x)
+        h, _ = step_gated_scan(v, g, state, out_state=state)
+        return self._output(h, x)
+
+
+class ScaledEmbedding(nn.Embedding):
+    """Token embedding times a constant: ``embed_tokens`` on a GPU, torch's
+    lookup elsewhere (for models whose op runs there)."""
+
+    def __init__(self, num_embeddings: int, dim: int, scale: float = 1.0):
+        super().__init__(num_embeddings, dim)
+        self.scale = scale
+
+    def forward(self, input_ids):
+        if self.weight.is_cuda:
+            return embed_tokens(input_ids, self.weight, self.scale, self.padding_idx)
+        y = super().forward(input_ids)
+        return y if self.scale == 1.0 else y * self.scale
+
+
 class NestedGDN2Block(nn.Module):
     """Pre-norm token mixing and channel mixing with residuals
     (modeling_nested_gdn2.py:43-67)."""
 
-    def __init__(self, cfg: ModelConfig, op=None):
+    def __init__(self, cfg: ModelConfig, op=None, recurrent=False):
         super().__init__()
         self.attn_norm = RMSNorm(cfg.hidden_size, cfg.norm_eps)
-        self.attn = NestedGDN2Attention(cfg, op)
+        self.attn = GatedRecurrence(cfg) if recurrent else NestedGDN2Attention(cfg, op)
         self.mlp_norm = RMSNorm(cfg.hidden_size, cfg.norm_eps)
         self.mlp = GatedMLP(cfg.hidden_size, cfg.hidden_ratio, cfg.intermediate_size)
 
     def forward(self, h):
         a, _ = self.attn(self.attn_norm(h))
         h = h + a
+        return h + self.mlp(self.mlp_norm(h))
+
+    def step(self, h, state):
+        h = h + self.attn.step(self.attn_norm(h), state)
         return h + self.mlp(self.mlp_norm(h))
 
 
@@ -200,8 +271,9 @@ class NestedGDN2ForCausalLM(nn.Module):
     def __init__(self, cfg: ModelConfig, op=None):
         super().__init__()
         self.cfg = cfg
-        self.embeddings = nn.Embedding(cfg.vocab_size, cfg.hidden_size)
-        self.layers = nn.ModuleList(NestedGDN2Block(cfg, op) for _ in range(cfg.num_hidden_layers))
+        self.embeddings = ScaledEmbedding(cfg.vocab_size, cfg.hidden_size, cfg.embed_scale)
+        self.layers = nn.ModuleList(NestedGDN2Block(cfg, op, i in cfg.recurrent_layers)
+                                    for i in range(cfg.num_hidden_layers))
         self.norm = RMSNorm(cfg.hidden_size, cfg.norm_eps)
         self.lm_head = nn.Linear(cfg.hidden_size, cfg.vocab_size, bias=False)
         for m in self.modules():
@@ -215,3 +287,29 @@ class NestedGDN2ForCausalLM(nn.Module):
         for layer in self.layers:
             h = layer(h)
         return self.lm_head(self.norm(h))
+
+    def prefill(self, input_ids):
+        """[B, T] ids -> (logits [B, T, V], the layers' states for ``step``);
+        for models whose every layer is a GatedRecurrence."""
+        self._require_recurrent()
+        h, states = self.embeddings(input_ids), []
+        for layer in self.layers:
+            a, state = layer.attn(layer.attn_norm(h))
+            states.append(state)
+            h = h + a
+            h = h + layer.mlp(layer.mlp_norm(h))
+        return self.lm_head(self.norm(h)), states
+
+    def step(self, input_ids, states):
+        """One decode token for every row: [B] ids -> logits [B, V]; the states
+        (from ``prefill``) are updated in place."""
+        self._require_recurrent()
+        h = self.embeddings(input_ids)
+        for layer, state in zip(self.layers, states, strict=True):
+            h = layer.step(h, state)
+        return self.lm_head(self.norm(h))
+
+    def _require_recurrent(self):
+        if not all(isinstance(layer.attn, GatedRecurrence) for layer in self.layers):
+            raise ValueError("token-by-token decoding needs every layer in recurrent_layers: the "
+                             "nested layers keep no decode cache here")

@@ -127,17 +127,6 @@ class _DeviceStatus:
             self.poll()
 
 
-    def word_ptr(self) -> int:
-        """Device address of the status word, for calls that poison their
-        outputs with NaN when they set it and so queue no copy of it: it
-        surfaces at ``check_status`` or the next forward's copy."""
-        return self.word.data_ptr()
-
-    def after_poisoning_launch(self):
-        if _SYNC_CHECK and not torch.cuda.is_current_stream_capturing():
-            self.check(sync=True)
-
-
 _SYNC_CHECK = __import__("os").environ.get("NGDN2_SYNC_CHECK", "0") not in ("", "0")
 
 
@@ -180,29 +169,44 @@ def _require_cuda(*ts):
                 f"got a tensor on {t.device}")
 
 
-class _SameDevice:
-    """No change of device (the tensors' device is already current)."""
-
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
+# The raw handle of the current stream of a device index (an order of magnitude
+# cheaper than building a torch.cuda.Stream object for each launch).
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-_SAME_DEVICE = _SameDevice()
+def _launch(fn, args, dev, what):
+    """Call the C entry point ``fn`` with ``args`` on the current stream of
+    ``dev`` (launches go to the current device, so it is changed when it is
+    another one) and raise for its return code."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(ctypes.byref(args), _raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(ctypes.byref(args), _raw_stream(dev.index))
+    if rc:
+        _raise_for(rc, what)
+    if _SYNC_CHECK and not torch.cuda.is_current_stream_capturing():
+        _DeviceStatus.get(dev).check(sync=True)
 
 
-def _on_device(dev):
-    """The context in which a launch on ``dev`` runs: launches go to the
-    current device, so it is changed when it is another one."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return _SAME_DEVICE
-    return torch.cuda.device(dev)
+def _status_ptr(dev):
+    """Device address of ``dev``'s status word, for calls that poison their
+    outputs with NaN when they set it and so queue no copy of it: it surfaces
+    at ``check_status`` or with the next forward's copy."""
+    st = _DeviceStatus._by_device.get(("cuda", dev.index))
+    return (st or _DeviceStatus.get(dev)).word.data_ptr()
 
 
-def _stream(dev):
-    return ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+def _require_same_device(t, *others):
+    """``t`` and the others (None passes) must be on one CUDA device."""
+    dev = t.device
+    if dev.type != "cuda":
+        _require_cuda(t)
+    for o in others:
+        if o is not None and o.device != dev:
+            _require_cuda(o)
+            raise RuntimeError(f"expected all tensors on {dev}, got one on {o.device}")
+    return dev
 
 
 def _fill_tok(args, name, t, rank):

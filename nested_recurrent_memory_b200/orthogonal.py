@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _code, _DeviceStatus, _on_device, _raise_for, _require_cuda, _stream
+from .ops import _code, _launch, _raise_for, _require_same_device, _status_ptr
 
 __all__ = ["orthogonalize"]
 
@@ -33,25 +33,21 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
     """
     if update.dim() < 2:
         raise ValueError(f"update must be [..., rows, cols], got {tuple(update.shape)}")
-    _require_cuda(update)
+    dev = _require_same_device(update)
     rows, cols = update.shape[-2:]
-    dev = update.device
-    out = torch.empty(update.shape, dtype=dtype or update.dtype, device=dev)
+    out = update.new_empty(update.shape, dtype=dtype)
     if out.numel() == 0:
         return out
     flat = update if update.dim() == 3 else update.reshape(-1, rows, cols)
-    status = _DeviceStatus.get(dev)
     a = _lib.OrthArgs()
     a.abi_version = _lib.ABI_VERSION
     a.dtype, a.out_dtype = _code(flat), _code(out)
     a.steps = int(steps)
-    for i, c in enumerate(coefficients):
-        a.coef[i] = c
+    a.coef[0], a.coef[1], a.coef[2] = coefficients
     a.eps = eps
     a.batch, a.rows, a.cols = flat.shape[0], rows, cols
-    a.update, a.out, a.status = flat.data_ptr(), out.data_ptr(), status.word_ptr()
-    for i, st in enumerate(flat.stride()):
-        a.update_stride[i] = st
+    a.update, a.out, a.status = flat.data_ptr(), out.data_ptr(), _status_ptr(dev)
+    a.update_stride = flat.stride()
     lib = _lib.load()
     need = ctypes.c_size_t(0)
     rc = lib.ngdn2_orth_workspace_size(ctypes.byref(a), ctypes.byref(need))
@@ -63,8 +59,5 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
         workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
     if need.value:
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
-    with _on_device(dev):
-        rc = lib.ngdn2_orth(ctypes.byref(a), _stream(dev))
-    _raise_for(rc, "ngdn2_orth")
-    status.after_poisoning_launch()
+    _launch(lib.ngdn2_orth, a, dev, "ngdn2_orth")
     return out

@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _code, _DeviceStatus, _fill_tok, _on_device, _raise_for, _require_cuda, _stream
+from .ops import _code, _launch, _raise_for, _require_same_device, _status_ptr
 
 __all__ = ["gated_scan", "gated_scan_fwd", "gated_scan_bwd", "step_gated_scan"]
 
@@ -23,9 +23,8 @@ __all__ = ["gated_scan", "gated_scan_fwd", "gated_scan_bwd", "step_gated_scan"]
 def _check_state(state, B, D, name):
     if state is None:
         return None
-    if tuple(state.shape) != (B, D):
+    if state.shape != (B, D):
         raise ValueError(f"{name} must be [{B}, {D}], got {tuple(state.shape)}")
-    _require_cuda(state)
     if state.dtype == torch.float32 and state.is_contiguous():
         return state
     return state.to(torch.float32).contiguous()
@@ -36,17 +35,17 @@ def _scan_args(x, g, init):
     a = _lib.ScanArgs()
     a.abi_version = _lib.ABI_VERSION
     a.B, a.T, a.D = B, T, D
-    _fill_tok(a, "x", x, 3)
-    _fill_tok(a, "g", g, 3)
+    a.x, a.x_dtype, a.x_stride = x.data_ptr(), _code(x), x.stride()
+    a.g, a.g_dtype, a.g_stride = g.data_ptr(), _code(g), g.stride()
     a.initial_state = init.data_ptr() if init is not None else None
     return a
 
 
-def _check_inputs(x, g):
+def _check_inputs(x, g, *others):
     if x.dim() != 3 or x.shape != g.shape:
         raise ValueError(f"x and g must both be [B, T, D], got {tuple(x.shape)} and "
                          f"{tuple(g.shape)}")
-    _require_cuda(x, g)
+    return _require_same_device(x, g, *others)
 
 
 def _workspace(a, workspace, dev):
@@ -66,15 +65,14 @@ def gated_scan_fwd(x, g, initial_state=None, output_final_state=False, return_au
     [B, D] float32 (None unless ``output_final_state``); with ``return_aux``
     also the dict that ``gated_scan_bwd`` takes (the states entering every
     128 steps)."""
-    _check_inputs(x, g)
+    dev = _check_inputs(x, g, initial_state)
     B, T, D = x.shape
-    dev = x.device
     init = _check_state(initial_state, B, D, "initial_state")
-    h = torch.empty(B, T, D, dtype=x.dtype, device=dev)
-    final = torch.empty(B, D, dtype=torch.float32, device=dev) if output_final_state else None
+    h = x.new_empty((B, T, D))
+    final = x.new_empty((B, D), dtype=torch.float32) if output_final_state else None
     carries = None
     if return_aux:
-        carries = torch.empty(B, -(-T // _lib.SCAN_CHUNK), D, dtype=torch.float32, device=dev)
+        carries = x.new_empty((B, -(-T // _lib.SCAN_CHUNK), D), dtype=torch.float32)
     if h.numel() == 0:
         if final is not None:
             final.zero_() if init is None else final.copy_(init)
@@ -86,12 +84,8 @@ def gated_scan_fwd(x, g, initial_state=None, output_final_state=False, return_au
         ws = _workspace(a, workspace, dev)
         if ws is not None:
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-        status = _DeviceStatus.get(dev)
-        a.status = status.word_ptr()
-        with _on_device(dev):
-            rc = _lib.load().ngdn2_scan(ctypes.byref(a), _stream(dev))
-        _raise_for(rc, "ngdn2_scan")
-        status.after_poisoning_launch()
+        a.status = _status_ptr(dev)
+        _launch(_lib.load().ngdn2_scan, a, dev, "ngdn2_scan")
     return (h, final, dict(carries=carries)) if return_aux else (h, final)
 
 
@@ -100,17 +94,14 @@ def gated_scan_bwd(x, g, dh, d_final=None, initial_state=None, aux=None, workspa
     ``(dx, dg, d_initial)`` in the dtypes of x, g and initial_state
     (``d_initial`` is None without an initial state). ``aux`` is the
     forward's; without it the forward runs again."""
-    _check_inputs(x, g)
+    dev = _check_inputs(x, g, dh, d_final, initial_state)
     B, T, D = x.shape
-    dev = x.device
     if dh.shape != x.shape:
         raise ValueError(f"dh must be {tuple(x.shape)}, got {tuple(dh.shape)}")
-    _require_cuda(dh)
     init = _check_state(initial_state, B, D, "initial_state")
     dfin = _check_state(d_final, B, D, "d_final")
-    dx = torch.empty(B, T, D, dtype=x.dtype, device=dev)
-    dg = torch.empty(B, T, D, dtype=g.dtype, device=dev)
-    dinit = torch.empty(B, D, dtype=torch.float32, device=dev) if init is not None else None
+    dx, dg = x.new_empty((B, T, D)), g.new_empty((B, T, D))
+    dinit = x.new_empty((B, D), dtype=torch.float32) if init is not None else None
     if dx.numel() == 0:
         if dinit is not None:
             dinit.zero_() if dfin is None else dinit.copy_(dfin)
@@ -131,16 +122,12 @@ def gated_scan_bwd(x, g, dh, d_final=None, initial_state=None, aux=None, workspa
         if ws is not None:
             a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
         a.fwd = fwd
-        _fill_tok(a, "d_h", dh, 3)
+        a.d_h, a.d_h_dtype, a.d_h_stride = dh.data_ptr(), _code(dh), dh.stride()
         a.d_final = dfin.data_ptr() if dfin is not None else None
         a.dx, a.dg = dx.data_ptr(), dg.data_ptr()
         a.d_initial = dinit.data_ptr() if dinit is not None else None
-        status = _DeviceStatus.get(dev)
-        a.status = status.word_ptr()
-        with _on_device(dev):
-            rc = _lib.load().ngdn2_scan_bwd(ctypes.byref(a), _stream(dev))
-        _raise_for(rc, "ngdn2_scan_bwd")
-        status.after_poisoning_launch()
+        a.status = _status_ptr(dev)
+        _launch(_lib.load().ngdn2_scan_bwd, a, dev, "ngdn2_scan_bwd")
     if dinit is not None and initial_state.dtype != torch.float32:
         dinit = dinit.to(initial_state.dtype)
     return dx, dg, dinit
@@ -178,23 +165,21 @@ def step_gated_scan(x, g, state, *, out_state=None):
     ``state`` itself to update in place."""
     if x.dim() != 2 or x.shape != g.shape:
         raise ValueError(f"x and g must both be [B, D], got {tuple(x.shape)} and {tuple(g.shape)}")
-    _require_cuda(x, g, state)
+    dev = _require_same_device(x, g, state, out_state)
     B, D = x.shape
     state = _check_state(state, B, D, "state")
     new = torch.empty_like(state) if out_state is None else out_state
-    if out_state is not None and (tuple(new.shape) != (B, D) or new.dtype != torch.float32
+    if out_state is not None and (new.shape != (B, D) or new.dtype != torch.float32
                                   or not new.is_contiguous()):
         raise ValueError(f"out_state must be a contiguous float32 [{B}, {D}]")
-    h = torch.empty(B, D, dtype=x.dtype, device=x.device)
+    h = x.new_empty((B, D))
     if h.numel() == 0:
         return h, new
     a = _lib.ScanStepArgs()
     a.abi_version = _lib.ABI_VERSION
     a.B, a.D = B, D
-    _fill_tok(a, "x", x, 2)
-    _fill_tok(a, "g", g, 2)
+    a.x, a.x_dtype, a.x_stride = x.data_ptr(), _code(x), x.stride()
+    a.g, a.g_dtype, a.g_stride = g.data_ptr(), _code(g), g.stride()
     a.state_in, a.state_out, a.h = state.data_ptr(), new.data_ptr(), h.data_ptr()
-    with _on_device(x.device):
-        rc = _lib.load().ngdn2_scan_step(ctypes.byref(a), _stream(x.device))
-    _raise_for(rc, "ngdn2_scan_step")
+    _launch(_lib.load().ngdn2_scan_step, a, dev, "ngdn2_scan_step")
     return h, new
