@@ -18,17 +18,22 @@
 // low-rank spectra; the last two steps would leave 1.8 times).
 //
 // Matrices of up to 128 x 256 take one CTA and one launch (orth_small_kernel).
-// Kernels for larger ones: the squared norm (partial sums in 64 bits), the conversion to
-// planes, then per step three products: A = X X^T, B = a I + b A + c A A
-// (both symmetric: tiles on and above the diagonal only, written twice) and
-// X' = B X, which reads X as it lies, rows along the reduction.
+// Larger ones: the squared norm (partial sums in 64 bits), the conversion to
+// planes, and the products of all steps: A = X X^T, B = a I + b A
+// + c A A (both symmetric: the tiles on and above the diagonal, written twice)
+// and X' = B X, which reads X as it lies, rows along the reduction. The
+// products are cut into tiles, handed out by a counter. For large batches one
+// launch does them all, in an order in which every tile's operands come from
+// tiles before it: a tile waits until those of its matrix are done, so one
+// matrix's next product starts while others' last one still runs. Every wait
+// is bounded.
 //
-// Products: a pair of CTAs computes tiles of 256 rows by 256 or 128 columns
-// (tcgen05, cta_group::2; each CTA holds its 128 rows of the left operand and
-// half of the right one), fed by a thread that issues TMA loads of 64-deep
-// stages ahead, with two accumulators in tensor memory so that one tile's
-// results are written while the next is multiplied. The pair tile halves what
-// each multiprocessor must read: 64 KB a stage for 12 MMAs of 256 columns. The
+// A pair of CTAs computes tiles of 256 rows by 256 or 128 columns (tcgen05,
+// cta_group::2; each CTA holds its 128 rows of the left operand and half of
+// the right one), fed by a thread that issues TMA loads of 64-deep stages
+// ahead, with two accumulators in tensor memory so that one tile's results are
+// written while the next is multiplied. The pair tile halves what each
+// multiprocessor must read: 64 KB a stage for 12 MMAs of 256 columns. The
 // narrower tile reads more for each MMA, but few tiles finish sooner. Either
 // sums in the same order, so a matrix has the same bits in any batch.
 
@@ -65,6 +70,14 @@ __device__ __forceinline__ void split(float x, __half& hi, __half& lo) {
 // Norm and conversion
 // ---------------------------------------------------------------------------
 
+// What the CTAs of a launch tell each other, zero at its start.
+struct Sync {
+  uint32_t units;    // handed out so far
+  uint32_t stop;     // a wait gave up
+  uint64_t done[1];  // of each matrix: the writing warps' finished units
+};
+constexpr int kSyncWords = (sizeof(Sync) - 8) / 8;  // before ``done``
+
 constexpr int kPrepThreads = 256, kNormParts = 128;
 
 struct PrepArgs {
@@ -78,6 +91,7 @@ struct PrepArgs {
   __half* x;               // [batch][2][m][ld]; the lo plane only where lo is set
   int64_t ld;
   bool lo;
+  uint64_t* sync;          // the products' Sync, cleared here
 };
 
 // Sixteen bytes as fp32.
@@ -104,6 +118,8 @@ __global__ void __launch_bounds__(kPrepThreads) orth_norm_kernel(const __grid_co
   __shared__ double red[kPrepThreads / 32];
   const int64_t b = blockIdx.x / p.parts;
   const int part = int(blockIdx.x % p.parts), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (threadIdx.x == 0 && part == 0) p.sync[kSyncWords + b] = 0;
+  if (threadIdx.x < kSyncWords && blockIdx.x == 0) p.sync[threadIdx.x] = 0;
   double s = 0.0;
   if constexpr (FLAT) {
     constexpr int kPer = DT == NGDN2_F32 ? 4 : 8;
@@ -266,44 +282,94 @@ static_assert(Shape<128>::kStages * Shape<128>::kStage == 3 * 65536, "");
 
 struct MulArgs {
   int64_t batch, m, n;   // X is m x n
-  int64_t depth;         // of the reduction
-  int64_t tiles_n, per;  // column tiles, tiles of a matrix
-  bool lo_left, lo_right;    // whether the operands' lo planes are read
-  bool lo_out;               // whether the result (and, kPoly, A) has a lo plane
+  int steps;
   float a, b, c;
-  const float* sigma;    // [batch], or NULL for 1 / kScale
-  const __half* old;     // kPoly: the planes of A
-  __half* mirror;        // kGram, kPoly: the planes of the result, for direct stores
-  int64_t ld;            // of A and B
-  void* final_out;       // the result of the last kApply; others go to the planes of ``out``
+  const float* sigma;    // [batch]: the scale of the first step's X; then 1 / kScale
+  bool x_lo;             // whether the first step's X has a lo plane
+  __half *A, *B;         // their planes, rows ld apart
+  int64_t ld;
+  void* final_out;       // [batch][m][n], or transposed
   int out_dtype, transposed;
+  uint32_t first, end;   // the launch's units
+  bool wait;             // whether their operands may come from the same launch
+  Sync* sync;
   int32_t* status;
+};
+
+// X and X' change places every step.
+struct Maps {
+  CUtensorMap x_left[2], x_right[2], x_out[2], a_left, a_right, a_out, b_left, b_out;
 };
 
 struct Barriers {
   uint64_t full[kStagesMost], empty[kStagesMost], acc_full[2], acc_empty[2];
+  uint64_t unit_full[2], unit_empty[2];
+  uint32_t unit[2];
   uint32_t tmem;
   int dead;
 };
 
-// Tile number t: all of a matrix's, or those that reach the diagonal or lie above it.
-template <int MODE, int BN>
-__device__ __forceinline__ void tile_at(const MulArgs& p, int64_t t, int64_t* b, int64_t* tm, int64_t* tn) {
-  *b = t / p.per;
-  int64_t q = t % p.per;
-  if (MODE == kApply) {
-    *tm = q / p.tiles_n;
-    *tn = q % p.tiles_n;
+// The work of the whole iteration in units, each a tile of one product of one
+// matrix; their order is one in which every unit's operands come from units
+// before it: by steps, then products, then matrices.
+template <int BN>
+struct Plan {
+  uint32_t sym, app;  // tiles of A or B (those that reach the diagonal or lie above it), and of X'
+  uint32_t cols_s, cols_a, per_step, total;
+  __host__ __device__ explicit Plan(const MulArgs& p) {
+    const uint32_t rows = uint32_t((p.m + kRows - 1) / kRows);
+    cols_s = uint32_t((p.m + BN - 1) / BN);
+    cols_a = uint32_t((p.n + BN - 1) / BN);
+    sym = rows * cols_s - rows * (rows - 1) / 2 * (kRows / BN);
+    app = rows * cols_a;
+    per_step = uint32_t(p.batch) * (2 * sym + app);
+    total = per_step * uint32_t(p.steps);
+  }
+};
+
+struct Unit {
+  int step, mode;
+  int64_t b, tm, tn;
+  int blocks;           // of the reduction
+  bool lo_left, lo_right;
+  bool lo_out;          // whether the result (and, kPoly, A) has a lo plane
+  bool last;
+  uint64_t need;        // of the matrix's finished warps' units, before this one may start
+};
+
+template <int BN>
+__device__ __forceinline__ Unit unit_at(const MulArgs& p, const Plan<BN>& plan, uint32_t t) {
+  Unit u;
+  u.step = int(t / plan.per_step);
+  uint32_t r = t % plan.per_step;
+  const uint32_t s = uint32_t(p.batch) * plan.sym;
+  u.mode = r < s ? kGram : r < 2 * s ? kPoly : kApply;
+  r -= u.mode * s;
+  const uint32_t per = u.mode == kApply ? plan.app : plan.sym;
+  u.b = r / per;
+  uint32_t q = r % per;
+  if (u.mode == kApply) {
+    u.tm = q / plan.cols_a;
+    u.tn = q % plan.cols_a;
   } else {
-    int64_t r = 0, len = p.tiles_n;
+    uint32_t row = 0, len = plan.cols_s;
     while (q >= len) {
       q -= len;
       len -= kRows / BN;
-      ++r;
+      ++row;
     }
-    *tm = r;
-    *tn = r * (kRows / BN) + q;
+    u.tm = row;
+    u.tn = row * (kRows / BN) + q;
   }
+  u.last = u.step + 1 == p.steps;
+  const bool full = !(u.last && p.out_dtype == NGDN2_BF16);
+  const bool x_lo = full && (u.step > 0 || p.x_lo);
+  u.blocks = int(((u.mode == kGram ? p.n : p.m) + kDepth - 1) / kDepth);
+  u.lo_left = u.mode == kGram ? x_lo : full;
+  u.lo_right = u.mode == kPoly ? full : x_lo;
+  u.lo_out = u.mode == kApply || full;
+  u.need = (uint64_t(u.step) * (2 * plan.sym + plan.app) + u.mode * plan.sym) * (2 * kWriters);
+  return u;
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -353,15 +419,84 @@ __device__ __forceinline__ uint64_t desc_sw128_mn(uint32_t saddr, uint32_t block
   return (desc_sw128(saddr, 1024) & ~(uint64_t(0x3FFF) << 16)) | uint64_t(block >> 4) << 16;
 }
 
-// A bounded wait that gives up for the whole CTA.
-__device__ __forceinline__ bool wait_or_die(Barriers* s, uint64_t* bar, uint32_t phase, int32_t* status) {
-  for (uint32_t i = 0; i < (1u << 20); ++i) {
-    if (mbar_try_wait(bar, phase)) return true;
-    if (*reinterpret_cast<volatile int*>(&s->dead)) return false;
-  }
+constexpr uint32_t kNone = 0xffffffffu;
+
+// Waits are bounded. One that gives up does so for its CTA, and tells the others.
+constexpr uint32_t kPolls = 1u << 23;
+
+__device__ __forceinline__ void give_up(Barriers* s, const MulArgs& p) {
   s->dead = 1;
-  atomicOr(status, NGDN2_STATUS_WAIT_TIMEOUT);
+  atomicExch(&p.sync->stop, 1u);
+  atomicOr(p.status, NGDN2_STATUS_WAIT_TIMEOUT);
+}
+
+__device__ __forceinline__ bool gone(Barriers* s, const MulArgs& p, uint32_t poll) {
+  if (*reinterpret_cast<volatile int*>(&s->dead)) return true;
+  if ((poll & 1023) == 1023 && *reinterpret_cast<volatile uint32_t*>(&p.sync->stop)) {
+    s->dead = 1;
+    return true;
+  }
   return false;
+}
+
+__device__ __forceinline__ bool wait_or_die(Barriers* s, uint64_t* bar, uint32_t phase, const MulArgs& p) {
+  for (uint32_t i = 0; i < kPolls; ++i) {
+    if (mbar_try_wait(bar, phase)) return true;
+    if (gone(s, p, i)) return false;
+  }
+  give_up(s, p);
+  return false;
+}
+
+// For a barrier at which another CTA arrives with data.
+__device__ __forceinline__ bool wait_cluster_or_die(Barriers* s, uint64_t* bar, uint32_t phase, const MulArgs& p) {
+  for (uint32_t i = 0; i < kPolls; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P1;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P1, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, P1;\n\t}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(phase)
+        : "memory");
+    if (ok) return true;
+    if (gone(s, p, i)) return false;
+  }
+  give_up(s, p);
+  return false;
+}
+
+// Until the matrix's operands of a unit are written; what follows, by whichever
+// path it reads, comes after.
+__device__ __forceinline__ bool wait_operands(Barriers* s, const MulArgs& p, const Unit& u) {
+  const uint64_t* done = p.sync->done + u.b;
+  for (uint32_t i = 0; i < kPolls; ++i) {
+    uint64_t v;
+    asm volatile("ld.acquire.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(done) : "memory");
+    if (v >= u.need) {
+      asm volatile("fence.proxy.async;" ::: "memory");
+      return true;
+    }
+    if (gone(s, p, i)) return false;
+  }
+  give_up(s, p);
+  return false;
+}
+
+// The next unit's number: in turn, where no unit waits for another, else from
+// the ring that the pair's first CTA fills.
+__device__ __forceinline__ bool next_unit(Barriers* s, const MulArgs& p, uint32_t* slot, uint32_t* phase,
+                                          uint32_t* t) {
+  if (!p.wait) {
+    *t = *t == kNone ? p.first + blockIdx.x / 2 : *t + gridDim.x / 2;
+    return true;
+  }
+  if (!wait_cluster_or_die(s, &s->unit_full[*slot], *phase, p)) return false;
+  *t = *reinterpret_cast<volatile uint32_t*>(&s->unit[*slot]);
+  arrive_at(in_first(&s->unit_empty[*slot]));
+  *slot ^= 1;
+  if (*slot == 0) *phase ^= 1;
+  return true;
 }
 
 // The result's 32 neighbouring values of one row.
@@ -425,13 +560,13 @@ __device__ __forceinline__ void stage_free() {
 // A row's 32 neighbouring results, from the sums v: to the planes by way of the
 // warp's stage, or the final values. Whole warps; r0 is lane 0's row.
 template <int MODE>
-__device__ __forceinline__ void emit32(const MulArgs& p, const CUtensorMap* out, unsigned char* mem, int64_t b,
+__device__ __forceinline__ void emit32(const MulArgs& p, const Unit& u, const CUtensorMap* out, unsigned char* mem,
                                        int64_t r0, int64_t c, bool mirror, float sigma, const float* v,
                                        const uint4* oh, const uint4* ol) {
-  const int lane = threadIdx.x & 31, z = int(b * 2);
+  const int lane = threadIdx.x & 31, z = int(u.b * 2);
   const int64_t r = r0 + lane, cols = MODE == kApply ? p.n : p.m;
-  if (MODE == kApply && p.final_out) {
-    if (r < p.m) write_final(p, b, r, c, sigma / kScale, v);
+  if (MODE == kApply && u.last) {
+    if (r < p.m) write_final(p, u.b, r, c, sigma / kScale, v);
     return;
   }
   __half h[32], l[32];
@@ -455,24 +590,68 @@ __device__ __forceinline__ void emit32(const MulArgs& p, const CUtensorMap* out,
     *reinterpret_cast<uint4*>(mem + out_at(lane, i)) = *reinterpret_cast<const uint4*>(h + i);
     *reinterpret_cast<uint4*>(mem + kOutPlane + out_at(lane, i)) = *reinterpret_cast<const uint4*>(l + i);
   }
-  store_stage(out, int(c), int(r0), z, smem_u32(mem), p.lo_out);
+  store_stage(out, int(c), int(r0), z, smem_u32(mem), u.lo_out);
   if (MODE != kApply && mirror && r < p.m) {
     // The same below the diagonal: lanes are neighbours there. (Through the
     // stage as well, each store would wait for the one before.)
-    __half* to = p.mirror + (int64_t(z) * p.m + c) * p.ld + r;
+    __half* to = (MODE == kGram ? p.A : p.B) + (int64_t(z) * p.m + c) * p.ld + r;
 #pragma unroll
     for (int i = 0; i < 32; ++i)
       if (c + i < cols) {
         to[i * p.ld] = h[i];
-        if (p.lo_out) to[(p.m + i) * p.ld] = l[i];
+        if (u.lo_out) to[(p.m + i) * p.ld] = l[i];
       }
   }
 }
 
+// A writing warp's part of a unit: 32 rows by BN / 2 columns.
 template <int MODE, int BN>
+__device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const Unit& u, const CUtensorMap* out,
+                                           unsigned char* mem, uint32_t rank, uint32_t acc, uint64_t* acc_full,
+                                           uint32_t acc_phase) {
+  const int lane = threadIdx.x & 31, quarter = threadIdx.x >> 5 & 3, half = (threadIdx.x >> 7) - 1;
+  const int64_t r0 = u.tm * kRows + rank * 128 + quarter * 32, c1 = u.tn * BN + half * (BN / 2);
+  const int64_t cols = MODE == kApply ? p.n : p.m;
+  const bool mirror = u.tn / (kRows / BN) != u.tm;
+  const float sigma = u.step == 0 ? p.sigma[u.b] : 1.f / kScale;
+  // A's own values for 32 columns from c on, asked for ahead of the product.
+  uint4 oh[4], ol[4];
+  auto ask = [&](int64_t c) {
+    const __half* old = p.A + (u.b * 2 * p.m + r0 + lane) * p.ld + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = r0 + lane < p.m && c + 8 * i < p.m;  // (a row has room for a multiple of 8)
+      oh[i] = in ? __ldcg(reinterpret_cast<const uint4*>(old) + i) : make_uint4(0, 0, 0, 0);
+      ol[i] = in && u.lo_out ? __ldcg(reinterpret_cast<const uint4*>(old + p.m * p.ld) + i) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  bool ok = wait_or_die(s, acc_full, acc_phase, p);
+  // (The product is there, so A is. Only now: eight warps of every CTA that
+  // polled for it would hold up those that announce it.)
+  if (MODE == kPoly && p.wait && lane == 0) ok = ok && wait_operands(s, p, u);
+  if (!__all_sync(0xffffffffu, ok)) return false;
+  __syncwarp();
+  fence_after_sync();
+  if (MODE == kPoly) ask(c1);
+#pragma unroll 1
+  for (int i = 0; i < BN / 2; i += 32) {
+    const int64_t c = c1 + i;
+    if (c >= cols || r0 >= p.m) break;
+    float v[32];
+    tmem_ld32(taddr(acc, quarter * 32, half * (BN / 2) + i), v);
+    emit32<MODE>(p, u, out, mem, r0, c, mirror, sigma, v, oh, ol);
+    if (MODE == kPoly) ask(c + 32);
+  }
+  return true;
+}
+
+// Pairs of CTAs take units as they come free, one's results written while the
+// next is multiplied. In each CTA a thread issues the loads (the first CTA's
+// also fetches unit numbers for both) and eight warps write; in the first CTA a
+// thread issues the MMAs for both.
+template <int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMulThreads, 1)
-orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUtensorMap left,
-                const __grid_constant__ CUtensorMap right, const __grid_constant__ CUtensorMap out) {
+orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Maps maps) {
   constexpr int kStages = Shape<BN>::kStages, kStage = Shape<BN>::kStage, kRight = Shape<BN>::kRight;
   extern __shared__ unsigned char raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -480,8 +659,7 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
   Barriers* s = reinterpret_cast<Barriers*>(smem + kStages * kStage + kOutBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
-  const int64_t first = blockIdx.x / 2, step = gridDim.x / 2, total = p.batch * p.per;
-  const int blocks = int((p.depth + kDepth - 1) / kDepth);
+  const Plan<BN> plan(p);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s->full[i], 1);
@@ -490,6 +668,8 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s->acc_full[i], 1);
       mbar_init(&s->acc_empty[i], 2 * kWriters);
+      mbar_init(&s->unit_full[i], 1);
+      mbar_init(&s->unit_empty[i], 2 + 2 * kWriters);  // multiply, load (second CTA), write
     }
     s->dead = 0;
     fence_mbar_init();
@@ -507,43 +687,55 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
   const uint32_t tmem = s->tmem;
   after_previous();
   let_next_start();
-
-  // A writing warp's rows and columns, its stage, and A's own values for 32
-  // columns from c on, asked for ahead of the product.
-  const int quarter = warp & 3, half = (warp >> 2) - 1;
-  unsigned char* const mem = smem + kStages * kStage + (warp - 4) * 2 * kOutPlane;
-  uint4 oh[4], ol[4];
-  auto ask = [&](int64_t b, int64_t r, int64_t c) {
-    const __half* old = p.old + (b * 2 * p.m + r) * p.ld + c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool in = r < p.m && c + 8 * i < p.m;  // (a row has room for a multiple of 8)
-      oh[i] = in ? __ldg(reinterpret_cast<const uint4*>(old) + i) : make_uint4(0, 0, 0, 0);
-      ol[i] = in && p.lo_out ? __ldg(reinterpret_cast<const uint4*>(old + p.m * p.ld) + i) : make_uint4(0, 0, 0, 0);
-    }
-  };
+  uint32_t slot = 0, unit_phase = 0, t = kNone;
 
   if (warp == 0 && lane == 0) {
-    // Loads of this CTA's halves: 128 rows of the left operand, 128 rows (or
-    // columns, kApply) of the right one, hi and lo.
+    // Loads of this CTA's halves: 128 rows of the left operand, BN / 2 rows (or
+    // columns, kApply) of the right one, hi and lo. The first CTA's thread also
+    // fetches the next unit's number, with its last load of a unit: earlier,
+    // and units would wait here while other pairs go idle (2048 x 2048, two
+    // units ahead in one launch: 1031 us against 662).
     uint32_t st = 0, phase = 0;
-    const uint32_t bytes = 2 * (kLeft * (p.lo_left ? 2 : 1) + kRight * (p.lo_right ? 2 : 1));
-    for (int64_t t = first; t < total; t += step) {
-      int64_t b, tm, tn;
-      tile_at<MODE, BN>(p, t, &b, &tm, &tn);
-      const int row = int(tm * kRows + rank * 128), col = int(tn * BN + rank * (BN / 2)), z = int(b * 2);
-      for (int k = 0; k < blocks; ++k) {
-        if (!wait_or_die(s, &s->empty[st], phase ^ 1, p.status)) goto done;
+    auto fetch = [&](uint32_t* next) {
+      *next = atomicAdd(&p.sync->units, 1u);
+      if (!wait_cluster_or_die(s, &s->unit_empty[slot], unit_phase ^ 1, p)) return false;
+      for (uint32_t r = 0; r < 2; ++r) {
+        uint32_t at, bar;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(&s->unit[slot])), "r"(r));
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(smem_u32(&s->unit_full[slot])), "r"(r));
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(*next) : "memory");
+        arrive_at(bar);
+      }
+      slot ^= 1;
+      if (slot == 0) unit_phase ^= 1;
+      return true;
+    };
+    uint32_t next = 0;
+    const bool fetches = rank == 0 && p.wait;
+    if (fetches && !fetch(&next)) goto done;
+    for (;;) {
+      if (fetches) t = next;
+      else if (!next_unit(s, p, &slot, &unit_phase, &t)) goto done;
+      if (t >= p.end) break;
+      const Unit u = unit_at<BN>(p, plan, t);
+      const CUtensorMap* left = u.mode == kGram ? &maps.x_left[u.step & 1] : u.mode == kPoly ? &maps.a_left : &maps.b_left;
+      const CUtensorMap* right = u.mode == kPoly ? &maps.a_right : &maps.x_right[u.step & 1];
+      const int row = int(u.tm * kRows + rank * 128), col = int(u.tn * BN + rank * (BN / 2)), z = int(u.b * 2);
+      const uint32_t bytes = 2 * (kLeft * (u.lo_left ? 2 : 1) + kRight * (u.lo_right ? 2 : 1));
+      if (p.wait && !wait_operands(s, p, u)) goto done;
+      for (int k = 0; k < u.blocks; ++k) {
+        if (fetches && k + 1 == u.blocks && !fetch(&next)) goto done;
+        if (!wait_or_die(s, &s->empty[st], phase ^ 1, p)) goto done;
         const uint32_t at = base + st * kStage, bar = in_first(&s->full[st]);
         if (rank == 0) mbar_arrive_expect_tx(&s->full[st], bytes);
         for (int pl = 0; pl < 2; ++pl) {
-          if (pl == 0 || p.lo_left) load_box(at + pl * kLeft, &left, k * kDepth, row, z + pl, bar);
-          if (pl == 0 || p.lo_right)
+          if (pl == 0 || u.lo_left) load_box(at + pl * kLeft, left, k * kDepth, row, z + pl, bar);
+          if (pl == 0 || u.lo_right)
 #pragma unroll
             for (int i = 0; i < BN / 128; ++i) {
               const uint32_t to = at + 2 * kLeft + pl * kRight + i * kBox;
-              if (MODE == kApply) load_box(to, &right, col + 64 * i, k * kDepth, z + pl, bar);
-              else load_box(to, &right, k * kDepth, col + 64 * i, z + pl, bar);
+              if (u.mode == kApply) load_box(to, right, col + 64 * i, k * kDepth, z + pl, bar);
+              else load_box(to, right, k * kDepth, col + 64 * i, z + pl, bar);
             }
         }
         if (++st == kStages) {
@@ -554,32 +746,39 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
     }
     // Until the last MMAs have signalled here, this CTA's memory is needed.
     for (int i = 0; i < kStages; ++i) {
-      if (!wait_or_die(s, &s->empty[st], phase ^ 1, p.status)) goto done;
+      if (!wait_or_die(s, &s->empty[st], phase ^ 1, p)) goto done;
       if (++st == kStages) {
         st = 0;
         phase ^= 1;
       }
     }
   } else if (warp == 1 && lane == 0 && rank == 0) {
-    const uint32_t idesc = idesc_f16(kRows, BN, false, false, MODE == kApply);
     uint32_t st = 0, phase = 0, buf = 0, acc_phase = 0;
-    for (int64_t t = first; t < total; t += step) {
-      if (!wait_or_die(s, &s->acc_empty[buf], acc_phase ^ 1, p.status)) goto done;
+    for (;;) {
+      if (!next_unit(s, p, &slot, &unit_phase, &t)) goto done;
+      if (t >= p.end) break;
+      const Unit u = unit_at<BN>(p, plan, t);
+      const bool down = u.mode == kApply;
+      const uint32_t idesc = idesc_f16(kRows, BN, false, false, down);
+      const uint64_t left_desc = desc_sw128(base, 1024), right_step = (down ? 2048 : 32) >> 4;
+      const uint64_t right_desc = down ? desc_sw128_mn(base + 2 * kLeft, kBox) : desc_sw128(base + 2 * kLeft, 1024);
+      if (!wait_or_die(s, &s->acc_empty[buf], acc_phase ^ 1, p)) goto done;
       const uint32_t d = tmem + buf * BN;
-      for (int k = 0; k < blocks; ++k) {
-        if (!wait_or_die(s, &s->full[st], phase, p.status)) goto done;
+      for (int k = 0; k < u.blocks; ++k) {
+        if (!wait_or_die(s, &s->full[st], phase, p)) goto done;
         fence_after_sync();
-        const uint32_t at = base + st * kStage;
+        // Descriptors count 16 bytes: the lo planes and the next 16 of the
+        // reduction (32 bytes of a row, or 16 rows) are additions away. One thread
+        // issues everything, so what it computes for an MMA must not take
+        // longer than the MMA (64 cycles for 128 columns).
+        uint64_t dl = left_desc + ((st * kStage) >> 4), dr = right_desc + ((st * kStage) >> 4);
 #pragma unroll
         for (int kk = 0; kk < kDepth / 16; ++kk) {
-          auto L = [&](int pl) { return desc_sw128(at + pl * kLeft + kk * 32, 1024); };
-          auto R = [&](int pl) {
-            const uint32_t r = at + 2 * kLeft + pl * kRight;
-            return MODE == kApply ? desc_sw128_mn(r + kk * 2048, kBox) : desc_sw128(r + kk * 32, 1024);
-          };
-          mma_pair(d, L(0), R(0), idesc, (k | kk) != 0);
-          if (p.lo_right) mma_pair(d, L(0), R(1), idesc, 1);
-          if (p.lo_left) mma_pair(d, L(1), R(0), idesc, 1);
+          mma_pair(d, dl, dr, idesc, (k | kk) != 0);
+          if (u.lo_right) mma_pair(d, dl, dr + (kRight >> 4), idesc, 1);
+          if (u.lo_left) mma_pair(d, dl + (kLeft >> 4), dr, idesc, 1);
+          dl += 32 >> 4;
+          dr += right_step;
         }
         commit_pair(&s->empty[st]);
         if (++st == kStages) {
@@ -593,28 +792,28 @@ orth_mul_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ CUten
     }
   } else if (warp >= 4) {
     uint32_t buf = 0, acc_phase = 0;
-    for (int64_t t = first; t < total; t += step) {
-      int64_t b, tm, tn;
-      tile_at<MODE, BN>(p, t, &b, &tm, &tn);
-      const int64_t r0 = tm * kRows + rank * 128 + quarter * 32, cols = MODE == kApply ? p.n : p.m;
-      const bool mirror = tn / (kRows / BN) != tm;
-      const float sigma = p.sigma ? p.sigma[b] : 1.f / kScale;
-      if (MODE == kPoly) ask(b, r0 + lane, tn * BN + half * (BN / 2));
-      if (!wait_or_die(s, &s->acc_full[buf], acc_phase, p.status)) goto done;
-      __syncwarp();
-      fence_after_sync();
-#pragma unroll 1
-      for (int c0 = half * (BN / 2); c0 < (half + 1) * (BN / 2); c0 += 32) {
-        const int64_t c = tn * BN + c0;
-        if (c >= cols || r0 >= p.m) break;
-        float v[32];
-        tmem_ld32(taddr(tmem, quarter * 32, buf * BN + c0), v);
-        emit32<MODE>(p, &out, mem, b, r0, c, mirror, sigma, v, oh, ol);
-        if (MODE == kPoly) ask(b, r0 + lane, c + 32);
-      }
+    unsigned char* const mem = smem + kStages * kStage + (warp - 4) * 2 * kOutPlane;
+    for (;;) {
+      bool ok = true;
+      if (lane == 0) ok = next_unit(s, p, &slot, &unit_phase, &t);
+      if (!__all_sync(0xffffffffu, ok)) goto done;
+      t = __shfl_sync(0xffffffffu, t, 0);
+      if (t >= p.end) break;
+      const Unit u = unit_at<BN>(p, plan, t);
+      const uint32_t acc = tmem + buf * BN;
+      if (u.mode == kGram) ok = write_unit<kGram, BN>(s, p, u, &maps.a_out, mem, rank, acc, &s->acc_full[buf], acc_phase);
+      else if (u.mode == kPoly) ok = write_unit<kPoly, BN>(s, p, u, &maps.b_out, mem, rank, acc, &s->acc_full[buf], acc_phase);
+      else ok = write_unit<kApply, BN>(s, p, u, &maps.x_out[~u.step & 1], mem, rank, acc, &s->acc_full[buf], acc_phase);
+      if (!__all_sync(0xffffffffu, ok)) goto done;
       fence_before_sync();
       __syncwarp();
-      if (lane == 0) arrive_at(in_first(&s->acc_empty[buf]));
+      if (lane == 0) {
+        arrive_at(in_first(&s->acc_empty[buf]));
+        // All of the warp's results are in memory before the unit counts: its
+        // bulk stores are waited for, the others come before the release.
+        if (p.wait) bulk_wait0();
+        if (p.wait) asm volatile("red.release.gpu.global.add.u64 [%0], %1;" ::"l"(p.sync->done + u.b), "l"(uint64_t(1)) : "memory");
+      }
       buf ^= 1;
       if (buf == 0) acc_phase ^= 1;
     }
@@ -628,6 +827,10 @@ done:
   if (warp == 2) {
     fence_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
+  }
+  if (s->dead) {  // nothing that was not computed passes as a result
+    for (int64_t e = threadIdx.x; e < p.batch * p.m * p.n; e += kMulThreads)
+      store_elem(p.final_out, e, __int_as_float(0x7fc00000), p.out_dtype);
   }
 }
 
@@ -846,7 +1049,7 @@ cudaError_t by_type(int dt, F&& f) {
 struct OrthLayout {
   int64_t m, n, ldx, lda;
   int parts;
-  size_t x, y, A, B, part, sigma, total;
+  size_t x, y, A, B, part, sigma, sync, total;
 };
 
 OrthLayout layout(const ngdn2_orth_args* a) {
@@ -868,6 +1071,7 @@ OrthLayout layout(const ngdn2_orth_args* a) {
   L.B = take(size_t(a->batch) * 2 * L.m * L.lda * 2);
   L.part = take(size_t(a->batch) * L.parts * sizeof(double));
   L.sigma = take(size_t(a->batch) * sizeof(float));
+  L.sync = take((kSyncWords + size_t(a->batch)) * sizeof(uint64_t));
   L.total = at + 256;
   return L;
 }
@@ -899,38 +1103,53 @@ bool make_map(CUtensorMap* map, const __half* p, int64_t batch, int64_t rows, in
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Tiles of one matrix.
-template <int MODE, int BN>
-int64_t tiles_of(const MulArgs& p) {
-  const int64_t rows = (p.m + kRows - 1) / kRows, cols = ((MODE == kApply ? p.n : p.m) + BN - 1) / BN;
-  return MODE == kApply ? rows * cols : rows * cols - rows * (rows - 1) / 2 * (kRows / BN);
-}
-
-template <int MODE, int BN>
-cudaError_t launch_mul(MulArgs p, const CUtensorMap& left, const CUtensorMap& right, const CUtensorMap& out,
-                       int pairs, cudaStream_t st) {
-  p.tiles_n = ((MODE == kApply ? p.n : p.m) + BN - 1) / BN;
-  p.per = tiles_of<MODE, BN>(p);
-  auto* kernel = orth_mul_kernel<MODE, BN>;
+template <int BN>
+cudaError_t launch_units(MulArgs p, const Maps& maps, uint32_t first, uint32_t n, uint32_t pairs, cudaStream_t st) {
+  auto* kernel = orth_steps_kernel<BN>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
-  const int64_t total = p.batch * p.per;
-  return launch_next(kernel, dim3(unsigned(2 * (total < pairs ? total : pairs))), dim3(kMulThreads), kSmem, st, true,
-                     p, left, right, out);
+  p.first = first;
+  p.end = first + n;
+  return launch_next(kernel, dim3(2 * (n < pairs ? n : pairs)), dim3(kMulThreads), kSmem, st, true, p, maps);
 }
 
-// Wide or narrow tiles, by the rounds of tiles that the pairs of CTAs go through:
-// a round of narrow tiles takes 0.6 of one of wide ones (12 x 1024 x 2816, all
-// products narrow: 2114 us against 1729; 1024 x 2816: 419 against 508). An
-// element's sum has the same order either way.
-template <int MODE>
-cudaError_t multiply(const MulArgs& p, const CUtensorMap& left, const CUtensorMap& right, const CUtensorMap& out,
-                     int sms, cudaStream_t st) {
-  const int pairs = sms / 2;
-  const int64_t wide = (p.batch * tiles_of<MODE, 256>(p) + pairs - 1) / pairs;
-  const int64_t narrow = (p.batch * tiles_of<MODE, 128>(p) + pairs - 1) / pairs;
-  return 6 * narrow < 10 * wide ? launch_mul<MODE, 128>(p, left, right, out, pairs, st)
-                                : launch_mul<MODE, 256>(p, left, right, out, pairs, st);
+// The units of one product (of all matrices) of one step.
+template <int BN>
+cudaError_t launch_product(const MulArgs& p, const Maps& maps, int step, int mode, uint32_t pairs, cudaStream_t st) {
+  const Plan<BN> plan(p);
+  const uint32_t sym = uint32_t(p.batch) * plan.sym, app = uint32_t(p.batch) * plan.app;
+  return launch_units<BN>(p, maps, step * plan.per_step + mode * sym, mode == kApply ? app : sym, pairs, st);
+}
+
+// Wide or narrow tiles go by the rounds that the pairs of CTAs take: a narrow
+// tile takes 0.6 of a wide one's time. An element's sum has the same order
+// either way.
+bool narrow_is_faster(double narrow, double wide) { return 0.6 * narrow < wide; }
+
+// One launch for all steps where a product of all matrices fills the pairs more
+// than once, so that there is always a unit whose operands are ready; otherwise
+// a launch for each product, whose start costs less than the signals between
+// units (us, one launch against one a product: 12 x 1024 x 2816 1394 and 1556, 12 x
+// 1024 x 1024 818 and 877; 1024 x 2816 423 and 394, 128 x 1024 195 and 162).
+cudaError_t launch_steps(MulArgs p, const Maps& maps, uint32_t pairs, cudaStream_t st) {
+  const Plan<256> wide(p);
+  const Plan<128> narrow(p);
+  auto rounds = [&](uint32_t tiles) { return double((uint64_t(p.batch) * tiles + pairs - 1) / pairs); };
+  p.wait = p.batch > 1 && p.batch * wide.sym > pairs;
+  if (p.wait) {
+    auto all = [&](uint32_t sym, uint32_t app) { return rounds(sym) * (p.n + p.m) + rounds(app) * p.m; };
+    return narrow_is_faster(all(narrow.sym, narrow.app), all(wide.sym, wide.app))
+               ? launch_units<128>(p, maps, 0, narrow.total, pairs, st)
+               : launch_units<256>(p, maps, 0, wide.total, pairs, st);
+  }
+  cudaError_t e = cudaSuccess;
+  for (int step = 0; step < p.steps; ++step)
+    for (int mode = kGram; mode <= kApply && e == cudaSuccess; ++mode)
+      e = (mode == kApply ? narrow_is_faster(rounds(narrow.app), rounds(wide.app))
+                          : narrow_is_faster(rounds(narrow.sym), rounds(wide.sym)))
+              ? launch_product<128>(p, maps, step, mode, pairs, st)
+              : launch_product<256>(p, maps, step, mode, pairs, st);
+  return e;
 }
 
 // The scalar iteration s <- s (a + b s^2 + c s^4) from every start in [0, 1]
@@ -997,6 +1216,7 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
   pr.x = x;
   pr.ld = L.ldx;
   pr.parts = L.parts;
+  pr.sync = reinterpret_cast<uint64_t*>(ws + L.sync);
   pr.lo = a->dtype == NGDN2_F32;  // 16-bit updates fit their hi plane
   if (a->steps > 0 && L.m <= kSmallM && L.n <= kSmallN) {
     SmallArgs q{};
@@ -1043,14 +1263,19 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
     return e == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
   }
   // Left operands (128 rows a box), right ones (64), results (32 x 32).
-  CUtensorMap mx[2], mxr[2], mxo[2], mA, mAr, mB, mAo, mBo;
-  if (!make_map(&mx[0], x, a->batch, L.m, L.n, L.ldx, 128) || !make_map(&mx[1], y, a->batch, L.m, L.n, L.ldx, 128) ||
-      !make_map(&mxr[0], x, a->batch, L.m, L.n, L.ldx, 64) || !make_map(&mxr[1], y, a->batch, L.m, L.n, L.ldx, 64) ||
-      !make_map(&mA, A, a->batch, L.m, L.m, L.lda, 128) || !make_map(&mB, B, a->batch, L.m, L.m, L.lda, 128) ||
-      !make_map(&mAr, A, a->batch, L.m, L.m, L.lda, 64) ||
-      !make_map(&mxo[0], x, a->batch, L.m, L.n, L.ldx, 32, 32) ||
-      !make_map(&mxo[1], y, a->batch, L.m, L.n, L.ldx, 32, 32) ||
-      !make_map(&mAo, A, a->batch, L.m, L.m, L.lda, 32, 32) || !make_map(&mBo, B, a->batch, L.m, L.m, L.lda, 32, 32))
+  Maps maps;
+  const auto of_x = [&](CUtensorMap* map, const __half* q, int box, int width) {
+    return make_map(map, q, a->batch, L.m, L.n, L.ldx, box, width);
+  };
+  const auto of_a = [&](CUtensorMap* map, const __half* q, int box, int width) {
+    return make_map(map, q, a->batch, L.m, L.m, L.lda, box, width);
+  };
+  for (int i = 0; i < 2; ++i)
+    if (!of_x(&maps.x_left[i], i ? y : x, 128, kDepth) || !of_x(&maps.x_right[i], i ? y : x, 64, kDepth) ||
+        !of_x(&maps.x_out[i], i ? y : x, 32, 32))
+      return NGDN2_ERR_CUDA;
+  if (!of_a(&maps.a_left, A, 128, kDepth) || !of_a(&maps.a_right, A, 64, kDepth) || !of_a(&maps.a_out, A, 32, 32) ||
+      !of_a(&maps.b_left, B, 128, kDepth) || !of_a(&maps.b_out, B, 32, 32))
     return NGDN2_ERR_CUDA;
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -1060,38 +1285,23 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
   p.batch = a->batch;
   p.m = L.m;
   p.n = L.n;
+  p.steps = a->steps;
   p.a = a->coef[0];
   p.b = a->coef[1];
   p.c = a->coef[2];
+  p.sigma = pr.sigma;
+  p.x_lo = pr.lo;
+  p.A = A;
+  p.B = B;
+  p.ld = L.lda;
+  p.final_out = a->out;
   p.out_dtype = a->out_dtype;
   p.transposed = tall;
+  p.sync = reinterpret_cast<Sync*>(pr.sync);
   p.status = a->status;
-  for (int k = 0; k < a->steps && e == cudaSuccess; ++k) {
-    const int in = k & 1;
-    const bool last = k + 1 == a->steps, full = !(last && a->out_dtype == NGDN2_BF16);
-    const bool lo = full && (k > 0 || a->dtype == NGDN2_F32);  // whether X's lo plane counts
-    p.sigma = k == 0 ? pr.sigma : nullptr;
-    p.old = nullptr;
-    p.final_out = nullptr;
-    p.depth = L.n;
-    p.lo_left = p.lo_right = lo;
-    p.lo_out = full;
-    p.ld = L.lda;
-    p.mirror = A;
-    e = multiply<kGram>(p, mx[in], mxr[in], mAo, sms, st);
-    if (e != cudaSuccess) break;
-    p.depth = L.m;
-    p.lo_left = p.lo_right = full;
-    p.old = A;
-    p.mirror = B;
-    e = multiply<kPoly>(p, mA, mAr, mBo, sms, st);
-    if (e != cudaSuccess) break;
-    p.old = nullptr;
-    p.lo_right = lo;
-    p.lo_out = true;
-    p.final_out = last ? a->out : nullptr;
-    e = multiply<kApply>(p, mB, mxr[in], mxo[1 - in], sms, st);
-  }
+  if (double(a->batch) * a->steps * (double(L.m) / 128 + 1) * (double(L.n + L.m) / 128 + 2) >= double(1u << 31))
+    return NGDN2_ERR_SHAPE;  // units are counted in 32 bits
+  e = launch_steps(p, maps, uint32_t(sms / 2), st);
   return e == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
 }
 
