@@ -94,7 +94,7 @@ __device__ __forceinline__ void store_stream(uint16_t* p, const uint16_t& t) {
   __stcs(reinterpret_cast<unsigned short*>(p), t);
 }
 
-constexpr int kLookupThreads = 256, kLookupEach = 4;
+constexpr int kLookupThreads = 256, kLookupEach = 2;
 
 // A CTA takes ``rows`` tokens as one range of W-element pieces, each thread
 // kLookupEach of them at a time with their loads in flight together. A token

@@ -33,4 +33,22 @@ cudaError_t launch_next(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem
   return cudaLaunchKernelEx(&c, kernel, P(args)...);
 }
 
+// A plain launch of clusters of CTAs (1: none).
+template <class... P, class... A>
+cudaError_t launch_clusters(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                            int cluster, const A&... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid;
+  c.blockDim = block;
+  c.dynamicSmemBytes = smem;
+  c.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  c.attrs = at;
+  c.numAttrs = cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&c, kernel, P(args)...);
+}
+
 }  // namespace ngdn2

@@ -17,8 +17,8 @@
 // of rounding the exact one to bf16 (simulated on full-rank, decaying and
 // low-rank spectra; the last two steps would leave 1.8 times).
 //
-// Matrices of up to 128 x 256 take one CTA and one launch (orth_small_kernel).
-// Larger ones: the squared norm (partial sums in 64 bits), the conversion to
+// Matrices of up to 128 rows and about 1500 columns (more for fewer rows) take one
+// launch, a CTA or a cluster each (orth_small_kernel). Larger ones: the squared norm (partial sums in 64 bits), the conversion to
 // planes, and the products of all steps: A = X X^T, B = a I + b A
 // + c A A (both symmetric: the tiles on and above the diagonal, written twice)
 // and X' = B X, which reads X as it lies, rows along the reduction. The
@@ -499,10 +499,9 @@ __device__ __forceinline__ bool next_unit(Barriers* s, const MulArgs& p, uint32_
   return true;
 }
 
-// The result's 32 neighbouring values of one row.
+// The result's ``left`` <= 32 neighbouring values of one row.
 __device__ __forceinline__ void write_final(const MulArgs& p, int64_t b, int64_t r, int64_t c, float s,
-                                            const float* v) {
-  const int left = int(p.n - c < 32 ? p.n - c : 32);
+                                            const float* v, int left) {
   if (p.transposed) {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
@@ -566,7 +565,7 @@ __device__ __forceinline__ void emit32(const MulArgs& p, const Unit& u, const CU
   const int lane = threadIdx.x & 31, z = int(u.b * 2);
   const int64_t r = r0 + lane, cols = MODE == kApply ? p.n : p.m;
   if (MODE == kApply && u.last) {
-    if (r < p.m) write_final(p, u.b, r, c, sigma / kScale, v);
+    if (r < p.m) write_final(p, u.b, r, c, sigma / kScale, v, int(p.n - c < 32 ? p.n - c : 32));
     return;
   }
   __half h[32], l[32];
@@ -835,45 +834,84 @@ done:
 }
 
 // ---------------------------------------------------------------------------
-// Small matrices (m <= 128, n <= 256): the whole iteration in one CTA. X and A (then B
-// in its place) stay in shared memory as hi and lo planes in blocks of 64
-// columns, 128 rows of 128 bytes, 128-byte swizzled: as they lie they are left
+// Matrices of m <= 128 and few enough columns: the whole iteration in one launch,
+// a cluster of CTAs a matrix, each with a slice of X's columns. X's slice and A
+// (then B in its place) stay in shared memory as hi and lo planes in blocks of
+// 64 columns, rows of 128 bytes, 128-byte swizzled: as they lie they are left
 // and right operands with the reduction along the rows, and X is the right
-// operand with the reduction down the columns.
+// operand with the reduction down the columns. A's slices are summed through
+// distributed shared memory: every CTA adds up a part of A's columns and
+// gives its planes to all. What bounds it is the chain of a step's three
+// products, 2.5 us each, most of it not the MMAs but getting the results out of
+// tensor memory and back as operands.
 // ---------------------------------------------------------------------------
 
-constexpr int kSmallM = 128, kSmallN = 256, kSmallThreads = 512;
-constexpr int kBlock = 128 * 128;  // bytes of one plane's 64 columns
-
-int small_smem(int64_t m, int64_t n) {
-  return int(2 * kBlock * ((n + 63) / 64 + (m + 63) / 64)) + 1024;
-}
-
-__device__ __forceinline__ uint32_t block_at(int r, int c) {
-  return (c >> 6) * kBlock + (r >> 3) * 1024 + (r & 7) * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4) + (c & 7) * 2;
-}
+constexpr int kSmallM = 128, kSmallThreads = 512, kSmallCtas = 8;
+constexpr int kSmallMost = 227 * 1024 - 512;  // bytes of shared memory
 
 struct SmallArgs {
   PrepArgs in;
   MulArgs out;
-  int steps;
+  int ctas, slice;  // of a matrix; columns of X a CTA, a multiple of 16
+  int rows;         // m up to a multiple of 16
+  int part;         // columns of A that a CTA adds up, a multiple of 4
 };
+
+// Bytes of a plane's block of 64 columns, of X's and A's planes, of the sums.
+struct SmallLayout {
+  int block, x_plane, a_plane, sums, total;
+  __host__ __device__ explicit SmallLayout(const SmallArgs& q) {
+    block = q.rows * 128;
+    x_plane = block * ((q.slice + 63) / 64);
+    a_plane = block * ((q.rows + 63) / 64);
+    sums = q.ctas > 1 ? q.ctas * q.part * q.rows * 4 : 0;
+    // An MMA reads 128 rows, whatever lies there: the last block's reach.
+    total = 2 * (x_plane + a_plane) + sums + (128 * 128 - block) + 1024;
+  }
+};
+
+// As few CTAs as hold the matrix; false where kSmallCtas do not.
+bool fits_small(SmallArgs* q, int64_t m, int64_t n) {
+  if (m > kSmallM) return false;
+  q->rows = int(m + 15) / 16 * 16;
+  for (q->ctas = 1; q->ctas <= kSmallCtas; q->ctas *= 2) {
+    const int64_t slice = ((n + q->ctas - 1) / q->ctas + 15) / 16 * 16;
+    if (slice > 256) continue;
+    q->slice = int(slice);
+    q->part = ((q->rows + q->ctas - 1) / q->ctas + 3) / 4 * 4;
+    if (SmallLayout(*q).total <= kSmallMost) return true;
+  }
+  return false;
+}
+
+// Byte of element (r, c) in a plane.
+__device__ __forceinline__ uint32_t block_at(int block, int r, int c) {
+  return (c >> 6) * block + (r >> 3) * 1024 + (r & 7) * 128 + ((((c & 63) >> 3) ^ (r & 7)) << 4) + (c & 7) * 2;
+}
+
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
 
 template <int DT>
 __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __grid_constant__ SmallArgs q) {
   extern __shared__ unsigned char raw[];
-  __shared__ double red[kSmallThreads / 32];
+  __shared__ double red[kSmallThreads / 32], slices[kSmallCtas];
   __shared__ uint64_t bar;
   __shared__ uint32_t tmem_at;
   const PrepArgs& p = q.in;
+  const SmallLayout lay(q);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int m = int(p.m), n = int(p.n);
-  const int64_t b = blockIdx.x;
+  const int m = int(p.m), ctas = q.ctas, rank = ctas > 1 ? int(cluster_rank()) : 0;
+  const int64_t b = blockIdx.x / ctas, col0 = int64_t(rank) * q.slice;
+  const int n = int(p.n - col0 < 0 ? 0 : p.n - col0 < q.slice ? p.n - col0 : q.slice);  // columns here
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   unsigned char* mem = raw + (base - smem_u32(raw));
-  const int xp = kBlock * ((n + 63) / 64), ap = kBlock * ((m + 63) / 64);  // bytes of a plane
-  unsigned char *mx = mem, *ma = mem + 2 * xp;
-  const uint32_t ax = base, aa = base + 2 * xp;
+  const int xp = lay.x_plane, ap = lay.a_plane, block = lay.block;
+  unsigned char *mx = mem, *ma = mem + 2 * xp, *ms = ma + 2 * ap;
+  const uint32_t ax = base, aa = base + 2 * xp, as = aa + 2 * ap;
   if (tid == 0) {
     mbar_init(&bar, 1);
     fence_mbar_init();
@@ -881,12 +919,14 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   if (warp == 0) tmem_alloc(&tmem_at, 256);
   for (int i = tid * 16; i < 2 * (xp + ap); i += kSmallThreads * 16)
     *reinterpret_cast<uint4*>(mem + i) = make_uint4(0, 0, 0, 0);
-  // The norm, then the planes of the scaled update. Threads along the
-  // dimension with the smaller stride.
+  // The norm, then the planes of the scaled update. Lanes along the dimension
+  // with the smaller stride; a warp takes four rows at a time, their loads in
+  // flight together.
   const bool along_c = p.sc <= p.sr;
   const int outer = along_c ? m : n, inner = along_c ? n : m;
   const int64_t so = along_c ? p.sr : p.sc, si = along_c ? p.sc : p.sr;
-  auto each = [&](auto&& f) {  // a warp takes four rows at a time, their loads in flight together
+  const int64_t origin = b * p.sb + col0 * p.sc;
+  auto each = [&](auto&& f) {
     constexpr int kWarps = kSmallThreads / 32;
     for (int i0 = warp; i0 < outer; i0 += 4 * kWarps)
 #pragma unroll 4
@@ -894,7 +934,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
         float x[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u)
-          x[u] = i0 + u * kWarps < outer ? load_typed<DT>(p.g, b * p.sb + (i0 + u * kWarps) * so + j * si) : 0.f;
+          x[u] = i0 + u * kWarps < outer ? load_typed<DT>(p.g, origin + (i0 + u * kWarps) * so + j * si) : 0.f;
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const int i = i0 + u * kWarps;
@@ -912,6 +952,13 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   fence_after_sync();
   sum = 0.0;
   for (int w = 0; w < kSmallThreads / 32; ++w) sum += red[w];
+  if (ctas > 1) {
+    if (tid < ctas)
+      asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(in_cta(smem_u32(&slices[rank]), tid)), "d"(sum) : "memory");
+    cluster_barrier();
+    sum = 0.0;
+    for (int i = 0; i < ctas; ++i) sum += slices[i];
+  }
   int k2;
   float sigma;
   scale_of(sum, p.eps, &k2, &sigma);
@@ -919,33 +966,33 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   each([&](int r, int c, float x) {
     __half h, l;
     split(x * s1 * s2, h, l);
-    *reinterpret_cast<__half*>(mx + block_at(r, c)) = h;
-    *reinterpret_cast<__half*>(mx + xp + block_at(r, c)) = l;
+    *reinterpret_cast<__half*>(mx + block_at(block, r, c)) = h;
+    *reinterpret_cast<__half*>(mx + xp + block_at(block, r, c)) = l;
   });
   const uint32_t tmem = tmem_at;
   const int quarter = warp & 3, c1 = (warp >> 2) * 32, row = quarter * 32 + lane;
-  const int mn = (m + 15) & ~15, nn = (n + 15) & ~15;
   uint32_t phase = 0;
   bool alive = true;
 
-  // D[128 x cols] = L R, reduction over ``depth`` (multiples of 16).
+  // D[128 x cols] = L R, reduction over ``depth`` (multiples of 16). After a wait
+  // that gave up nothing is multiplied any more, but the cluster goes on
+  // together.
   auto product = [&](uint32_t L, int lp, uint32_t R, int rp, int depth, int cols, bool down, bool full) {
     fence_proxy_async();
     fence_before_sync();
     __syncthreads();
+    if (!alive) return;
     if (tid == 0) {
       fence_after_sync();
       const uint32_t idesc = idesc_f16(128, cols, false, false, down);
       for (int kk = 0; kk < depth / 16; ++kk) {
-        auto dl = [&](int pl) { return desc_sw128(L + pl * lp + (kk >> 2) * kBlock + (kk & 3) * 32, 1024); };
-        auto dr = [&](int pl) {
-          return down ? desc_sw128_mn(R + pl * rp + kk * 2048, kBlock)
-                      : desc_sw128(R + pl * rp + (kk >> 2) * kBlock + (kk & 3) * 32, 1024);
-        };
-        mma_f16(tmem, dl(0), dr(0), idesc, kk > 0);
+        const uint64_t dl = desc_sw128(L + (kk >> 2) * block + (kk & 3) * 32, 1024);
+        const uint64_t dr = down ? desc_sw128_mn(R + kk * 2048, block)
+                                 : desc_sw128(R + (kk >> 2) * block + (kk & 3) * 32, 1024);
+        mma_f16(tmem, dl, dr, idesc, kk > 0);
         if (full) {
-          mma_f16(tmem, dl(0), dr(1), idesc, 1);
-          mma_f16(tmem, dl(1), dr(0), idesc, 1);
+          mma_f16(tmem, dl, dr + (rp >> 4), idesc, 1);
+          mma_f16(tmem, dl + (lp >> 4), dr, idesc, 1);
         }
       }
       mma_commit(&bar);
@@ -954,38 +1001,81 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
     phase ^= 1;
     fence_after_sync();
     if (!ok) atomicOr(q.out.status, NGDN2_STATUS_WAIT_TIMEOUT);
-    return !__syncthreads_or(!ok);
+    alive = !__syncthreads_or(!ok);
   };
   // Eight results as planes.
   auto put8 = [&](unsigned char* to, int plane, int c, const float* x) {
     alignas(16) __half h[8], l[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) split(x[j], h[j], l[j]);
-    *reinterpret_cast<uint4*>(to + block_at(row, c)) = *reinterpret_cast<const uint4*>(h);
-    *reinterpret_cast<uint4*>(to + plane + block_at(row, c)) = *reinterpret_cast<const uint4*>(l);
+    *reinterpret_cast<uint4*>(to + block_at(block, row, c)) = *reinterpret_cast<const uint4*>(h);
+    *reinterpret_cast<uint4*>(to + plane + block_at(block, row, c)) = *reinterpret_cast<const uint4*>(l);
   };
 
-  for (int step = 0; step < q.steps && alive; ++step, sigma = 1.f / kScale) {
-    const bool full = !(step + 1 == q.steps && q.out.out_dtype == NGDN2_BF16);
+  const int rows = q.rows, cols = (n + 15) & ~15;
+  for (int step = 0; step < q.out.steps; ++step, sigma = 1.f / kScale) {
+    const bool full = !(step + 1 == q.out.steps && q.out.out_dtype == NGDN2_BF16);
     float v[32];
-    alive = product(ax, xp, ax, xp, nn, mn, false, full);
-    if (!alive) break;
-    for (int c = c1; c < m; c += 128) {
-      tmem_ld32(taddr(tmem, quarter * 32, c), v);
+    product(ax, xp, ax, xp, cols, rows, false, full);
+    if (ctas == 1) {
+      for (int c = c1; c < m; c += 128) {
+        tmem_ld32(taddr(tmem, quarter * 32, c), v);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = c + i < m ? v[i] * sigma * sigma * kScale : 0.f;
+        for (int i = 0; i < 32; ++i) v[i] = c + i < m ? v[i] * sigma * sigma * kScale : 0.f;
 #pragma unroll
-      for (int i = 0; i < 32; i += 8) put8(ma, ap, c + i, v + i);
+        for (int i = 0; i < 32; i += 8)
+          if (row < rows && c + i < rows) put8(ma, ap, c + i, v + i);
+      }
+    } else {
+      // Four columns of all rows lie together, by source.
+      if (c1 < rows) {
+        tmem_ld32(taddr(tmem, quarter * 32, c1), v);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const int c = c1 + i, to = c / q.part, g = c % q.part / 4;
+          const float z = cols > 0 ? 1.f : 0.f;  // (no columns here: nothing was multiplied)
+          if (c < rows && row < rows)
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             in_cta(as + ((rank * (q.part / 4) + g) * rows + row) * 16, to)),
+                         "f"(z > 0.f ? v[i] : 0.f), "f"(z > 0.f ? v[i + 1] : 0.f), "f"(z > 0.f ? v[i + 2] : 0.f),
+                         "f"(z > 0.f ? v[i + 3] : 0.f)
+                         : "memory");
+        }
+      }
+      cluster_barrier();
+      for (int e = tid; e < rows * (q.part / 4); e += kSmallThreads) {
+        const int r = e % rows, g = e / rows, c = rank * q.part + 4 * g;
+        if (c >= rows) break;
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < ctas; ++j) {
+          const float4 f = *reinterpret_cast<const float4*>(ms + ((j * (q.part / 4) + g) * rows + r) * 16);
+          t.x += f.x;
+          t.y += f.y;
+          t.z += f.z;
+          t.w += f.w;
+        }
+        const float w[4] = {t.x, t.y, t.z, t.w};
+        alignas(8) __half h[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split(c + i < m ? w[i] * sigma * sigma * kScale : 0.f, h[i], l[i]);
+        const uint2 hv = *reinterpret_cast<const uint2*>(h), lv = *reinterpret_cast<const uint2*>(l);
+        for (int j = 0; j < ctas; ++j) {
+          const uint32_t at = in_cta(aa + block_at(block, r, c), j);
+          asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(hv.x), "r"(hv.y) : "memory");
+          asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at + ap), "r"(lv.x), "r"(lv.y) : "memory");
+        }
+      }
+      cluster_barrier();
     }
-    alive = product(aa, ap, aa, ap, mn, mn, false, full);
-    if (!alive) break;
+    product(aa, ap, aa, ap, rows, rows, false, full);
     for (int c = c1; c < m; c += 128) {
       tmem_ld32(taddr(tmem, quarter * 32, c), v);
 #pragma unroll
       for (int i = 0; i < 32; i += 8) {
+        if (row >= rows || c + i >= rows) continue;
         alignas(16) __half h[8], l[8];
-        *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(ma + block_at(row, c + i));
-        *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(ma + ap + block_at(row, c + i));
+        *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(ma + block_at(block, row, c + i));
+        *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(ma + ap + block_at(block, row, c + i));
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           v[i + j] = c + i + j < m ? q.out.c * (v[i + j] / kScale) +
@@ -995,23 +1085,23 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
         put8(ma, ap, c + i, v + i);
       }
     }
-    alive = product(aa, ap, ax, xp, mn, nn, true, full);
-    if (!alive) break;
+    if (cols > 0) product(aa, ap, ax, xp, rows, cols, true, full);
     for (int c = c1; c < n; c += 128) {
       tmem_ld32(taddr(tmem, quarter * 32, c), v);
-      if (step + 1 == q.steps) {
-        if (row < m) write_final(q.out, b, row, c, sigma / kScale, v);
+      if (step + 1 == q.out.steps) {
+        if (row < m) write_final(q.out, b, row, col0 + c, sigma / kScale, v, int(n - c < 32 ? n - c : 32));
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = c + i < n ? v[i] * sigma : 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) put8(mx, xp, c + i, v + i);
+        for (int i = 0; i < 32; i += 8)
+          if (row < rows && c + i < q.slice) put8(mx, xp, c + i, v + i);
       }
     }
   }
   if (!alive) {  // nothing that was not computed passes as a result
-    for (int e = tid; e < m * n; e += kSmallThreads)
-      store_elem(q.out.final_out, b * m * n + e, __int_as_float(0x7fc00000), q.out.out_dtype);
+    for (int64_t e = tid; e < p.m * p.n; e += kSmallThreads)
+      store_elem(q.out.final_out, b * p.m * p.n + e, __int_as_float(0x7fc00000), q.out.out_dtype);
   }
   fence_before_sync();
   __syncthreads();
@@ -1218,11 +1308,12 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
   pr.parts = L.parts;
   pr.sync = reinterpret_cast<uint64_t*>(ws + L.sync);
   pr.lo = a->dtype == NGDN2_F32;  // 16-bit updates fit their hi plane
-  if (a->steps > 0 && L.m <= kSmallM && L.n <= kSmallN) {
-    SmallArgs q{};
+  SmallArgs q{};
+  if (a->steps > 0 && fits_small(&q, L.m, L.n)) {
     q.in = pr;
     q.out.m = L.m;
     q.out.n = L.n;
+    q.out.steps = a->steps;
     q.out.a = a->coef[0];
     q.out.b = a->coef[1];
     q.out.c = a->coef[2];
@@ -1230,13 +1321,13 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
     q.out.out_dtype = a->out_dtype;
     q.out.transposed = tall;
     q.out.status = a->status;
-    q.steps = a->steps;
-    const int smem = small_smem(L.m, L.n);
+    const int smem = SmallLayout(q).total;
     const cudaError_t e = by_type(a->dtype, [&](auto T) {
       auto* kernel = orth_small_kernel<decltype(T)::value>;
       const cudaError_t f = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
       return f != cudaSuccess ? f
-                              : launch_next(kernel, dim3(unsigned(a->batch)), dim3(kSmallThreads), smem, st, false, q);
+                              : launch_clusters(kernel, dim3(unsigned(a->batch * q.ctas)), dim3(kSmallThreads), smem,
+                                                st, q.ctas, q);
     });
     return e == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
   }

@@ -76,6 +76,19 @@ def test_batches(shape):
         assert torch.equal(orthogonalize(flat[i]), fo[i])
 
 
+@pytest.mark.parametrize("shape", [(128, 1500), (16, 2048), (5, 1999), (2049, 1), (1100, 112), (3, 100, 900),
+                                   (128, 1600), (120, 4000), (2, 12, 64, 520)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_few_rows_and_many_columns(shape, dtype):
+    """A small side of at most 128: on either side of what one launch holds, and
+    slices that do not come out even."""
+    G = _update(shape, dtype, seed=11)
+    out = orthogonalize(G, dtype=torch.float32)
+    _check(G, out)
+    flat, fo = G.reshape(-1, *shape[-2:]), out.reshape(-1, *shape[-2:])
+    assert torch.equal(orthogonalize(flat[-1], dtype=torch.float32), fo[-1])
+
+
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_types(dtype, out):
