@@ -840,8 +840,8 @@ done:
 // 64 columns, rows of 128 bytes, 128-byte swizzled: as they lie they are left
 // and right operands with the reduction along the rows, and X is the right
 // operand with the reduction down the columns. A's slices are summed through
-// distributed shared memory: every CTA adds up a part of A's columns and
-// gives its planes to all. What bounds it is the chain of a step's three
+// distributed shared memory: every CTA adds up a part of A's rows and gives its
+// planes to all. What bounds it is the chain of a step's three
 // products, 2.5 us each, most of it not the MMAs but getting the results out of
 // tensor memory and back as operands.
 // ---------------------------------------------------------------------------
@@ -854,7 +854,7 @@ struct SmallArgs {
   MulArgs out;
   int ctas, slice;  // of a matrix; columns of X a CTA, a multiple of 16
   int rows;         // m up to a multiple of 16
-  int part;         // columns of A that a CTA adds up, a multiple of 4
+  int part;         // rows of A that a CTA adds up, a multiple of 8
 };
 
 // Bytes of a plane's block of 64 columns, of X's and A's planes, of the sums.
@@ -864,7 +864,7 @@ struct SmallLayout {
     block = q.rows * 128;
     x_plane = block * ((q.slice + 63) / 64);
     a_plane = block * ((q.rows + 63) / 64);
-    sums = q.ctas > 1 ? q.ctas * q.part * q.rows * 4 : 0;
+    sums = q.ctas > 1 ? q.ctas * (q.rows / 4) * (q.part + 1) * 16 : 0;
     // An MMA reads 128 rows, whatever lies there: the last block's reach.
     total = 2 * (x_plane + a_plane) + sums + (128 * 128 - block) + 1024;
   }
@@ -878,7 +878,7 @@ bool fits_small(SmallArgs* q, int64_t m, int64_t n) {
     const int64_t slice = ((n + q->ctas - 1) / q->ctas + 15) / 16 * 16;
     if (slice > 256) continue;
     q->slice = int(slice);
-    q->part = ((q->rows + q->ctas - 1) / q->ctas + 3) / 4 * 4;
+    q->part = ((q->rows + q->ctas - 1) / q->ctas + 7) / 8 * 8;
     if (SmallLayout(*q).total <= kSmallMost) return true;
   }
   return false;
@@ -1027,42 +1027,46 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
           if (row < rows && c + i < rows) put8(ma, ap, c + i, v + i);
       }
     } else {
-      // Four columns of all rows lie together, by source.
+      // By source, four columns of a CTA's rows lie together (and a gap, for the
+      // banks): neighbouring lanes send to neighbouring places.
+      const int groups = rows / 4, gap = q.part + 1;
       if (c1 < rows) {
         tmem_ld32(taddr(tmem, quarter * 32, c1), v);
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const int c = c1 + i, to = c / q.part, g = c % q.part / 4;
-          const float z = cols > 0 ? 1.f : 0.f;  // (no columns here: nothing was multiplied)
-          if (c < rows && row < rows)
-            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(
-                             in_cta(as + ((rank * (q.part / 4) + g) * rows + row) * 16, to)),
-                         "f"(z > 0.f ? v[i] : 0.f), "f"(z > 0.f ? v[i + 1] : 0.f), "f"(z > 0.f ? v[i + 2] : 0.f),
-                         "f"(z > 0.f ? v[i + 3] : 0.f)
+        for (int i = 0; i < 32; ++i) v[i] = cols > 0 ? v[i] : 0.f;  // (no columns here: nothing was multiplied)
+        const uint32_t to = in_cta(as + ((rank * groups + c1 / 4) * gap + row % q.part) * 16, row / q.part);
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          if (c1 + i < rows && row < rows)
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + i / 4 * gap * 16), "f"(v[i]),
+                         "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3])
                          : "memory");
-        }
       }
       cluster_barrier();
-      for (int e = tid; e < rows * (q.part / 4); e += kSmallThreads) {
-        const int r = e % rows, g = e / rows, c = rank * q.part + 4 * g;
-        if (c >= rows) break;
-        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+      // Eight columns of a row a thread; eight neighbours' results are 128 bytes.
+      for (int e = tid; e < q.part * (rows / 8); e += kSmallThreads) {
+        const int g = e % (rows / 8), r = rank * q.part + e / (rows / 8);
+        if (r >= rows) break;
+        float w[8] = {};
         for (int j = 0; j < ctas; ++j) {
-          const float4 f = *reinterpret_cast<const float4*>(ms + ((j * (q.part / 4) + g) * rows + r) * 16);
-          t.x += f.x;
-          t.y += f.y;
-          t.z += f.z;
-          t.w += f.w;
+          const unsigned char* f = ms + ((j * groups + 2 * g) * gap + e / (rows / 8)) * 16;
+          const float4 f0 = *reinterpret_cast<const float4*>(f), f1 = *reinterpret_cast<const float4*>(f + gap * 16);
+          w[0] += f0.x; w[1] += f0.y; w[2] += f0.z; w[3] += f0.w;
+          w[4] += f1.x; w[5] += f1.y; w[6] += f1.z; w[7] += f1.w;
         }
-        const float w[4] = {t.x, t.y, t.z, t.w};
-        alignas(8) __half h[4], l[4];
+        alignas(16) __half h[8], l[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) split(c + i < m ? w[i] * sigma * sigma * kScale : 0.f, h[i], l[i]);
-        const uint2 hv = *reinterpret_cast<const uint2*>(h), lv = *reinterpret_cast<const uint2*>(l);
+        for (int i = 0; i < 8; ++i) split(8 * g + i < m ? w[i] * sigma * sigma * kScale : 0.f, h[i], l[i]);
+        const uint4 hv = *reinterpret_cast<const uint4*>(h), lv = *reinterpret_cast<const uint4*>(l);
+        const uint32_t at = aa + block_at(block, r, 8 * g);
         for (int j = 0; j < ctas; ++j) {
-          const uint32_t at = in_cta(aa + block_at(block, r, c), j);
-          asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at), "r"(hv.x), "r"(hv.y) : "memory");
-          asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(at + ap), "r"(lv.x), "r"(lv.y) : "memory");
+          const uint32_t to = in_cta(at, j);
+          asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(hv.x), "r"(hv.y), "r"(hv.z),
+                       "r"(hv.w)
+                       : "memory");
+          asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + ap), "r"(lv.x), "r"(lv.y),
+                       "r"(lv.z), "r"(lv.w)
+                       : "memory");
         }
       }
       cluster_barrier();
