@@ -32,6 +32,12 @@ namespace {
 constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr unsigned kAll = 0xffffffffu;
+
+// CTAs a multiprocessor: 64 registers a thread forward, 80 (16-bit x) or 128
+// backward.
+constexpr int kFwdCtas = 8;
+constexpr int bwd_ctas(int x_dtype) { return x_dtype == NGDN2_F32 ? 4 : 6; }
+
 constexpr uint32_t kPollLimit = 1u << 21;
 
 bool dtype_ok(int d) { return d == NGDN2_F32 || d == NGDN2_BF16 || d == NGDN2_F16; }
@@ -284,7 +290,7 @@ constexpr int fwd_smem() {
 }
 
 template <int XT, int GT, int G, int CL, int R>
-__global__ void __launch_bounds__(kThreads, 8)
+__global__ void __launch_bounds__(kThreads, kFwdCtas)
 scan_kernel(const __grid_constant__ ngdn2_scan_args a, Chain chain, int row_strips) {
   constexpr int kCh = 4 * CL, NV = kCh / 32, kSteps = kThreads / CL * R;
   using SX = Stage<XT, CL, R>;
@@ -422,7 +428,7 @@ constexpr int bwd_smem() {
 }
 
 template <int XT, int GT, int G, int CL, int R>
-__global__ void __launch_bounds__(kThreads, XT == NGDN2_F32 ? 4 : 6)
+__global__ void __launch_bounds__(kThreads, bwd_ctas(XT))
 scan_bwd_kernel(const __grid_constant__ ngdn2_scan_bwd_args p, Chain chain, int row_strips) {
   constexpr int kCh = 4 * CL, NV = kCh / 32, kSteps = kThreads / CL * R;
   static_assert(NGDN2_SCAN_CHUNK % kSteps == 0, "a tile starts at a state that the forward left, or within its chunk as the only tile");
@@ -628,17 +634,18 @@ int granule(const void* p, int dt, const int64_t* st, int64_t D) {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-// At most as many CTAs as the GPU holds at once.
+// ``per_sm`` CTAs a multiprocessor at most (what the registers allow; where
+// shared memory holds fewer, the others find no tile left).
 template <class K, class... Args>
-cudaError_t launch(K kernel, int64_t tiles, int smem, cudaStream_t st, const Args&... args) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  int dev = 0, sms = 0, per_sm = 0;
+cudaError_t launch(K kernel, int64_t tiles, int per_sm, int smem, cudaStream_t st, const Args&... args) {
+  cudaError_t e = cudaSuccess;
+  if (smem > 32 * 1024)  // (with the static part it may pass what needs no asking)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  int dev = 0, sms = 0;
   if (e == cudaSuccess) e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e == cudaSuccess)
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, smem);
   if (e != cudaSuccess) return e;
-  const int64_t fit = int64_t(sms) * (per_sm > 0 ? per_sm : 1);
+  const int64_t fit = int64_t(sms) * per_sm;
   kernel<<<unsigned(tiles < fit ? tiles : fit), kThreads, smem, st>>>(args...);
   return cudaGetLastError();
 }
@@ -759,7 +766,7 @@ NGDN2_API int ngdn2_scan(const ngdn2_scan_args* a, void* stream) {
     constexpr int XT = decltype(X)::value, GT = decltype(Gt)::value;
     return by_tile(s.channels, g, [&](auto GR, auto CLc, auto Rc) {
       constexpr int G = decltype(GR)::value, CL = decltype(CLc)::value, R = decltype(Rc)::value;
-      return launch(scan_kernel<XT, GT, G, CL, R>, s.strips * s.tiles, fwd_smem<XT, GT, CL, R>(), st,
+      return launch(scan_kernel<XT, GT, G, CL, R>, s.strips * s.tiles, kFwdCtas, fwd_smem<XT, GT, CL, R>(), st,
                     *a, chain, s.row_strips);
     });
   });
@@ -784,7 +791,7 @@ NGDN2_API int ngdn2_scan_bwd(const ngdn2_scan_bwd_args* p, void* stream) {
     constexpr int XT = decltype(X)::value, GT = decltype(Gt)::value;
     return by_tile(s.channels, g, [&](auto GR, auto CLc, auto Rc) {
       constexpr int G = decltype(GR)::value, CL = decltype(CLc)::value, R = decltype(Rc)::value;
-      return launch(scan_bwd_kernel<XT, GT, G, CL, R>, s.strips * s.tiles,
+      return launch(scan_bwd_kernel<XT, GT, G, CL, R>, s.strips * s.tiles, bwd_ctas(XT),
                     bwd_smem<XT, GT, CL, R>(), st, *p, chain, s.row_strips);
     });
   });

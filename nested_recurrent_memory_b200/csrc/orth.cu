@@ -590,16 +590,27 @@ __device__ __forceinline__ void emit32(const MulArgs& p, const Unit& u, const CU
     *reinterpret_cast<uint4*>(mem + kOutPlane + out_at(lane, i)) = *reinterpret_cast<const uint4*>(l + i);
   }
   store_stage(out, int(c), int(r0), z, smem_u32(mem), u.lo_out);
-  if (MODE != kApply && mirror && r < p.m) {
-    // The same below the diagonal: lanes are neighbours there. (Through the
-    // stage as well, each store would wait for the one before.)
-    __half* to = (MODE == kGram ? p.A : p.B) + (int64_t(z) * p.m + c) * p.ld + r;
+  if (MODE != kApply && mirror) {
+    // The same below the diagonal, where lanes are neighbours: two lanes swap
+    // values so that each stores two of them, of every other column. (Through
+    // the stage as well, each store would wait for the one before.)
+    const int odd = lane & 1;
+    const int64_t even = r - odd;
+    __half* to = (MODE == kGram ? p.A : p.B) + (int64_t(z) * p.m + c + odd) * p.ld + even;
+    auto swap = [&](__half keep, __half give) {
+      const uint32_t g = __shfl_xor_sync(0xffffffffu, uint32_t(__half_as_ushort(give)), 1);
+      const uint32_t k = __half_as_ushort(keep);
+      return odd ? g | k << 16 : k | g << 16;
+    };
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (c + i < cols) {
-        to[i * p.ld] = h[i];
-        if (u.lo_out) to[(p.m + i) * p.ld] = l[i];
+    for (int i = 0; i < 32; i += 2) {
+      const uint32_t hv = swap(odd ? h[i + 1] : h[i], odd ? h[i] : h[i + 1]);
+      const uint32_t lv = swap(odd ? l[i + 1] : l[i], odd ? l[i] : l[i + 1]);
+      if (even < p.m && c + i + odd < cols) {  // (a row has room for an even number)
+        *reinterpret_cast<uint32_t*>(to + i * p.ld) = hv;
+        if (u.lo_out) *reinterpret_cast<uint32_t*>(to + (p.m + i) * p.ld) = lv;
       }
+    }
   }
 }
 
