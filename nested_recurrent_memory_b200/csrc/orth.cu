@@ -316,7 +316,7 @@ template <int BN>
 struct Plan {
   uint32_t sym, app;  // tiles of A or B (those that reach the diagonal or lie above it), and of X'
   uint32_t cols_s, cols_a, per_step, total;
-  __host__ __device__ explicit Plan(const MulArgs& p) {
+  explicit Plan(const MulArgs& p) {
     const uint32_t rows = uint32_t((p.m + kRows - 1) / kRows);
     cols_s = uint32_t((p.m + BN - 1) / BN);
     cols_a = uint32_t((p.n + BN - 1) / BN);
@@ -499,32 +499,38 @@ __device__ __forceinline__ bool next_unit(Barriers* s, const MulArgs& p, uint32_
   return true;
 }
 
-// The result's ``left`` <= 32 neighbouring values of one row.
+// Up to eight neighbouring values of one row of the result, ``left`` of them there.
 __device__ __forceinline__ void write_final(const MulArgs& p, int64_t b, int64_t r, int64_t c, float s,
                                             const float* v, int left) {
   if (p.transposed) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < 8; ++i)
       if (i < left) store_elem(p.final_out, (b * p.n + c + i) * p.m + r, s * v[i], p.out_dtype);
     return;
   }
   const int64_t o = (b * p.m + r) * p.n + c;
   const int el = p.out_dtype == NGDN2_F32 ? 4 : 2;
   char* to = static_cast<char*>(p.final_out) + o * el;
-  if (left == 32 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
+  if (left >= 8 && reinterpret_cast<uintptr_t>(to) % 16 == 0) {
+    alignas(16) unsigned char w[32];
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      alignas(16) unsigned char w[32];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) store_elem(w, j, s * v[i + j], p.out_dtype);
-      reinterpret_cast<uint4*>(to)[i * el / 16] = *reinterpret_cast<const uint4*>(w);
-      if (el == 4) reinterpret_cast<uint4*>(to)[i * el / 16 + 1] = *reinterpret_cast<const uint4*>(w + 16);
-    }
+    for (int j = 0; j < 8; ++j) store_elem(w, j, s * v[j], p.out_dtype);
+    *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(w);
+    if (el == 4) reinterpret_cast<uint4*>(to)[1] = *reinterpret_cast<const uint4*>(w + 16);
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
+    for (int i = 0; i < 8; ++i)
       if (i < left) store_elem(p.final_out, o + i, s * v[i], p.out_dtype);
   }
+}
+
+// Eight columns of a warp's 32 lanes of tensor memory.
+__device__ __forceinline__ void tmem_ld8(uint32_t at, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  __syncwarp();
+  tmem_ld8_nowait(at, r);
+  tmem_wait_ld();
+  tmem_regs_after_wait8(r);
 }
 
 // Byte of element (row, col) in a writing warp's stage plane.
@@ -556,85 +562,29 @@ __device__ __forceinline__ void stage_free() {
   __syncwarp();
 }
 
-// A row's 32 neighbouring results, from the sums v: to the planes by way of the
-// warp's stage, or the final values. Whole warps; r0 is lane 0's row.
-template <int MODE>
-__device__ __forceinline__ void emit32(const MulArgs& p, const Unit& u, const CUtensorMap* out, unsigned char* mem,
-                                       int64_t r0, int64_t c, bool mirror, float sigma, const float* v,
-                                       const uint4* oh, const uint4* ol) {
-  const int lane = threadIdx.x & 31, z = int(u.b * 2);
-  const int64_t r = r0 + lane, cols = MODE == kApply ? p.n : p.m;
-  if (MODE == kApply && u.last) {
-    if (r < p.m) write_final(p, u.b, r, c, sigma / kScale, v, int(p.n - c < 32 ? p.n - c : 32));
-    return;
-  }
-  __half h[32], l[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    float x;
-    if (MODE == kGram) {
-      x = v[i] * sigma * sigma * kScale;
-    } else if (MODE == kPoly) {
-      const __half *ph = reinterpret_cast<const __half*>(oh), *pl = reinterpret_cast<const __half*>(ol);
-      x = p.c * (v[i] / kScale) + p.b * (__half2float(ph[i]) + __half2float(pl[i])) +
-          (c + i == r ? p.a * kScale : 0.f);
-    } else {
-      x = v[i] * sigma;  // (sigma X^) (B^ / kScale), times kScale
-    }
-    split(x, h[i], l[i]);
-  }
-  stage_free();
-#pragma unroll
-  for (int i = 0; i < 32; i += 8) {
-    *reinterpret_cast<uint4*>(mem + out_at(lane, i)) = *reinterpret_cast<const uint4*>(h + i);
-    *reinterpret_cast<uint4*>(mem + kOutPlane + out_at(lane, i)) = *reinterpret_cast<const uint4*>(l + i);
-  }
-  store_stage(out, int(c), int(r0), z, smem_u32(mem), u.lo_out);
-  if (MODE != kApply && mirror) {
-    // The same below the diagonal, where lanes are neighbours: two lanes swap
-    // values so that each stores two of them, of every other column. (Through
-    // the stage as well, each store would wait for the one before.)
-    const int odd = lane & 1;
-    const int64_t even = r - odd;
-    __half* to = (MODE == kGram ? p.A : p.B) + (int64_t(z) * p.m + c + odd) * p.ld + even;
-    auto swap = [&](__half keep, __half give) {
-      const uint32_t g = __shfl_xor_sync(0xffffffffu, uint32_t(__half_as_ushort(give)), 1);
-      const uint32_t k = __half_as_ushort(keep);
-      return odd ? g | k << 16 : k | g << 16;
-    };
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const uint32_t hv = swap(odd ? h[i + 1] : h[i], odd ? h[i] : h[i + 1]);
-      const uint32_t lv = swap(odd ? l[i + 1] : l[i], odd ? l[i] : l[i + 1]);
-      if (even < p.m && c + i + odd < cols) {  // (a row has room for an even number)
-        *reinterpret_cast<uint32_t*>(to + i * p.ld) = hv;
-        if (u.lo_out) *reinterpret_cast<uint32_t*>(to + (p.m + i) * p.ld) = lv;
-      }
-    }
-  }
-}
-
-// A writing warp's part of a unit: 32 rows by BN / 2 columns.
+// A writing warp's part of a unit: 32 rows by BN / 2 columns, eight columns at a
+// time in a loop that is not unrolled: a launch that writes few tiles finds its
+// code cold, and 32 columns spelled out took 15000 cycles of a product's 26000
+// (1001 x 345) to be fetched.
 template <int MODE, int BN>
 __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const Unit& u, const CUtensorMap* out,
                                            unsigned char* mem, uint32_t rank, uint32_t acc, uint64_t* acc_full,
                                            uint32_t acc_phase) {
   const int lane = threadIdx.x & 31, quarter = threadIdx.x >> 5 & 3, half = (threadIdx.x >> 7) - 1;
-  const int64_t r0 = u.tm * kRows + rank * 128 + quarter * 32, c1 = u.tn * BN + half * (BN / 2);
-  const int64_t cols = MODE == kApply ? p.n : p.m;
-  const bool mirror = u.tn / (kRows / BN) != u.tm;
+  const int m = int(p.m), cols = int(MODE == kApply ? p.n : p.m), z = int(u.b * 2);
+  const int r0 = int(u.tm * kRows + rank * 128 + quarter * 32), r = r0 + lane, c1 = int(u.tn * BN + half * (BN / 2));
+  const bool mirror = MODE != kApply && u.tn / (kRows / BN) != u.tm;
   const float sigma = u.step == 0 ? p.sigma[u.b] : 1.f / kScale;
-  // A's own values for 32 columns from c on, asked for ahead of the product.
-  uint4 oh[4], ol[4];
-  auto ask = [&](int64_t c) {
-    const __half* old = p.A + (u.b * 2 * p.m + r0 + lane) * p.ld + c;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool in = r0 + lane < p.m && c + 8 * i < p.m;  // (a row has room for a multiple of 8)
-      oh[i] = in ? __ldcg(reinterpret_cast<const uint4*>(old) + i) : make_uint4(0, 0, 0, 0);
-      ol[i] = in && u.lo_out ? __ldcg(reinterpret_cast<const uint4*>(old + p.m * p.ld) + i) : make_uint4(0, 0, 0, 0);
+  // A's own values for eight columns from c on, asked for ahead.
+  const __half* old = p.A + (int64_t(z) * m + r) * p.ld;
+  uint4 oh = make_uint4(0, 0, 0, 0), ol = oh;
+  auto ask = [&](int c) {
+    if (r < m && c < m) {  // (a row has room for a multiple of 8)
+      oh = __ldcg(reinterpret_cast<const uint4*>(old + c));
+      if (u.lo_out) ol = __ldcg(reinterpret_cast<const uint4*>(old + int64_t(m) * p.ld + c));
     }
   };
+  if (MODE == kPoly && !p.wait) ask(c1);
   bool ok = wait_or_die(s, acc_full, acc_phase, p);
   // (The product is there, so A is. Only now: eight warps of every CTA that
   // polled for it would hold up those that announce it.)
@@ -642,15 +592,59 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
   if (!__all_sync(0xffffffffu, ok)) return false;
   __syncwarp();
   fence_after_sync();
-  if (MODE == kPoly) ask(c1);
+  if (MODE == kPoly && p.wait) ask(c1);
+  // Below the diagonal lanes are neighbours: two lanes swap values so that each
+  // stores two of them, of every other column. (Through the stage as well,
+  // each store would wait for the one before.)
+  const int odd = lane & 1, even = r - odd;
+  __half* below = (MODE == kGram ? p.A : p.B) + (int64_t(z) * m + c1 + odd) * p.ld + even;
+  auto swap = [&](__half keep, __half give) {
+    const uint32_t g = __shfl_xor_sync(0xffffffffu, uint32_t(__half_as_ushort(give)), 1);
+    const uint32_t k = __half_as_ushort(keep);
+    return odd ? g | k << 16 : k | g << 16;
+  };
 #pragma unroll 1
-  for (int i = 0; i < BN / 2; i += 32) {
-    const int64_t c = c1 + i;
-    if (c >= cols || r0 >= p.m) break;
-    float v[32];
-    tmem_ld32(taddr(acc, quarter * 32, half * (BN / 2) + i), v);
-    emit32<MODE>(p, u, out, mem, r0, c, mirror, sigma, v, oh, ol);
-    if (MODE == kPoly) ask(c + 32);
+  for (int i = 0; i < BN / 2; i += 8) {
+    const int c = c1 + i;
+    if (c >= cols || r0 >= m) break;
+    float v[8];
+    tmem_ld8(taddr(acc, quarter * 32, half * (BN / 2) + i), v);
+    if (MODE == kApply && u.last) {
+      if (r < m) write_final(p, u.b, r, c, sigma / kScale, v, cols - c);
+      continue;
+    }
+    alignas(16) __half h[8], l[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float x;
+      if (MODE == kGram) {
+        x = v[j] * sigma * sigma * kScale;
+      } else if (MODE == kPoly) {
+        const __half *ph = reinterpret_cast<const __half*>(&oh), *pl = reinterpret_cast<const __half*>(&ol);
+        x = p.c * (v[j] / kScale) + p.b * (__half2float(ph[j]) + __half2float(pl[j])) +
+            (c + j == r ? p.a * kScale : 0.f);
+      } else {
+        x = v[j] * sigma;  // (sigma X^) (B^ / kScale), times kScale
+      }
+      split(x, h[j], l[j]);
+    }
+    if (MODE == kPoly) ask(c + 8);
+    if ((i & 31) == 0) stage_free();
+    *reinterpret_cast<uint4*>(mem + out_at(lane, i & 31)) = *reinterpret_cast<const uint4*>(h);
+    *reinterpret_cast<uint4*>(mem + kOutPlane + out_at(lane, i & 31)) = *reinterpret_cast<const uint4*>(l);
+    if ((i & 31) == 24 || c + 8 >= cols) store_stage(out, c & ~31, r0, z, smem_u32(mem), u.lo_out);
+    if (mirror) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const uint32_t hv = swap(odd ? h[j + 1] : h[j], odd ? h[j] : h[j + 1]);
+        const uint32_t lv = swap(odd ? l[j + 1] : l[j], odd ? l[j] : l[j + 1]);
+        if (even < m && c + j + odd < cols) {  // (a row has room for an even number)
+          __half* to = below + int64_t(i + j) * p.ld;
+          *reinterpret_cast<uint32_t*>(to) = hv;
+          if (u.lo_out) *reinterpret_cast<uint32_t*>(to + int64_t(m) * p.ld) = lv;
+        }
+      }
+    }
   }
   return true;
 }
@@ -661,7 +655,8 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
 // thread issues the MMAs for both.
 template <int BN>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMulThreads, 1)
-orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Maps maps) {
+orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Plan<BN> plan,
+                  const __grid_constant__ Maps maps) {
   constexpr int kStages = Shape<BN>::kStages, kStage = Shape<BN>::kStage, kRight = Shape<BN>::kRight;
   extern __shared__ unsigned char raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -669,7 +664,6 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Map
   Barriers* s = reinterpret_cast<Barriers*>(smem + kStages * kStage + kOutBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
-  const Plan<BN> plan(p);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s->full[i], 1);
@@ -695,8 +689,9 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Map
   cluster_barrier();
   fence_after_sync();
   const uint32_t tmem = s->tmem;
-  after_previous();
   let_next_start();
+  // (Each thread that reads or writes global memory waits for the launches
+  // before this one when it comes to that.)
   uint32_t slot = 0, unit_phase = 0, t = kNone;
 
   if (warp == 0 && lane == 0) {
@@ -722,6 +717,7 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Map
     };
     uint32_t next = 0;
     const bool fetches = rank == 0 && p.wait;
+    if (p.wait) after_previous();
     if (fetches && !fetch(&next)) goto done;
     for (;;) {
       if (fetches) t = next;
@@ -732,7 +728,8 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Map
       const CUtensorMap* right = u.mode == kPoly ? &maps.a_right : &maps.x_right[u.step & 1];
       const int row = int(u.tm * kRows + rank * 128), col = int(u.tn * BN + rank * (BN / 2)), z = int(u.b * 2);
       const uint32_t bytes = 2 * (kLeft * (u.lo_left ? 2 : 1) + kRight * (u.lo_right ? 2 : 1));
-      if (p.wait && !wait_operands(s, p, u)) goto done;
+      if (!p.wait) after_previous();
+      else if (!wait_operands(s, p, u)) goto done;
       for (int k = 0; k < u.blocks; ++k) {
         if (fetches && k + 1 == u.blocks && !fetch(&next)) goto done;
         if (!wait_or_die(s, &s->empty[st], phase ^ 1, p)) goto done;
@@ -811,6 +808,7 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Map
       if (t >= p.end) break;
       const Unit u = unit_at<BN>(p, plan, t);
       const uint32_t acc = tmem + buf * BN;
+      after_previous();
       if (u.mode == kGram) ok = write_unit<kGram, BN>(s, p, u, &maps.a_out, mem, rank, acc, &s->acc_full[buf], acc_phase);
       else if (u.mode == kPoly) ok = write_unit<kPoly, BN>(s, p, u, &maps.b_out, mem, rank, acc, &s->acc_full[buf], acc_phase);
       else ok = write_unit<kApply, BN>(s, p, u, &maps.x_out[~u.step & 1], mem, rank, acc, &s->acc_full[buf], acc_phase);
@@ -1104,7 +1102,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
     for (int c = c1; c < n; c += 128) {
       tmem_ld32(taddr(tmem, quarter * 32, c), v);
       if (step + 1 == q.out.steps) {
-        if (row < m) write_final(q.out, b, row, col0 + c, sigma / kScale, v, int(n - c < 32 ? n - c : 32));
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+          if (row < m && c + i < n) write_final(q.out, b, row, col0 + c + i, sigma / kScale, v + i, n - c - i);
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = c + i < n ? v[i] * sigma : 0.f;
@@ -1215,7 +1215,7 @@ cudaError_t launch_units(MulArgs p, const Maps& maps, uint32_t first, uint32_t n
   if (e != cudaSuccess) return e;
   p.first = first;
   p.end = first + n;
-  return launch_next(kernel, dim3(2 * (n < pairs ? n : pairs)), dim3(kMulThreads), kSmem, st, true, p, maps);
+  return launch_next(kernel, dim3(2 * (n < pairs ? n : pairs)), dim3(kMulThreads), kSmem, st, true, p, Plan<BN>(p), maps);
 }
 
 // The units of one product (of all matrices) of one step.
