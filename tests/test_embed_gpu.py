@@ -81,6 +81,29 @@ def test_gradient_of_long_batches_is_reproducible(N, V):
         assert torch.equal(embed_tokens_bwd(ids, d, V, scale=8.0, padding_idx=0), first)
 
 
+@pytest.mark.parametrize("N", [5, 3000, 12000, 20000])
+def test_tables_larger_than_what_is_zeroed_beside_the_sort(N):
+    """164 MB of fp32 gradient, few of whose rows have a token."""
+    V, D = 40000, 1024
+    ids, _, d = _inputs(N, V, D, torch.float32, seed=8, zipf=False)
+    dw = torch.full((V, D), float("nan"), device="cuda")  # (freed: the result may take its place)
+    del dw
+    dw = embed_tokens_bwd(ids, d, V, scale=2.0, padding_idx=7)
+    _check_grad(dw, ids, d, 2.0, pad=7)
+
+
+def test_offsets_past_32_bits():
+    """Outputs and gradients of more than 2^31 elements: rows at the end."""
+    N, V, D = 1100000, 50, 2048
+    ids = torch.randint(0, V - 1, (N,), generator=torch.Generator().manual_seed(9)).cuda()
+    ids[-3:] = V - 1
+    w = torch.randn(V, D, generator=torch.Generator().manual_seed(10)).bfloat16().cuda()
+    y = embed_tokens_fwd(ids, w)
+    assert N * D > 2 ** 31 and torch.equal(y[-2000:], w[ids[-2000:]]) and torch.equal(y[:2000], w[ids[:2000]])
+    dw = embed_tokens_bwd(ids, y, V)
+    assert torch.equal(dw[V - 1], (3 * w[V - 1].float()).bfloat16())
+
+
 @pytest.mark.parametrize("pad", [0, -1, 17])
 def test_padding_row_gets_no_gradient(pad):
     V, D = 40, 48

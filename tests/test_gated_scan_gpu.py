@@ -158,6 +158,27 @@ def test_long_sequences_and_chunk_chain():
     check_status()
 
 
+def test_offsets_past_32_bits():
+    """More than 2^31 elements: the last sequence of a packed row, forward and
+    backward, against the recurrence on its own."""
+    T, D, last = 1100000, 2048, 300
+    assert T * D > 2 ** 31
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    x = torch.randn(1, T, D, generator=gen, device="cuda", dtype=torch.bfloat16)
+    g = torch.full((1, 1, 1), -0.05, device="cuda").expand(1, T, D).to(torch.bfloat16)
+    g[:, T - last] = -math.inf
+    h, final, aux = gated_scan_fwd(x, g, output_final_state=True, return_aux=True)
+    hs, Es, _ = _forward64(x[:, -last:], g[:, -last:], None)
+    _within(h[:, -last:], hs, Es)
+    _within(final, hs[:, -1], Es[:, -1])
+    dx, dg, _ = gated_scan_bwd(x, g, x, aux=aux)
+    tail = [t[:, -last:].contiguous() for t in (x, g)]
+    ref = gated_scan_bwd(*tail, tail[0])
+    for a, b in zip((dx, dg), ref):
+        a, b = a[:, -last:].float(), b.float()  # the same but for where tiles begin
+        assert float((a - b).norm()) <= 2.0 ** -7 * float(b.norm())
+
+
 def test_strides_broadcasts_and_offsets():
     B, T, D = 2, 270, 64
     x, g, dh, init, dfin = _inputs(B, T, D, torch.bfloat16, torch.float32, seed=7)
