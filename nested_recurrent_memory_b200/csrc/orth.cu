@@ -174,12 +174,28 @@ __device__ __forceinline__ void scale_of(double sum, float eps, int* k, float* s
   *sigma = float(1.0 / (norm + double(eps)) / scalbn(1.0, *k));
 }
 
-__device__ __forceinline__ void norm_scale(const PrepArgs& p, int64_t b, int* k, float* sigma) {
-  double s = 0.0;
-  for (int i = threadIdx.x & 31; i < p.parts; i += 32) s += p.part[b * p.parts + i];
+// What a CTA scales an update by, computed by one of its threads (64-bit square
+// roots and divisions by all of them queue up for the few 64-bit units):
+// x * s1 * s2 are the planes' values.
+struct Scale {
+  float s1, s2, sigma;
+  __device__ __forceinline__ void set(double sum, float eps) {
+    int k;
+    scale_of(sum, eps, &k, &sigma);
+    s1 = scalbnf(1.f, k / 2);
+    s2 = scalbnf(1.f, k - k / 2);
+  }
+};
+
+__device__ __forceinline__ void norm_scale(const PrepArgs& p, int64_t b, Scale* shared) {
+  if (threadIdx.x < 32) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < p.parts; i += 32) s += p.part[b * p.parts + i];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  scale_of(s, p.eps, k, sigma);
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (threadIdx.x == 0) shared->set(s, p.eps);
+  }
+  __syncthreads();
 }
 
 // The planes of X_0 / sigma. ROWS: X's rows lie on 16-byte boundaries in the
@@ -194,11 +210,10 @@ __global__ void __launch_bounds__(kPrepThreads) orth_convert_kernel(const __grid
   const int64_t tc = ROWS ? 1 : (p.n + kConvTile - 1) / kConvTile;
   const int64_t tr = ROWS ? (p.m + kConvRows - 1) / kConvRows : (p.m + kConvTile - 1) / kConvTile;
   const int64_t b = blockIdx.x / (tc * tr), q = blockIdx.x % (tc * tr);
-  int k;
-  float sigma;
-  norm_scale(p, b, &k, &sigma);
-  if (q == 0 && threadIdx.x == 0) p.sigma[b] = sigma;
-  const float s1 = scalbnf(1.f, k / 2), s2 = scalbnf(1.f, k - k / 2);
+  __shared__ Scale scale;
+  norm_scale(p, b, &scale);
+  if (q == 0 && threadIdx.x == 0) p.sigma[b] = scale.sigma;
+  const float s1 = scale.s1, s2 = scale.s2;
   __half* hi = p.x + b * 2 * p.m * p.ld;
   __half* lo = hi + p.m * p.ld;
   if constexpr (ROWS) {
@@ -524,15 +539,6 @@ __device__ __forceinline__ void write_final(const MulArgs& p, int64_t b, int64_t
   }
 }
 
-// Eight columns of a warp's 32 lanes of tensor memory.
-__device__ __forceinline__ void tmem_ld8(uint32_t at, float* v) {
-  uint32_t* r = reinterpret_cast<uint32_t*>(v);
-  __syncwarp();
-  tmem_ld8_nowait(at, r);
-  tmem_wait_ld();
-  tmem_regs_after_wait8(r);
-}
-
 // Byte of element (row, col) in a writing warp's stage plane.
 __device__ __forceinline__ uint32_t out_at(int row, int col) {
   return row * 64 + (((col >> 3) ^ (row >> 1 & 3)) << 4) + (col & 7) * 2;
@@ -562,7 +568,7 @@ __device__ __forceinline__ void stage_free() {
   __syncwarp();
 }
 
-// A writing warp's part of a unit: 32 rows by BN / 2 columns, eight columns at a
+// A writing warp's part of a unit: 32 rows by BN / 2 columns, sixteen columns at a
 // time in a loop that is not unrolled: a launch that writes few tiles finds its
 // code cold, and 32 columns spelled out took 15000 cycles of a product's 26000
 // (1001 x 345) to be fetched.
@@ -575,14 +581,16 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
   const int r0 = int(u.tm * kRows + rank * 128 + quarter * 32), r = r0 + lane, c1 = int(u.tn * BN + half * (BN / 2));
   const bool mirror = MODE != kApply && u.tn / (kRows / BN) != u.tm;
   const float sigma = u.step == 0 ? p.sigma[u.b] : 1.f / kScale;
-  // A's own values for eight columns from c on, asked for ahead.
+  // A's own values for sixteen columns from c on, asked for one turn ahead.
   const __half* old = p.A + (int64_t(z) * m + r) * p.ld;
-  uint4 oh = make_uint4(0, 0, 0, 0), ol = oh;
+  uint4 oh[2] = {}, ol[2] = {};
   auto ask = [&](int c) {
-    if (r < m && c < m) {  // (a row has room for a multiple of 8)
-      oh = __ldcg(reinterpret_cast<const uint4*>(old + c));
-      if (u.lo_out) ol = __ldcg(reinterpret_cast<const uint4*>(old + int64_t(m) * p.ld + c));
-    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      if (r < m && c + 8 * k < m) {  // (a row has room for a multiple of 8)
+        oh[k] = __ldcg(reinterpret_cast<const uint4*>(old + c + 8 * k));
+        if (u.lo_out) ol[k] = __ldcg(reinterpret_cast<const uint4*>(old + int64_t(m) * p.ld + c + 8 * k));
+      }
   };
   if (MODE == kPoly && !p.wait) ask(c1);
   bool ok = wait_or_die(s, acc_full, acc_phase, p);
@@ -604,38 +612,48 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
     return odd ? g | k << 16 : k | g << 16;
   };
 #pragma unroll 1
-  for (int i = 0; i < BN / 2; i += 8) {
+  for (int i = 0; i < BN / 2; i += 16) {
     const int c = c1 + i;
     if (c >= cols || r0 >= m) break;
-    float v[8];
-    tmem_ld8(taddr(acc, quarter * 32, half * (BN / 2) + i), v);
+    float v[16];
+    __syncwarp();
+    tmem_ld16(taddr(acc, quarter * 32, half * (BN / 2) + i), v);
+    tmem_regs_after_wait16(reinterpret_cast<uint32_t*>(v));
     if (MODE == kApply && u.last) {
-      if (r < m) write_final(p, u.b, r, c, sigma / kScale, v, cols - c);
+      if (r < m) {
+        write_final(p, u.b, r, c, sigma / kScale, v, cols - c);
+        if (c + 8 < cols) write_final(p, u.b, r, c + 8, sigma / kScale, v + 8, cols - c - 8);
+      }
       continue;
     }
-    alignas(16) __half h[8], l[8];
+    alignas(16) __half h[16], l[16];
+    const uint4 ph[2] = {oh[0], oh[1]}, pl[2] = {ol[0], ol[1]};
+    if (MODE == kPoly) ask(c + 16);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < 16; ++j) {
       float x;
       if (MODE == kGram) {
         x = v[j] * sigma * sigma * kScale;
       } else if (MODE == kPoly) {
-        const __half *ph = reinterpret_cast<const __half*>(&oh), *pl = reinterpret_cast<const __half*>(&ol);
-        x = p.c * (v[j] / kScale) + p.b * (__half2float(ph[j]) + __half2float(pl[j])) +
+        x = p.c * (v[j] / kScale) +
+            p.b * (__half2float(reinterpret_cast<const __half*>(ph)[j]) +
+                   __half2float(reinterpret_cast<const __half*>(pl)[j])) +
             (c + j == r ? p.a * kScale : 0.f);
       } else {
         x = v[j] * sigma;  // (sigma X^) (B^ / kScale), times kScale
       }
       split(x, h[j], l[j]);
     }
-    if (MODE == kPoly) ask(c + 8);
     if ((i & 31) == 0) stage_free();
-    *reinterpret_cast<uint4*>(mem + out_at(lane, i & 31)) = *reinterpret_cast<const uint4*>(h);
-    *reinterpret_cast<uint4*>(mem + kOutPlane + out_at(lane, i & 31)) = *reinterpret_cast<const uint4*>(l);
-    if ((i & 31) == 24 || c + 8 >= cols) store_stage(out, c & ~31, r0, z, smem_u32(mem), u.lo_out);
+#pragma unroll
+    for (int j = 0; j < 16; j += 8) {
+      *reinterpret_cast<uint4*>(mem + out_at(lane, (i & 31) + j)) = *reinterpret_cast<const uint4*>(h + j);
+      *reinterpret_cast<uint4*>(mem + kOutPlane + out_at(lane, (i & 31) + j)) = *reinterpret_cast<const uint4*>(l + j);
+    }
+    if ((i & 31) == 16 || c + 16 >= cols) store_stage(out, c & ~31, r0, z, smem_u32(mem), u.lo_out);
     if (mirror) {
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
+      for (int j = 0; j < 16; j += 2) {
         const uint32_t hv = swap(odd ? h[j + 1] : h[j], odd ? h[j] : h[j + 1]);
         const uint32_t lv = swap(odd ? l[j + 1] : l[j], odd ? l[j] : l[j + 1]);
         if (even < m && c + j + odd < cols) {  // (a row has room for an even number)
@@ -908,6 +926,7 @@ template <int DT>
 __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __grid_constant__ SmallArgs q) {
   extern __shared__ unsigned char raw[];
   __shared__ double red[kSmallThreads / 32], slices[kSmallCtas];
+  __shared__ Scale scale;
   __shared__ uint64_t bar;
   __shared__ uint32_t tmem_at;
   const PrepArgs& p = q.in;
@@ -959,19 +978,22 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   fence_before_sync();
   __syncthreads();
   fence_after_sync();
-  sum = 0.0;
-  for (int w = 0; w < kSmallThreads / 32; ++w) sum += red[w];
   if (ctas > 1) {
+    sum = 0.0;
+    for (int w = 0; w < kSmallThreads / 32; ++w) sum += red[w];
     if (tid < ctas)
       asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(in_cta(smem_u32(&slices[rank]), tid)), "d"(sum) : "memory");
     cluster_barrier();
-    sum = 0.0;
-    for (int i = 0; i < ctas; ++i) sum += slices[i];
   }
-  int k2;
-  float sigma;
-  scale_of(sum, p.eps, &k2, &sigma);
-  const float s1 = scalbnf(1.f, k2 / 2), s2 = scalbnf(1.f, k2 - k2 / 2);
+  if (tid == 0) {
+    const int parts = ctas > 1 ? ctas : kSmallThreads / 32;
+    sum = 0.0;
+    for (int i = 0; i < parts; ++i) sum += ctas > 1 ? slices[i] : red[i];
+    scale.set(sum, p.eps);
+  }
+  __syncthreads();
+  float sigma = scale.sigma;
+  const float s1 = scale.s1, s2 = scale.s2;
   each([&](int r, int c, float x) {
     __half h, l;
     split(x * s1 * s2, h, l);
