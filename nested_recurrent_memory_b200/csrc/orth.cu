@@ -61,9 +61,20 @@ constexpr float kScale = 1024.f;
 // host), so that the planes stay within fp16.
 constexpr double kMaxFactor = 60.0, kMaxSigma = 4.0;
 
-__device__ __forceinline__ void split(float x, __half& hi, __half& lo) {
-  hi = __float2half_rn(x);
-  lo = __float2half_rn(x - __half2float(hi));
+// Neighbouring values as words of the two planes.
+__device__ __forceinline__ void split(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// The sum of both planes.
+__device__ __forceinline__ float2 join(uint32_t hi, uint32_t lo) {
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+  return make_float2(h.x + l.x, h.y + l.y);
 }
 
 // ---------------------------------------------------------------------------
@@ -232,12 +243,12 @@ __global__ void __launch_bounds__(kPrepThreads) orth_convert_kernel(const __grid
       } else {
         unpack16<DT>(__ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.g) + at)), v);
       }
-      alignas(16) __half h[8], l[8];
+      uint32_t h[4], l[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) split(v[i] * s1 * s2, h[i], l[i]);
+      for (int i = 0; i < 4; ++i) split(v[2 * i] * s1 * s2, v[2 * i + 1] * s1 * s2, h[i], l[i]);
       const int64_t o = (r0 + r) * p.ld + c;
-      *reinterpret_cast<uint4*>(hi + o) = *reinterpret_cast<const uint4*>(h);
-      if (p.lo) *reinterpret_cast<uint4*>(lo + o) = *reinterpret_cast<const uint4*>(l);
+      *reinterpret_cast<uint4*>(hi + o) = make_uint4(h[0], h[1], h[2], h[3]);
+      if (p.lo) *reinterpret_cast<uint4*>(lo + o) = make_uint4(l[0], l[1], l[2], l[3]);
     }
   } else {
     const int64_t r0 = q / tc * kConvTile, c0 = q % tc * kConvTile;
@@ -255,12 +266,12 @@ __global__ void __launch_bounds__(kPrepThreads) orth_convert_kernel(const __grid
     for (int e = threadIdx.x; e < kConvTile * kConvTile / 4; e += kPrepThreads) {
       const int r = e / (kConvTile / 4), c = e % (kConvTile / 4) * 4;
       if (r0 + r >= p.m || c0 + c >= p.ld) continue;  // (ld is a multiple of 8)
-      __half h[4], l[4];
+      uint32_t h[2], l[2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) split(tile[r][c + i] * s1 * s2, h[i], l[i]);
+      for (int i = 0; i < 2; ++i) split(tile[r][c + 2 * i] * s1 * s2, tile[r][c + 2 * i + 1] * s1 * s2, h[i], l[i]);
       const int64_t o = (r0 + r) * p.ld + c0 + c;
-      *reinterpret_cast<uint2*>(hi + o) = *reinterpret_cast<const uint2*>(h);
-      if (p.lo) *reinterpret_cast<uint2*>(lo + o) = *reinterpret_cast<const uint2*>(l);
+      *reinterpret_cast<uint2*>(hi + o) = make_uint2(h[0], h[1]);
+      if (p.lo) *reinterpret_cast<uint2*>(lo + o) = make_uint2(l[0], l[1]);
     }
   }
   let_next_start();
@@ -606,10 +617,8 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
   // each store would wait for the one before.)
   const int odd = lane & 1, even = r - odd;
   __half* below = (MODE == kGram ? p.A : p.B) + (int64_t(z) * m + c1 + odd) * p.ld + even;
-  auto swap = [&](__half keep, __half give) {
-    const uint32_t g = __shfl_xor_sync(0xffffffffu, uint32_t(__half_as_ushort(give)), 1);
-    const uint32_t k = __half_as_ushort(keep);
-    return odd ? g | k << 16 : k | g << 16;
+  auto swap = [&](uint32_t w) {
+    return __byte_perm(w, __shfl_xor_sync(0xffffffffu, w, 1), odd ? 0x3276 : 0x5410);
   };
 #pragma unroll 1
   for (int i = 0; i < BN / 2; i += 16) {
@@ -618,7 +627,6 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
     float v[16];
     __syncwarp();
     tmem_ld16(taddr(acc, quarter * 32, half * (BN / 2) + i), v);
-    tmem_regs_after_wait16(reinterpret_cast<uint32_t*>(v));
     if (MODE == kApply && u.last) {
       if (r < m) {
         write_final(p, u.b, r, c, sigma / kScale, v, cols - c);
@@ -626,36 +634,38 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
       }
       continue;
     }
-    alignas(16) __half h[16], l[16];
+    uint32_t h[8], l[8];
     const uint4 ph[2] = {oh[0], oh[1]}, pl[2] = {ol[0], ol[1]};
     if (MODE == kPoly) ask(c + 16);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      float x;
+    for (int j = 0; j < 8; ++j) {
+      float x[2] = {v[2 * j], v[2 * j + 1]};
       if (MODE == kGram) {
-        x = v[j] * sigma * sigma * kScale;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) x[k] = x[k] * sigma * sigma * kScale;
       } else if (MODE == kPoly) {
-        x = p.c * (v[j] / kScale) +
-            p.b * (__half2float(reinterpret_cast<const __half*>(ph)[j]) +
-                   __half2float(reinterpret_cast<const __half*>(pl)[j])) +
-            (c + j == r ? p.a * kScale : 0.f);
+        const float2 o = join(reinterpret_cast<const uint32_t*>(ph)[j], reinterpret_cast<const uint32_t*>(pl)[j]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          x[k] = p.c * (x[k] / kScale) + p.b * (k ? o.y : o.x) + (c + 2 * j + k == r ? p.a * kScale : 0.f);
       } else {
-        x = v[j] * sigma;  // (sigma X^) (B^ / kScale), times kScale
+#pragma unroll
+        for (int k = 0; k < 2; ++k) x[k] *= sigma;  // (sigma X^) (B^ / kScale), times kScale
       }
-      split(x, h[j], l[j]);
+      split(x[0], x[1], h[j], l[j]);
     }
     if ((i & 31) == 0) stage_free();
 #pragma unroll
-    for (int j = 0; j < 16; j += 8) {
-      *reinterpret_cast<uint4*>(mem + out_at(lane, (i & 31) + j)) = *reinterpret_cast<const uint4*>(h + j);
-      *reinterpret_cast<uint4*>(mem + kOutPlane + out_at(lane, (i & 31) + j)) = *reinterpret_cast<const uint4*>(l + j);
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t at = out_at(lane, (i & 31) + 8 * j);
+      *reinterpret_cast<uint4*>(mem + at) = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
+      *reinterpret_cast<uint4*>(mem + kOutPlane + at) = make_uint4(l[4 * j], l[4 * j + 1], l[4 * j + 2], l[4 * j + 3]);
     }
     if ((i & 31) == 16 || c + 16 >= cols) store_stage(out, c & ~31, r0, z, smem_u32(mem), u.lo_out);
     if (mirror) {
 #pragma unroll
       for (int j = 0; j < 16; j += 2) {
-        const uint32_t hv = swap(odd ? h[j + 1] : h[j], odd ? h[j] : h[j + 1]);
-        const uint32_t lv = swap(odd ? l[j + 1] : l[j], odd ? l[j] : l[j + 1]);
+        const uint32_t hv = swap(h[j / 2]), lv = swap(l[j / 2]);
         if (even < m && c + j + odd < cols) {  // (a row has room for an even number)
           __half* to = below + int64_t(i + j) * p.ld;
           *reinterpret_cast<uint32_t*>(to) = hv;
@@ -869,11 +879,11 @@ done:
 // operand with the reduction down the columns. A's slices are summed through
 // distributed shared memory: every CTA adds up a part of A's rows and gives its
 // planes to all. What bounds it is the chain of a step's three
-// products, 2.5 us each, most of it not the MMAs but getting the results out of
-// tensor memory and back as operands.
+// products, 2.3 us each (16 matrices 128 x 128: 40.7 us), most of it not the
+// MMAs but getting the results out of tensor memory and back as operands.
 // ---------------------------------------------------------------------------
 
-constexpr int kSmallM = 128, kSmallThreads = 512, kSmallCtas = 8;
+constexpr int kSmallM = 128, kSmallSlice = 256, kSmallThreads = 512, kSmallCtas = 8;
 constexpr int kSmallMost = 227 * 1024 - 512;  // bytes of shared memory
 
 struct SmallArgs {
@@ -903,7 +913,7 @@ bool fits_small(SmallArgs* q, int64_t m, int64_t n) {
   q->rows = int(m + 15) / 16 * 16;
   for (q->ctas = 1; q->ctas <= kSmallCtas; q->ctas *= 2) {
     const int64_t slice = ((n + q->ctas - 1) / q->ctas + 15) / 16 * 16;
-    if (slice > 256) continue;
+    if (slice > kSmallSlice) continue;
     q->slice = int(slice);
     q->part = ((q->rows + q->ctas - 1) / q->ctas + 7) / 8 * 8;
     if (SmallLayout(*q).total <= kSmallMost) return true;
@@ -920,6 +930,20 @@ __device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
   return a;
+}
+
+// Four neighbours that lie on a multiple of four elements.
+template <int DT>
+__device__ __forceinline__ void load4(const void* p, int64_t at, float* v) {
+  if constexpr (DT == NGDN2_F32) {
+    const float4 t = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at));
+    v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+  } else {
+    const uint2 t = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at));
+    const uint16_t w[4] = {uint16_t(t.x), uint16_t(t.x >> 16), uint16_t(t.y), uint16_t(t.y >> 16)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = load_typed<DT>(w, i);
+  }
 }
 
 template <int DT>
@@ -947,31 +971,37 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   if (warp == 0) tmem_alloc(&tmem_at, 256);
   for (int i = tid * 16; i < 2 * (xp + ap); i += kSmallThreads * 16)
     *reinterpret_cast<uint4*>(mem + i) = make_uint4(0, 0, 0, 0);
-  // The norm, then the planes of the scaled update. Lanes along the dimension
-  // with the smaller stride; a warp takes four rows at a time, their loads in
-  // flight together.
+  // The slice, in registers: four neighbours along the dimension with the
+  // smaller stride are a piece, all pieces' loads are in flight together (16
+  // matrices 128 x 128: 46.2 us where the planes' values were read again after
+  // the norm).
   const bool along_c = p.sc <= p.sr;
   const int outer = along_c ? m : n, inner = along_c ? n : m;
   const int64_t so = along_c ? p.sr : p.sc, si = along_c ? p.sc : p.sr;
   const int64_t origin = b * p.sb + col0 * p.sc;
-  auto each = [&](auto&& f) {
-    constexpr int kWarps = kSmallThreads / 32;
-    for (int i0 = warp; i0 < outer; i0 += 4 * kWarps)
-#pragma unroll 4
-      for (int j = lane; j < inner; j += 32) {
-        float x[4];
+  const int log = inner <= 4 ? 0 : 32 - __clz((inner - 1) / 4);  // pieces a row, as a power of two
+  constexpr int kPieces = kSmallM * kSmallSlice / 4 / kSmallThreads;
+  float x[kPieces][4];
+  const bool quads = si == 1 && (so | origin | inner) % 4 == 0 &&
+                     reinterpret_cast<uintptr_t>(p.g) % (DT == NGDN2_F32 ? 16 : 8) == 0;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          x[u] = i0 + u * kWarps < outer ? load_typed<DT>(p.g, origin + (i0 + u * kWarps) * so + j * si) : 0.f;
+  for (int k = 0; k < kPieces; ++k) {
+    const int e = tid + k * kSmallThreads, i = e >> log, j = (e & ((1 << log) - 1)) * 4;
+    const int64_t at = origin + i * so + j * si;
+    const int left = i < outer ? inner - j : 0;
+    if (quads) {
+      if (left > 0) load4<DT>(p.g, at, x[k]);
+      else x[k][0] = x[k][1] = x[k][2] = x[k][3] = 0.f;
+    } else {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int i = i0 + u * kWarps;
-          if (i < outer) f(along_c ? i : j, along_c ? j : i, x[u]);
-        }
-      }
-  };
+      for (int u = 0; u < 4; ++u) x[k][u] = u < left ? load_typed<DT>(p.g, at + u * si) : 0.f;
+    }
+  }
   double sum = 0.0;
-  each([&](int, int, float x) { sum = fma(double(x), double(x), sum); });
+#pragma unroll
+  for (int k = 0; k < kPieces; ++k)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) sum = fma(double(x[k][u]), double(x[k][u]), sum);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) red[warp] = sum;
@@ -994,12 +1024,28 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   __syncthreads();
   float sigma = scale.sigma;
   const float s1 = scale.s1, s2 = scale.s2;
-  each([&](int r, int c, float x) {
-    __half h, l;
-    split(x * s1 * s2, h, l);
-    *reinterpret_cast<__half*>(mx + block_at(block, r, c)) = h;
-    *reinterpret_cast<__half*>(mx + xp + block_at(block, r, c)) = l;
-  });
+#pragma unroll
+  for (int k = 0; k < kPieces; ++k) {
+    const int e = tid + k * kSmallThreads, i = e >> log, j = (e & ((1 << log) - 1)) * 4;
+    const int left = i < outer ? inner - j : 0;
+    if (left <= 0) continue;
+    uint32_t h[2], l[2];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[k][u] = u < left ? x[k][u] * s1 * s2 : 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) split(x[k][2 * u], x[k][2 * u + 1], h[u], l[u]);
+    if (along_c) {
+      *reinterpret_cast<uint2*>(mx + block_at(block, i, j)) = make_uint2(h[0], h[1]);
+      *reinterpret_cast<uint2*>(mx + xp + block_at(block, i, j)) = make_uint2(l[0], l[1]);
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t at = block_at(block, j + u, i);
+        *reinterpret_cast<uint16_t*>(mx + at) = uint16_t(h[u / 2] >> (u & 1) * 16);
+        *reinterpret_cast<uint16_t*>(mx + xp + at) = uint16_t(l[u / 2] >> (u & 1) * 16);
+      }
+    }
+  }
   const uint32_t tmem = tmem_at;
   const int quarter = warp & 3, c1 = (warp >> 2) * 32, row = quarter * 32 + lane;
   uint32_t phase = 0;
@@ -1036,11 +1082,11 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   };
   // Eight results as planes.
   auto put8 = [&](unsigned char* to, int plane, int c, const float* x) {
-    alignas(16) __half h[8], l[8];
+    uint32_t h[4], l[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) split(x[j], h[j], l[j]);
-    *reinterpret_cast<uint4*>(to + block_at(block, row, c)) = *reinterpret_cast<const uint4*>(h);
-    *reinterpret_cast<uint4*>(to + plane + block_at(block, row, c)) = *reinterpret_cast<const uint4*>(l);
+    for (int j = 0; j < 4; ++j) split(x[2 * j], x[2 * j + 1], h[j], l[j]);
+    *reinterpret_cast<uint4*>(to + block_at(block, row, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(to + plane + block_at(block, row, c)) = make_uint4(l[0], l[1], l[2], l[3]);
   };
 
   const int rows = q.rows, cols = (n + 15) & ~15;
@@ -1085,10 +1131,12 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
           w[0] += f0.x; w[1] += f0.y; w[2] += f0.z; w[3] += f0.w;
           w[4] += f1.x; w[5] += f1.y; w[6] += f1.z; w[7] += f1.w;
         }
-        alignas(16) __half h[8], l[8];
+        uint32_t h[4], l[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) split(8 * g + i < m ? w[i] * sigma * sigma * kScale : 0.f, h[i], l[i]);
-        const uint4 hv = *reinterpret_cast<const uint4*>(h), lv = *reinterpret_cast<const uint4*>(l);
+        for (int i = 0; i < 8; ++i) w[i] = 8 * g + i < m ? w[i] * sigma * sigma * kScale : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) split(w[2 * i], w[2 * i + 1], h[i], l[i]);
+        const uint4 hv = make_uint4(h[0], h[1], h[2], h[3]), lv = make_uint4(l[0], l[1], l[2], l[3]);
         const uint32_t at = aa + block_at(block, r, 8 * g);
         for (int j = 0; j < ctas; ++j) {
           const uint32_t to = in_cta(at, j);
@@ -1108,15 +1156,15 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
 #pragma unroll
       for (int i = 0; i < 32; i += 8) {
         if (row >= rows || c + i >= rows) continue;
-        alignas(16) __half h[8], l[8];
-        *reinterpret_cast<uint4*>(h) = *reinterpret_cast<const uint4*>(ma + block_at(block, row, c + i));
-        *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(ma + ap + block_at(block, row, c + i));
+        const uint4 h = *reinterpret_cast<const uint4*>(ma + block_at(block, row, c + i));
+        const uint4 l = *reinterpret_cast<const uint4*>(ma + ap + block_at(block, row, c + i));
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          v[i + j] = c + i + j < m ? q.out.c * (v[i + j] / kScale) +
-                                         q.out.b * (__half2float(h[j]) + __half2float(l[j])) +
+        for (int j = 0; j < 8; ++j) {
+          const float2 o = join(reinterpret_cast<const uint32_t*>(&h)[j / 2], reinterpret_cast<const uint32_t*>(&l)[j / 2]);
+          v[i + j] = c + i + j < m ? q.out.c * (v[i + j] / kScale) + q.out.b * (j & 1 ? o.y : o.x) +
                                          (c + i + j == row ? q.out.a * kScale : 0.f)
                                    : 0.f;
+        }
         put8(ma, ap, c + i, v + i);
       }
     }
