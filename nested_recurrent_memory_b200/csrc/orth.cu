@@ -18,8 +18,8 @@
 // low-rank spectra; the last two steps would leave 1.8 times).
 //
 // Matrices of up to 128 rows and about 1500 columns (more for fewer rows) take one
-// launch, a CTA or a cluster each (orth_small_kernel). Larger ones: the squared norm (partial sums in 64 bits), the conversion to
-// planes, and the products of all steps: A = X X^T, B = a I + b A
+// launch, a CTA or a cluster each (orth_small_kernel). Larger ones: the squared
+// norm (partial sums in 64 bits), the conversion to planes, and the products of all steps: A = X X^T, B = a I + b A
 // + c A A (both symmetric: the tiles on and above the diagonal, written twice)
 // and X' = B X, which reads X as it lies, rows along the reduction. The
 // products are cut into tiles, handed out by a counter. For large batches one
@@ -28,14 +28,14 @@
 // matrix's next product starts while others' last one still runs. Every wait
 // is bounded.
 //
-// A pair of CTAs computes tiles of 256 rows by 256 or 128 columns (tcgen05,
+// A pair of CTAs computes tiles of 256 rows by 256, 128 or 64 columns (tcgen05,
 // cta_group::2; each CTA holds its 128 rows of the left operand and half of
 // the right one), fed by a thread that issues TMA loads of 64-deep stages
 // ahead, with two accumulators in tensor memory so that one tile's results are
 // written while the next is multiplied. The pair tile halves what each
 // multiprocessor must read: 64 KB a stage for 12 MMAs of 256 columns. The
-// narrower tile reads more for each MMA, but few tiles finish sooner. Either
-// sums in the same order, so a matrix has the same bits in any batch.
+// narrower tiles read more for each MMA, but few tiles finish sooner. All
+// sum in the same order, so a matrix has the same bits in any batch.
 
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -286,13 +286,17 @@ enum { kGram = 0, kPoly = 1, kApply = 2 };  // A = X X^T; B = a I + b A + c A A;
 constexpr int kRows = 256;            // of a pair's tile
 constexpr int kDepth = 64;            // reduction elements of a stage
 constexpr int kLeft = 128 * kDepth * 2;  // bytes of the left operand's plane in one CTA, a stage
-constexpr int kBox = 64 * kDepth * 2;    // of 64 of the right operand's columns
 
 // Tiles of BN columns: a stage holds both operands' planes; as many stages as
-// fit beside the results' stage.
+// fit beside the results' stage (four at most). The right operand comes in boxes
+// of kBoxCols of its columns; where it lies rows along the reduction a box has
+// 64, so a tile of 64 columns, half of them in each CTA, is for A and B only.
 template <int BN>
 struct Shape {
-  static constexpr int kRight = BN / 128 * kBox;
+  static constexpr int kBoxCols = BN / 2 < 64 ? BN / 2 : 64, kBoxes = BN / 2 / kBoxCols;
+  static constexpr int kBox = kBoxCols * kDepth * 2;
+  static constexpr int kRight = kBoxes * kBox;
+  static constexpr bool kApplies = kBoxCols == 64;
   static constexpr int kStage = 2 * (kLeft + kRight);
   static constexpr int kStages = BN == 256 ? 3 : 4;
 };
@@ -305,6 +309,7 @@ constexpr int kOutPlane = 32 * 64, kOutBytes = kWriters * 2 * kOutPlane;
 constexpr int kSmem = 3 * 65536 + kOutBytes + 1024 + 256;
 static_assert(Shape<256>::kStages * Shape<256>::kStage == 3 * 65536, "");
 static_assert(Shape<128>::kStages * Shape<128>::kStage == 3 * 65536, "");
+static_assert(Shape<64>::kStages * Shape<64>::kStage <= 3 * 65536, "");
 
 struct MulArgs {
   int64_t batch, m, n;   // X is m x n
@@ -767,10 +772,11 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
           if (pl == 0 || u.lo_left) load_box(at + pl * kLeft, left, k * kDepth, row, z + pl, bar);
           if (pl == 0 || u.lo_right)
 #pragma unroll
-            for (int i = 0; i < BN / 128; ++i) {
-              const uint32_t to = at + 2 * kLeft + pl * kRight + i * kBox;
-              if (u.mode == kApply) load_box(to, right, col + 64 * i, k * kDepth, z + pl, bar);
-              else load_box(to, right, k * kDepth, col + 64 * i, z + pl, bar);
+            for (int i = 0; i < Shape<BN>::kBoxes; ++i) {
+              const uint32_t to = at + 2 * kLeft + pl * kRight + i * Shape<BN>::kBox;
+              const int c = col + i * Shape<BN>::kBoxCols;
+              if (Shape<BN>::kApplies && u.mode == kApply) load_box(to, right, c, k * kDepth, z + pl, bar);
+              else load_box(to, right, k * kDepth, c, z + pl, bar);
             }
         }
         if (++st == kStages) {
@@ -793,10 +799,10 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
       if (!next_unit(s, p, &slot, &unit_phase, &t)) goto done;
       if (t >= p.end) break;
       const Unit u = unit_at<BN>(p, plan, t);
-      const bool down = u.mode == kApply;
+      const bool down = Shape<BN>::kApplies && u.mode == kApply;
       const uint32_t idesc = idesc_f16(kRows, BN, false, false, down);
       const uint64_t left_desc = desc_sw128(base, 1024), right_step = (down ? 2048 : 32) >> 4;
-      const uint64_t right_desc = down ? desc_sw128_mn(base + 2 * kLeft, kBox) : desc_sw128(base + 2 * kLeft, 1024);
+      const uint64_t right_desc = down ? desc_sw128_mn(base + 2 * kLeft, Shape<BN>::kBox) : desc_sw128(base + 2 * kLeft, 1024);
       if (!wait_or_die(s, &s->acc_empty[buf], acc_phase ^ 1, p)) goto done;
       const uint32_t d = tmem + buf * BN;
       for (int k = 0; k < u.blocks; ++k) {
@@ -839,7 +845,8 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
       after_previous();
       if (u.mode == kGram) ok = write_unit<kGram, BN>(s, p, u, &maps.a_out, mem, rank, acc, &s->acc_full[buf], acc_phase);
       else if (u.mode == kPoly) ok = write_unit<kPoly, BN>(s, p, u, &maps.b_out, mem, rank, acc, &s->acc_full[buf], acc_phase);
-      else ok = write_unit<kApply, BN>(s, p, u, &maps.x_out[~u.step & 1], mem, rank, acc, &s->acc_full[buf], acc_phase);
+      else if constexpr (Shape<BN>::kApplies)
+        ok = write_unit<kApply, BN>(s, p, u, &maps.x_out[~u.step & 1], mem, rank, acc, &s->acc_full[buf], acc_phase);
       if (!__all_sync(0xffffffffu, ok)) goto done;
       fence_before_sync();
       __syncwarp();
@@ -1296,34 +1303,40 @@ cudaError_t launch_product(const MulArgs& p, const Maps& maps, int step, int mod
   return launch_units<BN>(p, maps, step * plan.per_step + mode * sym, mode == kApply ? app : sym, pairs, st);
 }
 
-// Wide or narrow tiles go by the rounds that the pairs of CTAs take: a narrow
-// tile takes 0.6 of a wide one's time. An element's sum has the same order
-// either way.
-bool narrow_is_faster(double narrow, double wide) { return 0.6 * narrow < wide; }
+// The tiles' width goes by the rounds that the pairs of CTAs take: one of 128
+// columns takes 0.6 of the time of one of 256, one of 64 0.5 (all steps where A
+// and B take one round either way, 64 columns against 128: 1001 x 345 167.0 and
+// 179.4 us, 1024 x 2816 321.2 and 346.0, 8 x 256 x 512 126.1 and 136.2). An
+// element's sum has the same order in all.
+constexpr double kTime128 = 0.6, kTime64 = 0.5;
 
 // One launch for all steps where a product of all matrices fills the pairs more
 // than once, so that there is always a unit whose operands are ready; otherwise
 // a launch for each product, whose start costs less than the signals between
 // units (us, one launch against one a product: 12 x 1024 x 2816 1394 and 1556, 12 x
-// 1024 x 1024 818 and 877; 1024 x 2816 423 and 394, 128 x 1024 195 and 162).
-cudaError_t launch_steps(MulArgs p, const Maps& maps, uint32_t pairs, cudaStream_t st) {
+// 1024 x 1024 818 and 877; 1024 x 2816 423 and 394).
+cudaError_t launch_steps(MulArgs p, const Maps& maps, const Maps& maps64, uint32_t pairs, cudaStream_t st) {
   const Plan<256> wide(p);
   const Plan<128> narrow(p);
+  const Plan<64> thin(p);
   auto rounds = [&](uint32_t tiles) { return double((uint64_t(p.batch) * tiles + pairs - 1) / pairs); };
   p.wait = p.batch > 1 && p.batch * wide.sym > pairs;
   if (p.wait) {
     auto all = [&](uint32_t sym, uint32_t app) { return rounds(sym) * (p.n + p.m) + rounds(app) * p.m; };
-    return narrow_is_faster(all(narrow.sym, narrow.app), all(wide.sym, wide.app))
+    return kTime128 * all(narrow.sym, narrow.app) < all(wide.sym, wide.app)
                ? launch_units<128>(p, maps, 0, narrow.total, pairs, st)
                : launch_units<256>(p, maps, 0, wide.total, pairs, st);
   }
+  auto product = [&](int step, int mode) {
+    const bool app = mode == kApply;
+    const double t256 = rounds(app ? wide.app : wide.sym), t128 = kTime128 * rounds(app ? narrow.app : narrow.sym);
+    if (!app && kTime64 * rounds(thin.sym) < fmin(t128, t256)) return launch_product<64>(p, maps64, step, mode, pairs, st);
+    return t128 < t256 ? launch_product<128>(p, maps, step, mode, pairs, st)
+                       : launch_product<256>(p, maps, step, mode, pairs, st);
+  };
   cudaError_t e = cudaSuccess;
   for (int step = 0; step < p.steps; ++step)
-    for (int mode = kGram; mode <= kApply && e == cudaSuccess; ++mode)
-      e = (mode == kApply ? narrow_is_faster(rounds(narrow.app), rounds(wide.app))
-                          : narrow_is_faster(rounds(narrow.sym), rounds(wide.sym)))
-              ? launch_product<128>(p, maps, step, mode, pairs, st)
-              : launch_product<256>(p, maps, step, mode, pairs, st);
+    for (int mode = kGram; mode <= kApply && e == cudaSuccess; ++mode) e = product(step, mode);
   return e;
 }
 
@@ -1438,7 +1451,8 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
                     a->out_dtype, int(tall));
     return e == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
   }
-  // Left operands (128 rows a box), right ones (64), results (32 x 32).
+  // Left operands (128 rows a box), right ones (64, or 32 for thin tiles),
+  // results (32 x 32).
   Maps maps;
   const auto of_x = [&](CUtensorMap* map, const __half* q, int box, int width) {
     return make_map(map, q, a->batch, L.m, L.n, L.ldx, box, width);
@@ -1447,12 +1461,16 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
     return make_map(map, q, a->batch, L.m, L.m, L.lda, box, width);
   };
   for (int i = 0; i < 2; ++i)
-    if (!of_x(&maps.x_left[i], i ? y : x, 128, kDepth) || !of_x(&maps.x_right[i], i ? y : x, 64, kDepth) ||
-        !of_x(&maps.x_out[i], i ? y : x, 32, 32))
+    if (!of_x(&maps.x_left[i], i ? y : x, 128, kDepth) ||
+        !of_x(&maps.x_right[i], i ? y : x, Shape<128>::kBoxCols, kDepth) || !of_x(&maps.x_out[i], i ? y : x, 32, 32))
       return NGDN2_ERR_CUDA;
-  if (!of_a(&maps.a_left, A, 128, kDepth) || !of_a(&maps.a_right, A, 64, kDepth) || !of_a(&maps.a_out, A, 32, 32) ||
-      !of_a(&maps.b_left, B, 128, kDepth) || !of_a(&maps.b_out, B, 32, 32))
+  if (!of_a(&maps.a_left, A, 128, kDepth) || !of_a(&maps.a_right, A, Shape<128>::kBoxCols, kDepth) ||
+      !of_a(&maps.a_out, A, 32, 32) || !of_a(&maps.b_left, B, 128, kDepth) || !of_a(&maps.b_out, B, 32, 32))
     return NGDN2_ERR_CUDA;
+  Maps maps64 = maps;
+  for (int i = 0; i < 2; ++i)
+    if (!of_x(&maps64.x_right[i], i ? y : x, Shape<64>::kBoxCols, kDepth)) return NGDN2_ERR_CUDA;
+  if (!of_a(&maps64.a_right, A, Shape<64>::kBoxCols, kDepth)) return NGDN2_ERR_CUDA;
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
@@ -1475,9 +1493,9 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
   p.transposed = tall;
   p.sync = reinterpret_cast<Sync*>(pr.sync);
   p.status = a->status;
-  if (double(a->batch) * a->steps * (double(L.m) / 128 + 1) * (double(L.n + L.m) / 128 + 2) >= double(1u << 31))
+  if (double(a->batch) * a->steps * (double(L.m) / 128 + 1) * (double(L.n + L.m) / 64 + 2) >= double(1u << 31))
     return NGDN2_ERR_SHAPE;  // units are counted in 32 bits
-  e = launch_steps(p, maps, uint32_t(sms / 2), st);
+  e = launch_steps(p, maps, maps64, uint32_t(sms / 2), st);
   return e == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
 }
 
