@@ -289,14 +289,12 @@ constexpr int kLeft = 128 * kDepth * 2;  // bytes of the left operand's plane in
 
 // Tiles of BN columns: a stage holds both operands' planes; as many stages as
 // fit beside the results' stage (four at most). The right operand comes in boxes
-// of kBoxCols of its columns; where it lies rows along the reduction a box has
-// 64, so a tile of 64 columns, half of them in each CTA, is for A and B only.
+// of kBoxCols of its columns.
 template <int BN>
 struct Shape {
   static constexpr int kBoxCols = BN / 2 < 64 ? BN / 2 : 64, kBoxes = BN / 2 / kBoxCols;
   static constexpr int kBox = kBoxCols * kDepth * 2;
   static constexpr int kRight = kBoxes * kBox;
-  static constexpr bool kApplies = kBoxCols == 64;
   static constexpr int kStage = 2 * (kLeft + kRight);
   static constexpr int kStages = BN == 256 ? 3 : 4;
 };
@@ -443,11 +441,14 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
       "h"(static_cast<uint16_t>(3))
       : "memory");
 }
-// Descriptor of a right operand that lies rows along the reduction: blocks of 64
-// columns (rows of 128 bytes, 128-byte swizzle) ``block`` bytes apart, 8-row groups
-// of 1 KB.
-__device__ __forceinline__ uint64_t desc_sw128_mn(uint32_t saddr, uint32_t block) {
-  return (desc_sw128(saddr, 1024) & ~(uint64_t(0x3FFF) << 16)) | uint64_t(block >> 4) << 16;
+// Descriptor of a right operand that lies rows along the reduction: blocks of
+// COLS columns (64: rows of 128 bytes, 128-byte swizzle; 32: half of both)
+// ``block`` bytes apart, in groups of 8 rows.
+template <int COLS = 64>
+__device__ __forceinline__ uint64_t desc_down(uint32_t saddr, uint32_t block) {
+  static_assert(COLS == 64 || COLS == 32, "");
+  const uint64_t d = desc_sw128(saddr, COLS * 16) & ~(uint64_t(0x3FFF) << 16) & ~(uint64_t(7) << 61);
+  return d | uint64_t(block >> 4) << 16 | uint64_t(COLS == 64 ? 2 : 4) << 61;
 }
 
 constexpr uint32_t kNone = 0xffffffffu;
@@ -686,7 +687,10 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
 // next is multiplied. In each CTA a thread issues the loads (the first CTA's
 // also fetches unit numbers for both) and eight warps write; in the first CTA a
 // thread issues the MMAs for both.
-template <int BN>
+// SYM, APP: whether the launch has units of A or B, and of X' (a kernel for all
+// takes longer to start: all steps of 512 x 4096 take 298 us with it, 291 with
+// one for each).
+template <int BN, bool SYM, bool APP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMulThreads, 1)
 orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Plan<BN> plan,
                   const __grid_constant__ Maps maps) {
@@ -775,7 +779,7 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
             for (int i = 0; i < Shape<BN>::kBoxes; ++i) {
               const uint32_t to = at + 2 * kLeft + pl * kRight + i * Shape<BN>::kBox;
               const int c = col + i * Shape<BN>::kBoxCols;
-              if (Shape<BN>::kApplies && u.mode == kApply) load_box(to, right, c, k * kDepth, z + pl, bar);
+              if (APP && (!SYM || u.mode == kApply)) load_box(to, right, c, k * kDepth, z + pl, bar);
               else load_box(to, right, k * kDepth, c, z + pl, bar);
             }
         }
@@ -799,10 +803,11 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
       if (!next_unit(s, p, &slot, &unit_phase, &t)) goto done;
       if (t >= p.end) break;
       const Unit u = unit_at<BN>(p, plan, t);
-      const bool down = Shape<BN>::kApplies && u.mode == kApply;
+      const bool down = APP && (!SYM || u.mode == kApply);
       const uint32_t idesc = idesc_f16(kRows, BN, false, false, down);
-      const uint64_t left_desc = desc_sw128(base, 1024), right_step = (down ? 2048 : 32) >> 4;
-      const uint64_t right_desc = down ? desc_sw128_mn(base + 2 * kLeft, Shape<BN>::kBox) : desc_sw128(base + 2 * kLeft, 1024);
+      const uint64_t left_desc = desc_sw128(base, 1024), right_step = (down ? Shape<BN>::kBoxCols * 32 : 32) >> 4;
+      const uint64_t right_desc = down ? desc_down<Shape<BN>::kBoxCols>(base + 2 * kLeft, Shape<BN>::kBox)
+                                       : desc_sw128(base + 2 * kLeft, 1024);
       if (!wait_or_die(s, &s->acc_empty[buf], acc_phase ^ 1, p)) goto done;
       const uint32_t d = tmem + buf * BN;
       for (int k = 0; k < u.blocks; ++k) {
@@ -843,10 +848,14 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
       const Unit u = unit_at<BN>(p, plan, t);
       const uint32_t acc = tmem + buf * BN;
       after_previous();
-      if (u.mode == kGram) ok = write_unit<kGram, BN>(s, p, u, &maps.a_out, mem, rank, acc, &s->acc_full[buf], acc_phase);
-      else if (u.mode == kPoly) ok = write_unit<kPoly, BN>(s, p, u, &maps.b_out, mem, rank, acc, &s->acc_full[buf], acc_phase);
-      else if constexpr (Shape<BN>::kApplies)
-        ok = write_unit<kApply, BN>(s, p, u, &maps.x_out[~u.step & 1], mem, rank, acc, &s->acc_full[buf], acc_phase);
+      auto write = [&](auto mode, const CUtensorMap* out) {
+        return write_unit<decltype(mode)::value, BN>(s, p, u, out, mem, rank, acc, &s->acc_full[buf], acc_phase);
+      };
+      if constexpr (SYM)
+        if (u.mode == kGram) ok = write(std::integral_constant<int, kGram>{}, &maps.a_out);
+        else if (u.mode == kPoly) ok = write(std::integral_constant<int, kPoly>{}, &maps.b_out);
+      if constexpr (APP)
+        if (u.mode == kApply) ok = write(std::integral_constant<int, kApply>{}, &maps.x_out[~u.step & 1]);
       if (!__all_sync(0xffffffffu, ok)) goto done;
       fence_before_sync();
       __syncwarp();
@@ -1071,7 +1080,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
       const uint32_t idesc = idesc_f16(128, cols, false, false, down);
       for (int kk = 0; kk < depth / 16; ++kk) {
         const uint64_t dl = desc_sw128(L + (kk >> 2) * block + (kk & 3) * 32, 1024);
-        const uint64_t dr = down ? desc_sw128_mn(R + kk * 2048, block)
+        const uint64_t dr = down ? desc_down(R + kk * 2048, block)
                                  : desc_sw128(R + (kk >> 2) * block + (kk & 3) * 32, 1024);
         mma_f16(tmem, dl, dr, idesc, kk > 0);
         if (full) {
@@ -1285,9 +1294,9 @@ bool make_map(CUtensorMap* map, const __half* p, int64_t batch, int64_t rows, in
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN>
+template <int BN, bool SYM, bool APP>
 cudaError_t launch_units(MulArgs p, const Maps& maps, uint32_t first, uint32_t n, uint32_t pairs, cudaStream_t st) {
-  auto* kernel = orth_steps_kernel<BN>;
+  auto* kernel = orth_steps_kernel<BN, SYM, APP>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return e;
   p.first = first;
@@ -1300,14 +1309,16 @@ template <int BN>
 cudaError_t launch_product(const MulArgs& p, const Maps& maps, int step, int mode, uint32_t pairs, cudaStream_t st) {
   const Plan<BN> plan(p);
   const uint32_t sym = uint32_t(p.batch) * plan.sym, app = uint32_t(p.batch) * plan.app;
-  return launch_units<BN>(p, maps, step * plan.per_step + mode * sym, mode == kApply ? app : sym, pairs, st);
+  const uint32_t first = step * plan.per_step + mode * sym;
+  return mode == kApply ? launch_units<BN, false, true>(p, maps, first, app, pairs, st)
+                        : launch_units<BN, true, false>(p, maps, first, sym, pairs, st);
 }
 
 // The tiles' width goes by the rounds that the pairs of CTAs take: one of 128
-// columns takes 0.6 of the time of one of 256, one of 64 0.5 (all steps where A
-// and B take one round either way, 64 columns against 128: 1001 x 345 167.0 and
-// 179.4 us, 1024 x 2816 321.2 and 346.0, 8 x 256 x 512 126.1 and 136.2). An
-// element's sum has the same order in all.
+// columns takes 0.6 of the time of one of 256, one of 64 0.5 (all steps, one round
+// either way, 64 columns against 128: 1001 x 345 159.5 and 179.4 us, 256 x 512
+// 112.4 and 130.6, 8 x 256 x 512 123.2 and 136.2). An element's sum has the same
+// order in all.
 constexpr double kTime128 = 0.6, kTime64 = 0.5;
 
 // One launch for all steps where a product of all matrices fills the pairs more
@@ -1315,7 +1326,8 @@ constexpr double kTime128 = 0.6, kTime64 = 0.5;
 // a launch for each product, whose start costs less than the signals between
 // units (us, one launch against one a product: 12 x 1024 x 2816 1394 and 1556, 12 x
 // 1024 x 1024 818 and 877; 1024 x 2816 423 and 394).
-cudaError_t launch_steps(MulArgs p, const Maps& maps, const Maps& maps64, uint32_t pairs, cudaStream_t st) {
+cudaError_t launch_steps(MulArgs p, const Maps& maps, const Maps& thin_rows, const Maps& thin_down, uint32_t pairs,
+                         cudaStream_t st) {
   const Plan<256> wide(p);
   const Plan<128> narrow(p);
   const Plan<64> thin(p);
@@ -1324,13 +1336,14 @@ cudaError_t launch_steps(MulArgs p, const Maps& maps, const Maps& maps64, uint32
   if (p.wait) {
     auto all = [&](uint32_t sym, uint32_t app) { return rounds(sym) * (p.n + p.m) + rounds(app) * p.m; };
     return kTime128 * all(narrow.sym, narrow.app) < all(wide.sym, wide.app)
-               ? launch_units<128>(p, maps, 0, narrow.total, pairs, st)
-               : launch_units<256>(p, maps, 0, wide.total, pairs, st);
+               ? launch_units<128, true, true>(p, maps, 0, narrow.total, pairs, st)
+               : launch_units<256, true, true>(p, maps, 0, wide.total, pairs, st);
   }
   auto product = [&](int step, int mode) {
     const bool app = mode == kApply;
     const double t256 = rounds(app ? wide.app : wide.sym), t128 = kTime128 * rounds(app ? narrow.app : narrow.sym);
-    if (!app && kTime64 * rounds(thin.sym) < fmin(t128, t256)) return launch_product<64>(p, maps64, step, mode, pairs, st);
+    if (kTime64 * rounds(app ? thin.app : thin.sym) < fmin(t128, t256))
+      return launch_product<64>(p, app ? thin_down : thin_rows, step, mode, pairs, st);
     return t128 < t256 ? launch_product<128>(p, maps, step, mode, pairs, st)
                        : launch_product<256>(p, maps, step, mode, pairs, st);
   };
@@ -1467,10 +1480,12 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
   if (!of_a(&maps.a_left, A, 128, kDepth) || !of_a(&maps.a_right, A, Shape<128>::kBoxCols, kDepth) ||
       !of_a(&maps.a_out, A, 32, 32) || !of_a(&maps.b_left, B, 128, kDepth) || !of_a(&maps.b_out, B, 32, 32))
     return NGDN2_ERR_CUDA;
-  Maps maps64 = maps;
+  Maps thin_rows = maps, thin_down = maps;  // (for tiles of 64 columns, 32 in each CTA)
   for (int i = 0; i < 2; ++i)
-    if (!of_x(&maps64.x_right[i], i ? y : x, Shape<64>::kBoxCols, kDepth)) return NGDN2_ERR_CUDA;
-  if (!of_a(&maps64.a_right, A, Shape<64>::kBoxCols, kDepth)) return NGDN2_ERR_CUDA;
+    if (!of_x(&thin_rows.x_right[i], i ? y : x, Shape<64>::kBoxCols, kDepth) ||
+        !of_x(&thin_down.x_right[i], i ? y : x, kDepth, Shape<64>::kBoxCols))
+      return NGDN2_ERR_CUDA;
+  if (!of_a(&thin_rows.a_right, A, Shape<64>::kBoxCols, kDepth)) return NGDN2_ERR_CUDA;
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
@@ -1495,7 +1510,7 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
   p.status = a->status;
   if (double(a->batch) * a->steps * (double(L.m) / 128 + 1) * (double(L.n + L.m) / 64 + 2) >= double(1u << 31))
     return NGDN2_ERR_SHAPE;  // units are counted in 32 bits
-  e = launch_steps(p, maps, maps64, uint32_t(sms / 2), st);
+  e = launch_steps(p, maps, thin_rows, thin_down, uint32_t(sms / 2), st);
   return e == cudaSuccess ? NGDN2_OK : NGDN2_ERR_CUDA;
 }
 
