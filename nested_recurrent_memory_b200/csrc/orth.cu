@@ -11,11 +11,10 @@
 // hi hi + hi lo + lo hi, summed in fp32 in tensor memory: the accuracy of fp32
 // arithmetic (about 1e-6 .. 1e-5 on the same updates) at a third of the
 // tensor cores' rate. A 16-bit update fits its hi plane, so the first step
-// needs one product for A and two for X. The last step's roundings are not
-// stretched any more: where the result is bf16 (unit 2^-8) it uses the hi
-// planes alone (2^-11), which leaves the result's error within 1.13 times that
-// of rounding the exact one to bf16 (simulated on full-rank, decaying and
-// low-rank spectra; the last two steps would leave 1.8 times).
+// needs one product for A and two for X. That holds for the last step too,
+// whatever the result's type: a 16-bit result is the fp32 one rounded once.
+// (Its hi planes alone would take 13/15 of the MMAs, and change bf16 results
+// by as much as their rounding does.)
 //
 // Matrices of up to 128 rows and about 1500 columns (more for fewer rows) take one
 // launch, a CTA or a cluster each (orth_small_kernel). Larger ones: the squared
@@ -361,7 +360,6 @@ struct Unit {
   int64_t b, tm, tn;
   int blocks;           // of the reduction
   bool lo_left, lo_right;
-  bool lo_out;          // whether the result (and, kPoly, A) has a lo plane
   bool last;
   uint64_t need;        // of the matrix's finished warps' units, before this one may start
 };
@@ -391,12 +389,10 @@ __device__ __forceinline__ Unit unit_at(const MulArgs& p, const Plan<BN>& plan, 
     u.tn = row * (kRows / BN) + q;
   }
   u.last = u.step + 1 == p.steps;
-  const bool full = !(u.last && p.out_dtype == NGDN2_BF16);
-  const bool x_lo = full && (u.step > 0 || p.x_lo);
+  const bool x_lo = u.step > 0 || p.x_lo;
   u.blocks = int(((u.mode == kGram ? p.n : p.m) + kDepth - 1) / kDepth);
-  u.lo_left = u.mode == kGram ? x_lo : full;
-  u.lo_right = u.mode == kPoly ? full : x_lo;
-  u.lo_out = u.mode == kApply || full;
+  u.lo_left = u.mode != kGram || x_lo;
+  u.lo_right = u.mode == kPoly || x_lo;
   u.need = (uint64_t(u.step) * (2 * plan.sym + plan.app) + u.mode * plan.sym) * (2 * kWriters);
   return u;
 }
@@ -569,12 +565,12 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, int c0, int c1
 }
 
 // The stage's planes to the matrix, from row r0 and column c0 on.
-__device__ __forceinline__ void store_stage(const CUtensorMap* map, int c0, int r0, int z, uint32_t stage, bool lo) {
+__device__ __forceinline__ void store_stage(const CUtensorMap* map, int c0, int r0, int z, uint32_t stage) {
   fence_proxy_async();
   __syncwarp();
   if ((threadIdx.x & 31) == 0) {
     store_box(map, c0, r0, z, stage);
-    if (lo) store_box(map, c0, r0, z + 1, stage + kOutPlane);
+    store_box(map, c0, r0, z + 1, stage + kOutPlane);
     bulk_commit();
   }
 }
@@ -606,7 +602,7 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
     for (int k = 0; k < 2; ++k)
       if (r < m && c + 8 * k < m) {  // (a row has room for a multiple of 8)
         oh[k] = __ldcg(reinterpret_cast<const uint4*>(old + c + 8 * k));
-        if (u.lo_out) ol[k] = __ldcg(reinterpret_cast<const uint4*>(old + int64_t(m) * p.ld + c + 8 * k));
+        ol[k] = __ldcg(reinterpret_cast<const uint4*>(old + int64_t(m) * p.ld + c + 8 * k));
       }
   };
   if (MODE == kPoly && !p.wait) ask(c1);
@@ -667,7 +663,7 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
       *reinterpret_cast<uint4*>(mem + at) = make_uint4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
       *reinterpret_cast<uint4*>(mem + kOutPlane + at) = make_uint4(l[4 * j], l[4 * j + 1], l[4 * j + 2], l[4 * j + 3]);
     }
-    if ((i & 31) == 16 || c + 16 >= cols) store_stage(out, c & ~31, r0, z, smem_u32(mem), u.lo_out);
+    if ((i & 31) == 16 || c + 16 >= cols) store_stage(out, c & ~31, r0, z, smem_u32(mem));
     if (mirror) {
 #pragma unroll
       for (int j = 0; j < 16; j += 2) {
@@ -675,7 +671,7 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
         if (even < m && c + j + odd < cols) {  // (a row has room for an even number)
           __half* to = below + int64_t(i + j) * p.ld;
           *reinterpret_cast<uint32_t*>(to) = hv;
-          if (u.lo_out) *reinterpret_cast<uint32_t*>(to + int64_t(m) * p.ld) = lv;
+          *reinterpret_cast<uint32_t*>(to + int64_t(m) * p.ld) = lv;
         }
       }
     }
@@ -1070,7 +1066,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   // D[128 x cols] = L R, reduction over ``depth`` (multiples of 16). After a wait
   // that gave up nothing is multiplied any more, but the cluster goes on
   // together.
-  auto product = [&](uint32_t L, int lp, uint32_t R, int rp, int depth, int cols, bool down, bool full) {
+  auto product = [&](uint32_t L, int lp, uint32_t R, int rp, int depth, int cols, bool down) {
     fence_proxy_async();
     fence_before_sync();
     __syncthreads();
@@ -1083,10 +1079,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
         const uint64_t dr = down ? desc_down(R + kk * 2048, block)
                                  : desc_sw128(R + (kk >> 2) * block + (kk & 3) * 32, 1024);
         mma_f16(tmem, dl, dr, idesc, kk > 0);
-        if (full) {
-          mma_f16(tmem, dl, dr + (rp >> 4), idesc, 1);
-          mma_f16(tmem, dl + (lp >> 4), dr, idesc, 1);
-        }
+        mma_f16(tmem, dl, dr + (rp >> 4), idesc, 1);
+        mma_f16(tmem, dl + (lp >> 4), dr, idesc, 1);
       }
       mma_commit(&bar);
     }
@@ -1107,9 +1101,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
 
   const int rows = q.rows, cols = (n + 15) & ~15;
   for (int step = 0; step < q.out.steps; ++step, sigma = 1.f / kScale) {
-    const bool full = !(step + 1 == q.out.steps && q.out.out_dtype == NGDN2_BF16);
     float v[32];
-    product(ax, xp, ax, xp, cols, rows, false, full);
+    product(ax, xp, ax, xp, cols, rows, false);
     if (ctas == 1) {
       for (int c = c1; c < m; c += 128) {
         tmem_ld32(taddr(tmem, quarter * 32, c), v);
@@ -1166,7 +1159,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
       }
       cluster_barrier();
     }
-    product(aa, ap, aa, ap, rows, rows, false, full);
+    product(aa, ap, aa, ap, rows, rows, false);
     for (int c = c1; c < m; c += 128) {
       tmem_ld32(taddr(tmem, quarter * 32, c), v);
 #pragma unroll
@@ -1184,7 +1177,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
         put8(ma, ap, c + i, v + i);
       }
     }
-    if (cols > 0) product(aa, ap, ax, xp, rows, cols, true, full);
+    if (cols > 0) product(aa, ap, ax, xp, rows, cols, true);
     for (int c = c1; c < n; c += 128) {
       tmem_ld32(taddr(tmem, quarter * 32, c), v);
       if (step + 1 == q.out.steps) {

@@ -194,3 +194,15 @@ def test_same_bits_every_time_streams_and_capture():
 def test_empty():
     assert orthogonalize(torch.zeros(0, 4, 5, device="cuda")).shape == (0, 4, 5)
     assert orthogonalize(torch.zeros(4, 0, device="cuda")).shape == (4, 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(48, 80), (128, 130), (3, 16, 16), (100, 900), (200, 264), (300, 700),
+                                   (1001, 345)])
+def test_sixteen_bit_results_are_the_fp32_ones_rounded(shape, dtype):
+    """Products and sums do not depend on the result's type: a 16-bit result is
+    the fp32 result rounded once, bit for bit."""
+    G = _update(shape, dtype, seed=12)
+    full = orthogonalize(G, dtype=torch.float32)
+    for out in (torch.bfloat16, torch.float16):
+        assert torch.equal(orthogonalize(G, dtype=out), full.to(out))
