@@ -15,7 +15,8 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _code, _launch, _raise_for, _require_same_device, _status_ptr
+from .ops import (_code, _launch, _raise_for, _require_same_device, _scratch, _set_workspace,
+                  _status_ptr)
 
 __all__ = ["embed_tokens", "embed_tokens_fwd", "embed_tokens_bwd"]
 
@@ -72,7 +73,9 @@ def embed_tokens_bwd(ids, d_out, num_embeddings, scale=1.0, padding_idx=None, dt
     respect to weight: [num_embeddings, D] in ``dtype`` (default d_out's).
 
     Tokens equal to ``padding_idx`` add nothing, nor do tokens outside
-    [0, num_embeddings) (reported as in ``embed_tokens_fwd``).
+    [0, num_embeddings) (reported as in ``embed_tokens_fwd``). ``workspace``
+    is an optional contiguous CUDA tensor used instead of new memory where it
+    is large enough.
     """
     if d_out.shape[:-1] != ids.shape:
         raise ValueError(f"d_out must be [*ids.shape, D], got {tuple(d_out.shape)} for ids "
@@ -100,10 +103,8 @@ def embed_tokens_bwd(ids, d_out, num_embeddings, scale=1.0, padding_idx=None, dt
     need = ctypes.c_size_t(0)
     _raise_for(lib.ngdn2_embed_bwd_workspace_size(ctypes.byref(a), ctypes.byref(need)),
                "ngdn2_embed_bwd")
-    if need.value and (workspace is None or workspace.numel() < need.value):
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
-    if need.value:
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    workspace = _scratch(need.value, workspace, dev)
+    _set_workspace(a, workspace)
     _launch(lib.ngdn2_embed_bwd, a, dev, "ngdn2_embed_bwd")
     return dweight
 

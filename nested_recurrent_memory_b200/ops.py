@@ -197,6 +197,24 @@ def _status_ptr(dev):
     return (st or _DeviceStatus.get(dev)).word.data_ptr()
 
 
+def _scratch(need, workspace, dev):
+    """``need`` bytes of device memory for one call: the caller's workspace
+    where it is large enough, else a new one; None for no bytes."""
+    if workspace is not None and (workspace.device != dev or not workspace.is_contiguous()):
+        raise ValueError(f"workspace must be a contiguous tensor on {dev}, got one on "
+                         f"{workspace.device} with strides {tuple(workspace.stride())}")
+    if not need:
+        return None
+    if workspace is not None and workspace.numel() * workspace.element_size() >= need:
+        return workspace
+    return torch.empty(need, dtype=torch.uint8, device=dev)
+
+
+def _set_workspace(args, ws):
+    if ws is not None:
+        args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+
+
 def _require_same_device(t, *others):
     """``t`` and the others (None passes) must be on one CUDA device."""
     dev = t.device

@@ -14,7 +14,8 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _code, _launch, _raise_for, _require_same_device, _status_ptr
+from .ops import (_code, _launch, _raise_for, _require_same_device, _scratch, _set_workspace,
+                  _status_ptr)
 
 __all__ = ["orthogonalize"]
 
@@ -29,7 +30,8 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
 
     ``coefficients`` (a, b, c) must keep every singular value that starts in
     [0, 1] within [0, 4] over ``steps`` steps, else ValueError. A zero update
-    gives zeros.
+    gives zeros. ``workspace`` is an optional contiguous CUDA tensor used
+    instead of new memory where it is large enough.
     """
     if update.dim() < 2:
         raise ValueError(f"update must be [..., rows, cols], got {tuple(update.shape)}")
@@ -55,9 +57,7 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
         raise ValueError(f"coefficients {tuple(coefficients)} do not keep singular values in "
                          f"[0, 1] within [0, 4] over {steps} steps")
     _raise_for(rc, "ngdn2_orth")
-    if need.value and (workspace is None or workspace.numel() < need.value):
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
-    if need.value:
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel()
+    workspace = _scratch(need.value, workspace, dev)
+    _set_workspace(a, workspace)
     _launch(lib.ngdn2_orth, a, dev, "ngdn2_orth")
     return out

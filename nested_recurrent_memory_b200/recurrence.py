@@ -15,7 +15,8 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import _code, _launch, _raise_for, _require_same_device, _status_ptr
+from .ops import (_code, _launch, _raise_for, _require_same_device, _scratch, _set_workspace,
+                  _status_ptr)
 
 __all__ = ["gated_scan", "gated_scan_fwd", "gated_scan_bwd", "step_gated_scan"]
 
@@ -52,9 +53,7 @@ def _workspace(a, workspace, dev):
     need = ctypes.c_size_t(0)
     _raise_for(_lib.load().ngdn2_scan_workspace_size(ctypes.byref(a), ctypes.byref(need)),
                "ngdn2_scan")
-    if need.value and (workspace is None or workspace.numel() < need.value):
-        workspace = torch.empty(need.value, dtype=torch.uint8, device=dev)
-    return workspace if need.value else None
+    return _scratch(need.value, workspace, dev)
 
 
 def gated_scan_fwd(x, g, initial_state=None, output_final_state=False, return_aux=False,
@@ -64,7 +63,8 @@ def gated_scan_fwd(x, g, initial_state=None, output_final_state=False, return_au
     Returns ``(h, final_state)``: h [B, T, D] in x's dtype, final_state
     [B, D] float32 (None unless ``output_final_state``); with ``return_aux``
     also the dict that ``gated_scan_bwd`` takes (the states entering every
-    128 steps)."""
+    128 steps). ``workspace`` is an optional contiguous CUDA tensor used
+    instead of new memory where it is large enough."""
     dev = _check_inputs(x, g, initial_state)
     B, T, D = x.shape
     init = _check_state(initial_state, B, D, "initial_state")
@@ -82,8 +82,7 @@ def gated_scan_fwd(x, g, initial_state=None, output_final_state=False, return_au
         a.final_state = final.data_ptr() if final is not None else None
         a.carries = carries.data_ptr() if carries is not None else None
         ws = _workspace(a, workspace, dev)
-        if ws is not None:
-            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        _set_workspace(a, ws)
         a.status = _status_ptr(dev)
         _launch(_lib.load().ngdn2_scan, a, dev, "ngdn2_scan")
     return (h, final, dict(carries=carries)) if return_aux else (h, final)
@@ -119,8 +118,7 @@ def gated_scan_bwd(x, g, dh, d_final=None, initial_state=None, aux=None, workspa
         fwd = _scan_args(x, g, init)
         fwd.carries = carries.data_ptr()
         ws = _workspace(fwd, workspace, dev)
-        if ws is not None:
-            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        _set_workspace(a, ws)
         a.fwd = fwd
         a.d_h, a.d_h_dtype, a.d_h_stride = dh.data_ptr(), _code(dh), dh.stride()
         a.d_final = dfin.data_ptr() if dfin is not None else None

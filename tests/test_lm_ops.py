@@ -152,3 +152,17 @@ def test_shapes_are_refused():
         step_gated_scan(x, x, x)
     with pytest.raises(ValueError, match="rows, cols"):
         orthogonalize(torch.zeros(5))
+
+
+def test_scratch_memory_is_checked():
+    """Workspaces of another device or with gaps never reach a kernel."""
+    from nested_recurrent_memory_b200.ops import _scratch
+
+    cpu, need = torch.device("cpu"), 100
+    own = torch.empty(200, dtype=torch.uint8)
+    assert _scratch(need, own, cpu) is own
+    assert _scratch(need, torch.empty(50), cpu).dtype == torch.float32  # 200 bytes
+    assert _scratch(need, own[:99], cpu).numel() == need and _scratch(0, own, cpu) is None
+    for bad in (own.to("meta"), own[::2], torch.empty(1, dtype=torch.uint8).expand(200)):
+        with pytest.raises(ValueError, match="workspace"):
+            _scratch(need, bad, cpu)
