@@ -108,9 +108,9 @@ def gated_scan_bwd(x, g, dh, d_final=None, initial_state=None, aux=None, workspa
         carries = aux["carries"] if aux is not None else None
         if carries is None:
             carries = gated_scan_fwd(x, g, init, return_aux=True, workspace=workspace)[2]["carries"]
-        if (tuple(carries.shape) != (B, -(-T // _lib.SCAN_CHUNK), D)
+        if (tuple(carries.shape) != (B, -(-T // _lib.SCAN_CHUNK), D) or carries.device != dev
                 or carries.dtype != torch.float32 or not carries.is_contiguous()):
-            raise ValueError("aux is not that of a forward of these shapes")
+            raise ValueError(f"aux is not that of a forward of these shapes on {dev}")
         if dh.dtype != x.dtype:
             dh = dh.to(x.dtype)
         a = _lib.ScanBwdArgs()

@@ -37,3 +37,13 @@ def test_workspaces_elsewhere_or_with_gaps_are_refused():
         for ws in (torch.empty(1 << 22, dtype=torch.uint8), one.expand(1 << 22)):
             with pytest.raises(ValueError, match="workspace"):
                 call(ws)
+
+
+def test_forward_states_elsewhere_are_refused():
+    x, g = torch.randn(2, 300, 36, device="cuda"), -torch.rand(2, 300, 36, device="cuda")
+    carries = gated_scan_fwd(x, g, return_aux=True)[2]["carries"]
+    ref = gated_scan_bwd(x, g, x, aux=dict(carries=carries))
+    assert all(torch.equal(p, q) for p, q in zip(ref[:2], gated_scan_bwd(x, g, x)[:2]))
+    for bad in (carries.cpu(), carries.double(), carries[:, :2], carries.mT.contiguous().mT):
+        with pytest.raises(ValueError, match="aux"):
+            gated_scan_bwd(x, g, x, aux=dict(carries=bad))
