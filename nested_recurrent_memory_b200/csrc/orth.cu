@@ -494,6 +494,12 @@ __device__ __forceinline__ bool wait_cluster_or_die(Barriers* s, uint64_t* bar, 
   return false;
 }
 
+// What is still under way when a CTA leaves early, waited for with a limit of its own.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t phase, uint32_t polls) {
+  for (uint32_t i = 0; i < polls; ++i)
+    if (mbar_try_wait(bar, phase)) return;
+}
+
 // Until the matrix's operands of a unit are written; what follows, by whichever
 // path it reads, comes after.
 __device__ __forceinline__ bool wait_operands(Barriers* s, const MulArgs& p, const Unit& u) {
@@ -748,24 +754,25 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
       if (slot == 0) unit_phase ^= 1;
       return true;
     };
-    uint32_t next = 0;
+    uint32_t next = 0, filled = 0;  // (stages, kStages at most)
     const bool fetches = rank == 0 && p.wait;
     if (p.wait) after_previous();
-    if (fetches && !fetch(&next)) goto done;
-    for (;;) {
+    bool ok = !fetches || fetch(&next);
+    while (ok) {
       if (fetches) t = next;
-      else if (!next_unit(s, p, &slot, &unit_phase, &t)) goto done;
-      if (t >= p.end) break;
+      else if (!next_unit(s, p, &slot, &unit_phase, &t)) ok = false;
+      if (!ok || t >= p.end) break;
       const Unit u = unit_at<BN>(p, plan, t);
       const CUtensorMap* left = u.mode == kGram ? &maps.x_left[u.step & 1] : u.mode == kPoly ? &maps.a_left : &maps.b_left;
       const CUtensorMap* right = u.mode == kPoly ? &maps.a_right : &maps.x_right[u.step & 1];
       const int row = int(u.tm * kRows + rank * 128), col = int(u.tn * BN + rank * (BN / 2)), z = int(u.b * 2);
       const uint32_t bytes = 2 * (kLeft * (u.lo_left ? 2 : 1) + kRight * (u.lo_right ? 2 : 1));
       if (!p.wait) after_previous();
-      else if (!wait_operands(s, p, u)) goto done;
-      for (int k = 0; k < u.blocks; ++k) {
-        if (fetches && k + 1 == u.blocks && !fetch(&next)) goto done;
-        if (!wait_or_die(s, &s->empty[st], phase ^ 1, p)) goto done;
+      else ok = wait_operands(s, p, u);
+      for (int k = 0; ok && k < u.blocks; ++k) {
+        if (fetches && k + 1 == u.blocks) ok = fetch(&next);
+        ok = ok && wait_or_die(s, &s->empty[st], phase ^ 1, p);
+        if (!ok) break;
         const uint32_t at = base + st * kStage, bar = in_first(&s->full[st]);
         if (rank == 0) mbar_arrive_expect_tx(&s->full[st], bytes);
         for (int pl = 0; pl < 2; ++pl) {
@@ -779,6 +786,7 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
               else load_box(to, right, k * kDepth, c, z + pl, bar);
             }
         }
+        filled += filled < kStages;
         if (++st == kStages) {
           st = 0;
           phase ^= 1;
@@ -786,28 +794,41 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
       }
     }
     // Until the last MMAs have signalled here, this CTA's memory is needed.
-    for (int i = 0; i < kStages; ++i) {
-      if (!wait_or_die(s, &s->empty[st], phase ^ 1, p)) goto done;
-      if (++st == kStages) {
-        st = 0;
+    uint32_t end = st, end_phase = phase;
+    for (int i = 0; ok && i < kStages; ++i) {
+      ok = wait_or_die(s, &s->empty[end], end_phase ^ 1, p);
+      if (++end == kStages) {
+        end = 0;
+        end_phase ^= 1;
+      }
+    }
+    // Left early: the loads under way, as far as both CTAs' parts of a stage are
+    // counted here.
+    for (; !ok && rank == 0 && filled > 0; --filled) {
+      if (st == 0) {
+        st = kStages;
         phase ^= 1;
       }
+      drain(&s->full[--st], phase, 1u << 16);
     }
   } else if (warp == 1 && lane == 0 && rank == 0) {
     uint32_t st = 0, phase = 0, buf = 0, acc_phase = 0;
+    uint64_t* last = nullptr;  // signalled by the latest MMAs, in phase last_phase
+    uint32_t last_phase = 0;
+    bool ok = true;
     for (;;) {
-      if (!next_unit(s, p, &slot, &unit_phase, &t)) goto done;
-      if (t >= p.end) break;
+      if (!next_unit(s, p, &slot, &unit_phase, &t) || t >= p.end) break;
       const Unit u = unit_at<BN>(p, plan, t);
       const bool down = APP && (!SYM || u.mode == kApply);
       const uint32_t idesc = idesc_f16(kRows, BN, false, false, down);
       const uint64_t left_desc = desc_sw128(base, 1024), right_step = (down ? Shape<BN>::kBoxCols * 32 : 32) >> 4;
       const uint64_t right_desc = down ? desc_down<Shape<BN>::kBoxCols>(base + 2 * kLeft, Shape<BN>::kBox)
                                        : desc_sw128(base + 2 * kLeft, 1024);
-      if (!wait_or_die(s, &s->acc_empty[buf], acc_phase ^ 1, p)) goto done;
+      ok = wait_or_die(s, &s->acc_empty[buf], acc_phase ^ 1, p);
       const uint32_t d = tmem + buf * BN;
-      for (int k = 0; k < u.blocks; ++k) {
-        if (!wait_or_die(s, &s->full[st], phase, p)) goto done;
+      for (int k = 0; ok && k < u.blocks; ++k) {
+        ok = wait_or_die(s, &s->full[st], phase, p);
+        if (!ok) break;
         fence_after_sync();
         // Descriptors count 16 bytes: the lo planes and the next 16 of the
         // reduction (32 bytes of a row, or 16 rows) are additions away. One thread
@@ -823,22 +844,27 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
           dr += right_step;
         }
         commit_pair(&s->empty[st]);
+        last = &s->empty[st];
+        last_phase = phase;
         if (++st == kStages) {
           st = 0;
           phase ^= 1;
         }
       }
+      if (!ok) break;
       commit_pair(&s->acc_full[buf]);
       buf ^= 1;
       if (buf == 0) acc_phase ^= 1;
     }
+    // (The loads' thread waits for the same, unless it has left early.)
+    if (last) drain(last, last_phase, kPolls);
   } else if (warp >= 4) {
     uint32_t buf = 0, acc_phase = 0;
     unsigned char* const mem = smem + kStages * kStage + (warp - 4) * 2 * kOutPlane;
     for (;;) {
       bool ok = true;
       if (lane == 0) ok = next_unit(s, p, &slot, &unit_phase, &t);
-      if (!__all_sync(0xffffffffu, ok)) goto done;
+      if (!__all_sync(0xffffffffu, ok)) break;
       t = __shfl_sync(0xffffffffu, t, 0);
       if (t >= p.end) break;
       const Unit u = unit_at<BN>(p, plan, t);
@@ -852,7 +878,7 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
         else if (u.mode == kPoly) ok = write(std::integral_constant<int, kPoly>{}, &maps.b_out);
       if constexpr (APP)
         if (u.mode == kApply) ok = write(std::integral_constant<int, kApply>{}, &maps.x_out[~u.step & 1]);
-      if (!__all_sync(0xffffffffu, ok)) goto done;
+      if (!__all_sync(0xffffffffu, ok)) break;
       fence_before_sync();
       __syncwarp();
       if (lane == 0) {
@@ -866,11 +892,14 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
       if (buf == 0) acc_phase ^= 1;
     }
   }
-done:
   if (warp >= 4 && lane == 0) bulk_wait0();
   __syncwarp();
   fence_before_sync();
   __syncthreads();
+  // The second CTA's loads signal in the first, which may have left before it
+  // counted them: a copy takes microseconds, and this CTA's memory stays that long.
+  if (s->dead)
+    for (int i = 0; i < 200; ++i) __nanosleep(1000);
   cluster_barrier();
   if (warp == 2) {
     fence_after_sync();
@@ -1087,7 +1116,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
     const bool ok = mbar_wait(&bar, phase, 1u << 20);
     phase ^= 1;
     fence_after_sync();
-    if (!ok) atomicOr(q.out.status, NGDN2_STATUS_WAIT_TIMEOUT);
+    if (!ok) {
+      atomicOr(q.out.status, NGDN2_STATUS_WAIT_TIMEOUT);
+      mbar_wait(&bar, phase ^ 1, 1u << 20);  // (once more: nothing is under way when the CTA leaves)
+    }
     alive = !__syncthreads_or(!ok);
   };
   // Eight results as planes.
