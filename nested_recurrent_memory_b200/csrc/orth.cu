@@ -599,7 +599,11 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
   const int m = int(p.m), cols = int(MODE == kApply ? p.n : p.m), z = int(u.b * 2);
   const int r0 = int(u.tm * kRows + rank * 128 + quarter * 32), r = r0 + lane, c1 = int(u.tn * BN + half * (BN / 2));
   const bool mirror = MODE != kApply && u.tn / (kRows / BN) != u.tm;
-  const float sigma = u.step == 0 ? p.sigma[u.b] : 1.f / kScale;
+  float sigma = u.step == 0 ? p.sigma[u.b] : 1.f / kScale;
+  // Once a wait of this call has given up, in this launch or an earlier one, operands
+  // may be unfinished: nothing made of them passes as a result.
+  if (MODE == kApply && u.last && *reinterpret_cast<volatile uint32_t*>(&p.sync->stop))
+    sigma = __int_as_float(0x7fc00000);
   // A's own values for sixteen columns from c on, asked for one turn ahead.
   const __half* old = p.A + (int64_t(z) * m + r) * p.ld;
   uint4 oh[2] = {}, ol[2] = {};
@@ -905,7 +909,7 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
     fence_after_sync();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
   }
-  if (s->dead) {  // nothing that was not computed passes as a result
+  if (s->dead) {  // (its units may not have been written at all)
     for (int64_t e = threadIdx.x; e < p.batch * p.m * p.n; e += kMulThreads)
       store_elem(p.final_out, e, __int_as_float(0x7fc00000), p.out_dtype);
   }

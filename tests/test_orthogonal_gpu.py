@@ -240,3 +240,11 @@ def test_a_call_that_gave_up_ends_and_leaves_the_next_one_alone():
     _stopped_call()
     assert torch.equal(orthogonalize(G), ref)
     check_status()
+
+
+def test_a_call_that_gave_up_leaves_no_numbers():
+    """Whatever later launches of the call compute from operands that were never
+    finished does not pass as a result."""
+    _, out = _stopped_call()
+    assert bool(torch.isnan(out).all())
+    check_status()
