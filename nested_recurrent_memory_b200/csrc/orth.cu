@@ -998,6 +998,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   __shared__ Scale scale;
   __shared__ uint64_t bar;
   __shared__ uint32_t tmem_at;
+  __shared__ int lost;  // a CTA of the cluster gave up
   const PrepArgs& p = q.in;
   const SmallLayout lay(q);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -1012,6 +1013,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   if (tid == 0) {
     mbar_init(&bar, 1);
     fence_mbar_init();
+    lost = 0;
   }
   if (warp == 0) tmem_alloc(&tmem_at, 256);
   for (int i = tid * 16; i < 2 * (xp + ap); i += kSmallThreads * 16)
@@ -1098,7 +1100,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
 
   // D[128 x cols] = L R, reduction over ``depth`` (multiples of 16). After a wait
   // that gave up nothing is multiplied any more, but the cluster goes on
-  // together.
+  // together, and learns of it when A's slices are exchanged.
   auto product = [&](uint32_t L, int lp, uint32_t R, int rp, int depth, int cols, bool down) {
     fence_proxy_async();
     fence_before_sync();
@@ -1164,7 +1166,10 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
                          "f"(v[i + 1]), "f"(v[i + 2]), "f"(v[i + 3])
                          : "memory");
       }
+      if (!alive && tid < ctas)
+        asm volatile("st.shared::cluster.u32 [%0], 1;" ::"r"(in_cta(smem_u32(&lost), tid)) : "memory");
       cluster_barrier();
+      alive = alive && !*reinterpret_cast<volatile int*>(&lost);
       // Eight columns of a row a thread; eight neighbours' results are 128 bytes.
       for (int e = tid; e < q.part * (rows / 8); e += kSmallThreads) {
         const int g = e % (rows / 8), r = rank * q.part + e / (rows / 8);
@@ -1214,12 +1219,15 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
       }
     }
     if (cols > 0) product(aa, ap, ax, xp, rows, cols, true);
+    // Nothing that was not computed passes as a result. (A CTA that gave up since A was
+    // summed has spoilt only its own columns.)
+    const float last = alive ? sigma / kScale : __int_as_float(0x7fc00000);
     for (int c = c1; c < n; c += 128) {
       tmem_ld32(taddr(tmem, quarter * 32, c), v);
       if (step + 1 == q.out.steps) {
 #pragma unroll
         for (int i = 0; i < 32; i += 8)
-          if (row < m && c + i < n) write_final(q.out, b, row, col0 + c + i, sigma / kScale, v + i, n - c - i);
+          if (row < m && c + i < n) write_final(q.out, b, row, col0 + c + i, last, v + i, n - c - i);
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = c + i < n ? v[i] * sigma : 0.f;
@@ -1228,10 +1236,6 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
           if (row < rows && c + i < q.slice) put8(mx, xp, c + i, v + i);
       }
     }
-  }
-  if (!alive) {  // nothing that was not computed passes as a result
-    for (int64_t e = tid; e < p.m * p.n; e += kSmallThreads)
-      store_elem(q.out.final_out, b * p.m * p.n + e, __int_as_float(0x7fc00000), q.out.out_dtype);
   }
   fence_before_sync();
   __syncthreads();
