@@ -54,8 +54,23 @@ namespace {
 
 bool dtype_ok(int d) { return d == NGDN2_F32 || d == NGDN2_BF16 || d == NGDN2_F16; }
 
-// Planes hold kScale times the values of X (after the first step), A and B.
+// Planes hold kScale times the values of A and B, and of X (after the first step)
+// where X may reach 1/2. Where it cannot, because |G|_F is far below eps or the
+// coefficients shrink it, they hold as many powers of two more: at a fixed scale its
+// digits fell below fp16's smallest number (|G|_F = 1e-14, eps = 1e-7: off by 1 %).
 constexpr float kScale = 1024.f;
+
+// A bound on a step's X: its Frobenius norm, grown by |a| + |b| s^2 + |c| s^4 a step.
+__device__ __forceinline__ float grown(float u, float a, float b, float c) {
+  const float q = u * u;
+  return u * (fabsf(a) + q * (fabsf(b) + q * fabsf(c)));
+}
+
+// The power of two that brings a bound below 1/2 into [1/2, 1), 2^112 at most; 1 for others.
+__device__ __forceinline__ float room(float u) {
+  const int e = 126 - int(__float_as_uint(u) >> 23);
+  return __uint_as_float(uint32_t(127 + (e < 0 ? 0 : e > 112 ? 112 : e)) << 23);
+}
 // |a + b s^2 + c s^4| and singular values s stay below these (checked on the
 // host), so that the planes stay within fp16.
 constexpr double kMaxFactor = 60.0, kMaxSigma = 4.0;
@@ -97,7 +112,10 @@ struct PrepArgs {
   float eps;
   int parts;               // of a matrix's sum of squares, a multiple of 32
   double* part;            // [batch][parts]
-  float* sigma;            // [batch]: X_0 = sigma * planes
+  float2* scale;           // [batch][steps] (one at least): X = x * planes, and B X * y gives
+                           // the next step's planes, or the result
+  int steps;
+  float ca, cb, cc;        // coefficients
   __half* x;               // [batch][2][m][ld]; the lo plane only where lo is set
   int64_t ld;
   bool lo;
@@ -173,27 +191,24 @@ __global__ void __launch_bounds__(kPrepThreads) orth_norm_kernel(const __grid_co
   let_next_start();
 }
 
-// For a sum of squares: the power of two that brings the norm into [2^11, 2^12),
-// and sigma.
-__device__ __forceinline__ void scale_of(double sum, float eps, int* k, float* sigma) {
-  const double norm = sqrt(sum);
-  const bool finite = norm > 0.0 && norm < 1e300;
-  int e = 12;
-  if (finite) frexp(norm, &e);
-  *k = 12 - e;
-  *sigma = float(1.0 / (norm + double(eps)) / scalbn(1.0, *k));
-}
-
 // What a CTA scales an update by, computed by one of its threads (64-bit square
 // roots and divisions by all of them queue up for the few 64-bit units):
-// x * s1 * s2 are the planes' values.
+// x * s1 * s2, by a power of two that brings the norm into [2^11, 2^12), are the
+// planes' values, and sigma times them X_0, whose norm is u. (2^140 at most: it brings
+// even the smallest fp32 number into fp16's range, and sigma stays a normal number.)
 struct Scale {
-  float s1, s2, sigma;
+  float s1, s2, sigma, u;
   __device__ __forceinline__ void set(double sum, float eps) {
-    int k;
-    scale_of(sum, eps, &k, &sigma);
+    const double norm = sqrt(sum);
+    const bool finite = norm > 0.0 && norm < 1e300;
+    int e = 12;
+    if (finite) frexp(norm, &e);
+    const int k = 12 - e < 140 ? 12 - e : 140;
     s1 = scalbnf(1.f, k / 2);
     s2 = scalbnf(1.f, k - k / 2);
+    const double per = 1.0 / (norm + double(eps));
+    sigma = float(per / scalbn(1.0, k));
+    u = finite ? float(norm * per) : 1.f;
   }
 };
 
@@ -222,7 +237,17 @@ __global__ void __launch_bounds__(kPrepThreads) orth_convert_kernel(const __grid
   const int64_t b = blockIdx.x / (tc * tr), q = blockIdx.x % (tc * tr);
   __shared__ Scale scale;
   norm_scale(p, b, &scale);
-  if (q == 0 && threadIdx.x == 0) p.sigma[b] = scale.sigma;
+  if (q == 0 && threadIdx.x == 0) {
+    float x = scale.sigma, u = scale.u;
+    float2* to = p.scale + b * (p.steps > 0 ? p.steps : 1);
+    to[0].x = x;
+    for (int k = 0; k < p.steps; ++k) {
+      u = grown(u, p.ca, p.cb, p.cc);
+      const float more = room(u);
+      to[k] = make_float2(x, k + 1 < p.steps ? x * more : x / kScale);
+      x = 1.f / (kScale * more);
+    }
+  }
   const float s1 = scale.s1, s2 = scale.s2;
   __half* hi = p.x + b * 2 * p.m * p.ld;
   __half* lo = hi + p.m * p.ld;
@@ -312,7 +337,7 @@ struct MulArgs {
   int64_t batch, m, n;   // X is m x n
   int steps;
   float a, b, c;
-  const float* sigma;    // [batch]: the scale of the first step's X; then 1 / kScale
+  const float2* scale;   // [batch][steps], as PrepArgs has it
   bool x_lo;             // whether the first step's X has a lo plane
   __half *A, *B;         // their planes, rows ld apart
   int64_t ld;
@@ -599,11 +624,11 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
   const int m = int(p.m), cols = int(MODE == kApply ? p.n : p.m), z = int(u.b * 2);
   const int r0 = int(u.tm * kRows + rank * 128 + quarter * 32), r = r0 + lane, c1 = int(u.tn * BN + half * (BN / 2));
   const bool mirror = MODE != kApply && u.tn / (kRows / BN) != u.tm;
-  float sigma = u.step == 0 ? p.sigma[u.b] : 1.f / kScale;
+  float2 scale = p.scale[u.b * p.steps + u.step];
   // Once a wait of this call has given up, in this launch or an earlier one, operands
   // may be unfinished: nothing made of them passes as a result.
   if (MODE == kApply && u.last && *reinterpret_cast<volatile uint32_t*>(&p.sync->stop))
-    sigma = __int_as_float(0x7fc00000);
+    scale.y = __int_as_float(0x7fc00000);
   // A's own values for sixteen columns from c on, asked for one turn ahead.
   const __half* old = p.A + (int64_t(z) * m + r) * p.ld;
   uint4 oh[2] = {}, ol[2] = {};
@@ -641,8 +666,8 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
     tmem_ld16(taddr(acc, quarter * 32, half * (BN / 2) + i), v);
     if (MODE == kApply && u.last) {
       if (r < m) {
-        write_final(p, u.b, r, c, sigma / kScale, v, cols - c);
-        if (c + 8 < cols) write_final(p, u.b, r, c + 8, sigma / kScale, v + 8, cols - c - 8);
+        write_final(p, u.b, r, c, scale.y, v, cols - c);
+        if (c + 8 < cols) write_final(p, u.b, r, c + 8, scale.y, v + 8, cols - c - 8);
       }
       continue;
     }
@@ -654,7 +679,7 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
       float x[2] = {v[2 * j], v[2 * j + 1]};
       if (MODE == kGram) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) x[k] = x[k] * sigma * sigma * kScale;
+        for (int k = 0; k < 2; ++k) x[k] = x[k] * scale.x * scale.x * kScale;
       } else if (MODE == kPoly) {
         const float2 o = join(reinterpret_cast<const uint32_t*>(ph)[j], reinterpret_cast<const uint32_t*>(pl)[j]);
 #pragma unroll
@@ -662,7 +687,7 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
           x[k] = p.c * (x[k] / kScale) + p.b * (k ? o.y : o.x) + (c + 2 * j + k == r ? p.a * kScale : 0.f);
       } else {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) x[k] *= sigma;  // (sigma X^) (B^ / kScale), times kScale
+        for (int k = 0; k < 2; ++k) x[k] *= scale.y;
       }
       split(x[0], x[1], h[j], l[j]);
     }
@@ -1069,7 +1094,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
     scale.set(sum, p.eps);
   }
   __syncthreads();
-  float sigma = scale.sigma;
+  float sigma = scale.sigma, bound = scale.u;
   const float s1 = scale.s1, s2 = scale.s2;
 #pragma unroll
   for (int k = 0; k < kPieces; ++k) {
@@ -1138,7 +1163,9 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
   };
 
   const int rows = q.rows, cols = (n + 15) & ~15;
-  for (int step = 0; step < q.out.steps; ++step, sigma = 1.f / kScale) {
+  for (int step = 0; step < q.out.steps; ++step) {
+    bound = grown(bound, q.out.a, q.out.b, q.out.c);
+    const float more = room(bound);
     float v[32];
     product(ax, xp, ax, xp, cols, rows, false);
     if (ctas == 1) {
@@ -1221,7 +1248,8 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
     if (cols > 0) product(aa, ap, ax, xp, rows, cols, true);
     // Nothing that was not computed passes as a result. (A CTA that gave up since A was
     // summed has spoilt only its own columns.)
-    const float last = alive ? sigma / kScale : __int_as_float(0x7fc00000);
+    const float last = alive ? sigma / kScale : __int_as_float(0x7fc00000), next = sigma * more;
+    sigma = 1.f / (kScale * more);
     for (int c = c1; c < n; c += 128) {
       tmem_ld32(taddr(tmem, quarter * 32, c), v);
       if (step + 1 == q.out.steps) {
@@ -1230,7 +1258,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
           if (row < m && c + i < n) write_final(q.out, b, row, col0 + c + i, last, v + i, n - c - i);
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = c + i < n ? v[i] * sigma : 0.f;
+        for (int i = 0; i < 32; ++i) v[i] = c + i < n ? v[i] * next : 0.f;
 #pragma unroll
         for (int i = 0; i < 32; i += 8)
           if (row < rows && c + i < q.slice) put8(mx, xp, c + i, v + i);
@@ -1253,7 +1281,7 @@ orth_scale_kernel(const __grid_constant__ PrepArgs p, void* out, int out_dtype, 
   if (i >= p.batch * p.m * p.n) return;
   const int64_t b = i / (p.m * p.n), r = i / p.n % p.m, c = i % p.n;
   const __half* hi = p.x + b * 2 * p.m * p.ld + r * p.ld + c;
-  const float x = (__half2float(hi[0]) + (p.lo ? __half2float(hi[p.m * p.ld]) : 0.f)) * p.sigma[b];
+  const float x = (__half2float(hi[0]) + (p.lo ? __half2float(hi[p.m * p.ld]) : 0.f)) * p.scale[b].x;
   store_elem(out, b * p.m * p.n + (transposed ? c * p.m + r : r * p.n + c), x, out_dtype);
 }
 
@@ -1273,7 +1301,7 @@ cudaError_t by_type(int dt, F&& f) {
 struct OrthLayout {
   int64_t m, n, ldx, lda;
   int parts;
-  size_t x, y, A, B, part, sigma, sync, total;
+  size_t x, y, A, B, part, scale, sync, total;
 };
 
 OrthLayout layout(const ngdn2_orth_args* a) {
@@ -1294,7 +1322,7 @@ OrthLayout layout(const ngdn2_orth_args* a) {
   L.A = take(size_t(a->batch) * 2 * L.m * L.lda * 2);
   L.B = take(size_t(a->batch) * 2 * L.m * L.lda * 2);
   L.part = take(size_t(a->batch) * L.parts * sizeof(double));
-  L.sigma = take(size_t(a->batch) * sizeof(float));
+  L.scale = take(size_t(a->batch) * (a->steps > 0 ? a->steps : 1) * sizeof(float2));
   L.sync = take((kSyncWords + size_t(a->batch)) * sizeof(uint64_t));
   L.total = at + 256;
   return L;
@@ -1446,7 +1474,11 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
   pr.sc = a->update_stride[tall ? 1 : 2];
   pr.eps = a->eps;
   pr.part = reinterpret_cast<double*>(ws + L.part);
-  pr.sigma = reinterpret_cast<float*>(ws + L.sigma);
+  pr.scale = reinterpret_cast<float2*>(ws + L.scale);
+  pr.steps = a->steps;
+  pr.ca = a->coef[0];
+  pr.cb = a->coef[1];
+  pr.cc = a->coef[2];
   pr.x = x;
   pr.ld = L.ldx;
   pr.parts = L.parts;
@@ -1531,7 +1563,7 @@ NGDN2_API int ngdn2_orth(const ngdn2_orth_args* a, void* stream) {
   p.a = a->coef[0];
   p.b = a->coef[1];
   p.c = a->coef[2];
-  p.sigma = pr.sigma;
+  p.scale = pr.scale;
   p.x_lo = pr.lo;
   p.A = A;
   p.B = B;

@@ -248,3 +248,29 @@ def test_a_call_that_gave_up_leaves_no_numbers():
     _, out = _stopped_call()
     assert bool(torch.isnan(out).all())
     check_status()
+
+
+@pytest.mark.parametrize("norm", [1.0, 1e-3, 1e-7, 1e-11, 1e-14, 1e-20, 1e-30])
+@pytest.mark.parametrize("shape", [(64, 80), (900, 100), (200, 260), (2, 384, 1000)])
+def test_updates_below_eps_keep_their_digits(shape, norm):
+    """X_0 = G / (|G| + eps) is small where |G| is far below eps, and every error
+    is relative to it: the bound above times |X_0|."""
+    G = _update(shape, torch.float32, seed=15)
+    G = G / torch.linalg.matrix_norm(G, keepdim=True) * norm
+    ref = _exact(G)
+    size = torch.linalg.matrix_norm(G.double())
+    X0 = size / (size + 1e-7)
+    for dtype in (torch.float32, torch.bfloat16):
+        err = torch.linalg.matrix_norm(orthogonalize(G, dtype=dtype).double() - ref)
+        bound = 6 * MUON[0] ** 5 * DELTA * X0 + UNIT[dtype] * torch.linalg.matrix_norm(ref)
+        assert bool((err <= bound).all()), (err / bound).max().item()
+
+
+def test_iterations_that_shrink_keep_their_digits():
+    """Coefficients below one: forty halvings."""
+    for shape in ((48, 64), (150, 270)):
+        G = _update(shape, torch.float32, seed=16)
+        out = orthogonalize(G, steps=40, coefficients=(0.5, 0.0, 0.0), dtype=torch.float32)
+        ref = _exact(G, steps=40, coefficients=(0.5, 0.0, 0.0))
+        err = torch.linalg.matrix_norm(out.double() - ref)
+        assert bool((err <= 41 * DELTA * 0.5 ** 40).all())
