@@ -41,6 +41,17 @@ class Muon(torch.optim.Optimizer):
                 if p.dim() < 2:
                     raise ValueError(f"Muon takes matrices [..., rows, cols], got {tuple(p.shape)}")
 
+    def load_state_dict(self, state_dict):
+        """As torch's, which casts a state to its parameter's type; momenta stay
+        float32."""
+        super().load_state_dict(state_dict)
+        for saved, group in zip(state_dict["param_groups"], self.param_groups):
+            for i, p in zip(saved["params"], group["params"]):
+                if "momentum" in state_dict["state"].get(i, ()):
+                    self.state[p]["momentum"] = state_dict["state"][i]["momentum"].to(
+                        device=p.device, dtype=torch.float32, copy=True,
+                        memory_format=torch.contiguous_format)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
