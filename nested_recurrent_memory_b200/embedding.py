@@ -15,8 +15,8 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import (_code, _launch, _raise_for, _require_same_device, _scratch, _set_workspace,
-                  _status_ptr)
+from .ops import (_code, _has_tangent, _launch, _raise_for, _require_same_device, _scratch,
+                  _set_workspace, _status_ptr)
 
 __all__ = ["embed_tokens", "embed_tokens_fwd", "embed_tokens_bwd"]
 
@@ -109,25 +109,62 @@ def embed_tokens_bwd(ids, d_out, num_embeddings, scale=1.0, padding_idx=None, dt
     return dweight
 
 
+def _differentiated(t):
+    return torch.is_grad_enabled() and t.requires_grad or _has_tangent(t)
+
+
 class EmbedTokensFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx):
         ctx.save_for_backward(ids)
+        ctx.save_for_forward(ids)
         ctx.meta = (weight.shape[0], scale, padding_idx, weight.dtype)
         return embed_tokens_fwd(ids, weight, scale)
 
     @staticmethod
     def backward(ctx, d_out):
         (ids,) = ctx.saved_tensors
-        V, scale, padding_idx, dtype = ctx.meta
-        return None, embed_tokens_bwd(ids, d_out, V, scale, padding_idx, dtype), None, None
+        gradient = EmbedTokensBwdFunction.apply if _differentiated(d_out) else embed_tokens_bwd
+        return None, gradient(ids, d_out, *ctx.meta), None, None
+
+    @staticmethod
+    def jvp(ctx, _ids, d_weight, _scale, _padding_idx):
+        (ids,) = ctx.saved_tensors
+        return embed_tokens(ids, d_weight, ctx.meta[1], ctx.meta[2])
+
+
+class EmbedTokensBwdFunction(torch.autograd.Function):
+    """The gradient as a function of d_out: linear, so its own derivative is
+    the lookup, zero for padding."""
+
+    @staticmethod
+    def forward(ctx, ids, d_out, V, scale, padding_idx, dtype):
+        ctx.save_for_backward(ids)
+        ctx.save_for_forward(ids)
+        ctx.meta = (V, scale, padding_idx, dtype)
+        ctx.d_type = d_out.dtype
+        return embed_tokens_bwd(ids, d_out, V, scale, padding_idx, dtype)
+
+    @staticmethod
+    def backward(ctx, d_weight):
+        (ids,) = ctx.saved_tensors
+        V, scale, padding_idx, _ = ctx.meta
+        d = embed_tokens(ids, d_weight, scale, padding_idx).to(ctx.d_type)
+        if padding_idx is not None:
+            d = d.masked_fill((ids == padding_idx % V).unsqueeze(-1), 0.0)
+        return None, d, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, _ids, d_out, *_):
+        (ids,) = ctx.saved_tensors
+        return EmbedTokensBwdFunction.apply(ids, d_out, *ctx.meta)
 
 
 def embed_tokens(ids, weight, scale=1.0, padding_idx=None):
     """``embed_tokens_fwd`` with its gradient (``embed_tokens_bwd``) in
-    autograd. ``padding_idx``'s row is looked up like any other and gets no
-    gradient."""
+    autograd, to any order and in forward mode. ``padding_idx``'s row is looked
+    up like any other and gets no gradient."""
     _padding(padding_idx, weight.shape[0])
-    if not (torch.is_grad_enabled() and weight.requires_grad):
+    if not _differentiated(weight):
         return embed_tokens_fwd(ids, weight, scale)
     return EmbedTokensFunction.apply(ids, weight, float(scale), padding_idx)

@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -213,6 +214,12 @@ def _scratch(need, workspace, dev):
 def _set_workspace(args, ws):
     if ws is not None:
         args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
+
+
+def _has_tangent(*ts):
+    """Whether any of them (None passes) carries a forward-mode tangent, of
+    which ``requires_grad`` says nothing."""
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 def _require_same_device(t, *others):

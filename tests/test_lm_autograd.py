@@ -1,0 +1,108 @@
+"""The autograd functions of the embedding and the recurrence on the host,
+their kernels replaced by plain operations that leave no graph (as kernels do
+not): second derivatives and forward-mode tangents are right or refused,
+never dropped."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+import torch.nn.functional as F
+
+from nested_recurrent_memory_b200 import embedding
+from nested_recurrent_memory_b200.embedding import embed_tokens
+
+V, D, SCALE = 7, 3, 1.5
+
+
+@pytest.fixture
+def plain_embedding(monkeypatch):
+    def fwd(ids, weight, scale=1.0):
+        return (weight.detach()[ids] * scale).clone()
+
+    def bwd(ids, d_out, num_embeddings, scale=1.0, padding_idx=None, dtype=None, workspace=None):
+        d = d_out.detach().reshape(-1, d_out.shape[-1]) * scale
+        keep = torch.ones(ids.numel(), dtype=torch.bool)
+        if padding_idx is not None:
+            keep = ids.flatten() != padding_idx % num_embeddings
+        dw = torch.zeros(num_embeddings, d.shape[1], dtype=d.dtype)
+        return dw.index_add_(0, ids.flatten()[keep], d[keep]).to(dtype or d.dtype)
+
+    monkeypatch.setattr(embedding, "embed_tokens_fwd", fwd)
+    monkeypatch.setattr(embedding, "embed_tokens_bwd", bwd)
+
+
+def _case():
+    gen = torch.Generator().manual_seed(0)
+    ids = torch.randint(0, V, (4, 5), generator=gen)
+    w, t = (torch.randn(V, D, generator=gen, dtype=torch.float64) for _ in range(2))
+    return ids, w, t, torch.randn(4, 5, D, generator=gen, dtype=torch.float64)
+
+
+def _torch(ids, w, pad):
+    return F.embedding(ids, w, pad) * SCALE
+
+
+@pytest.mark.parametrize("pad", [None, 2, -1])
+def test_embedding_second_derivatives(plain_embedding, pad):
+    """A penalty on the gradient of a loss that is not linear in the rows."""
+    ids, w, t, c = _case()
+    got = []
+    for fn in (lambda x: embed_tokens(ids, x, SCALE, pad), lambda x: _torch(ids, x, pad)):
+        x = w.clone().requires_grad_()
+        (g,) = torch.autograd.grad((fn(x).sin() * c).sum(), x, create_graph=True)
+        assert g.requires_grad
+        (g2,) = torch.autograd.grad((g * g * t).sum(), x, create_graph=True)
+        (g3,) = torch.autograd.grad(g2.pow(3).sum(), x)
+        got.append((g, g2, g3))
+    for p, q in zip(*got):
+        assert torch.allclose(p, q, rtol=1e-12, atol=1e-12)
+
+
+def test_embedding_gradients_against_differences(plain_embedding):
+    ids, w, _, _ = _case()
+    w.requires_grad_()
+    torch.autograd.gradcheck(lambda x: embed_tokens(ids, x, SCALE, 2)[ids != 2], (w,),
+                             check_forward_ad=True)
+    torch.autograd.gradgradcheck(lambda x: embed_tokens(ids, x, SCALE, 2)[ids != 2].sin(), (w,))
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_embedding_forward_mode(plain_embedding, requires_grad):
+    ids, w, t, _ = _case()
+    w.requires_grad_(requires_grad)
+    with fwAD.dual_level():
+        x = fwAD.make_dual(w, t)
+        y, ref = embed_tokens(ids, x, SCALE, 2), _torch(ids, x, 2)
+        assert torch.equal(fwAD.unpack_dual(y).tangent, fwAD.unpack_dual(ref).tangent)
+
+
+def test_embedding_reverse_over_forward(plain_embedding):
+    """The tangent of a gradient (a Hessian-vector product) without second reverse."""
+    ids, w, t, c = _case()
+    got = []
+    for fn in (lambda x: embed_tokens(ids, x, SCALE, 2), lambda x: _torch(ids, x, 2)):
+        with fwAD.dual_level():
+            x = fwAD.make_dual(w.clone().requires_grad_(), t)
+            (g,) = torch.autograd.grad((fn(x).sin() * c).sum(), x)
+            got.append(fwAD.unpack_dual(g).tangent)
+    assert got[0] is not None and torch.allclose(*got, rtol=1e-12, atol=1e-12)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_embedding_derivatives_on_the_kernels(dtype):
+    """All values are small whole numbers: no sum rounds, so both agree exactly."""
+    gen = torch.Generator().manual_seed(1)
+    small = lambda *s: torch.randint(-2, 3, s, generator=gen).to(dtype).cuda()  # noqa: E731
+    ids = torch.randint(0, 50, (6, 9), generator=gen).cuda()
+    w, t, c = small(50, 24), small(50, 24), small(6, 9, 24)
+    got = []
+    for fn in (lambda x: embed_tokens(ids, x, 2.0, 3), lambda x: F.embedding(ids, x, 3) * 2.0):
+        x = w.clone().requires_grad_()
+        (g,) = torch.autograd.grad((fn(x) ** 2 * c).sum(), x, create_graph=True)
+        (g2,) = torch.autograd.grad((g * t).sum(), x)
+        with fwAD.dual_level():
+            tangent = fwAD.unpack_dual(fn(fwAD.make_dual(w, t))).tangent
+        got.append((g.detach(), g2, tangent))
+    for p, q in zip(*got):
+        assert torch.equal(p, q)
