@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import (_code, _has_tangent, _launch, _raise_for, _require_same_device, _scratch,
+from .ops import (_code, _differentiated, _launch, _raise_for, _require_same_device, _scratch,
                   _set_workspace, _status_ptr)
 
 __all__ = ["embed_tokens", "embed_tokens_fwd", "embed_tokens_bwd"]
@@ -107,10 +107,6 @@ def embed_tokens_bwd(ids, d_out, num_embeddings, scale=1.0, padding_idx=None, dt
     _set_workspace(a, workspace)
     _launch(lib.ngdn2_embed_bwd, a, dev, "ngdn2_embed_bwd")
     return dweight
-
-
-def _differentiated(t):
-    return torch.is_grad_enabled() and t.requires_grad or _has_tangent(t)
 
 
 class EmbedTokensFunction(torch.autograd.Function):

@@ -216,10 +216,12 @@ def _set_workspace(args, ws):
         args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
 
 
-def _has_tangent(*ts):
-    """Whether any of them (None passes) carries a forward-mode tangent, of
-    which ``requires_grad`` says nothing."""
-    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)
+def _differentiated(*ts):
+    """Whether autograd follows any of them (None passes): in reverse, or by a
+    forward-mode tangent, of which ``requires_grad`` says nothing."""
+    reverse = torch.is_grad_enabled()
+    return any(t is not None and (reverse and t.requires_grad
+                                  or forward_ad.unpack_dual(t).tangent is not None) for t in ts)
 
 
 def _require_same_device(t, *others):

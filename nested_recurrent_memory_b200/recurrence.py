@@ -15,8 +15,8 @@ import ctypes
 import torch
 
 from . import _lib
-from .ops import (_code, _launch, _raise_for, _require_same_device, _scratch, _set_workspace,
-                  _status_ptr)
+from .ops import (_code, _differentiated, _launch, _raise_for, _require_same_device, _scratch,
+                  _set_workspace, _status_ptr)
 
 __all__ = ["gated_scan", "gated_scan_fwd", "gated_scan_bwd", "step_gated_scan"]
 
@@ -141,18 +141,29 @@ class GatedScanFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dh, d_final):
         x, g, init, carries = ctx.saved_tensors
-        if dh is None:
-            dh = torch.zeros((), dtype=x.dtype, device=x.device).expand(x.shape)
-        dx, dg, dinit = gated_scan_bwd(x, g, dh, d_final, init, dict(carries=carries))
-        return dx, dg, dinit, None
+        if _differentiated(x, g, init, dh, d_final):
+            return *GatedScanBwdFunction.apply(x, g, dh, d_final, init, carries), None
+        return *gated_scan_bwd(x, g, dh, d_final, init, dict(carries=carries)), None
+
+
+class GatedScanBwdFunction(torch.autograd.Function):
+    """The gradients, tied to what they depend on: asking for their derivative
+    raises, however it is asked for (once_differentiable's error is passed by
+    where only some inputs' gradients are asked for)."""
+
+    @staticmethod
+    def forward(ctx, x, g, dh, d_final, initial_state, carries):
+        return gated_scan_bwd(x, g, dh, d_final, initial_state, dict(carries=carries))
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("gated_scan has no second derivatives")
 
 
 def gated_scan(x, g, initial_state=None, output_final_state=False):
     """``gated_scan_fwd`` with its gradient (``gated_scan_bwd``) in autograd:
-    returns ``(h, final_state)``."""
-    if not torch.is_grad_enabled() or not (
-            x.requires_grad or g.requires_grad
-            or (initial_state is not None and initial_state.requires_grad)):
+    returns ``(h, final_state)``. Second derivatives and forward mode raise."""
+    if not _differentiated(x, g, initial_state):
         return gated_scan_fwd(x, g, initial_state, output_final_state)
     return GatedScanFunction.apply(x, g, initial_state, output_final_state)
 

@@ -8,7 +8,7 @@ import torch
 import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
 
-from nested_recurrent_memory_b200 import embedding
+from nested_recurrent_memory_b200 import embedding, gated_scan, recurrence
 from nested_recurrent_memory_b200.embedding import embed_tokens
 
 V, D, SCALE = 7, 3, 1.5
@@ -106,3 +106,41 @@ def test_embedding_derivatives_on_the_kernels(dtype):
         got.append((g.detach(), g2, tangent))
     for p, q in zip(*got):
         assert torch.equal(p, q)
+
+
+@pytest.fixture
+def plain_recurrence(monkeypatch):
+    def fwd(x, g, initial_state=None, output_final_state=False, return_aux=False, workspace=None):
+        h = x.detach() * 2
+        final = h[:, -1].clone() if output_final_state else None
+        return (h, final, dict(carries=h)) if return_aux else (h, final)
+
+    def bwd(x, g, dh, d_final=None, initial_state=None, aux=None, workspace=None):
+        init = None if initial_state is None else torch.zeros_like(initial_state)
+        return dh.detach() * 2, torch.zeros_like(g), init
+
+    monkeypatch.setattr(recurrence, "gated_scan_fwd", fwd)
+    monkeypatch.setattr(recurrence, "gated_scan_bwd", bwd)
+
+
+def test_recurrence_refuses_second_derivatives(plain_recurrence):
+    x = torch.randn(2, 4, 3, requires_grad=True)
+    gate = torch.zeros(2, 4, 3, requires_grad=True)
+    (dx, dg) = torch.autograd.grad((gated_scan(x, gate)[0] ** 2).sum(), (x, gate), create_graph=True)
+    for loss in ((dx ** 2).sum(), dg.sum(), dx.sum()):
+        for leaf in (x, gate):
+            with pytest.raises(RuntimeError, match="second derivatives"):
+                torch.autograd.grad(loss + (x * gate).sum(), leaf, retain_graph=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        (dx ** 2).sum().backward()
+    (dx,) = torch.autograd.grad(gated_scan(x, gate)[0].sum(), x)  # first ones leave no graph
+    assert not dx.requires_grad
+
+
+@pytest.mark.parametrize("which", ["x", "g", "initial_state"])
+def test_recurrence_refuses_forward_mode(plain_recurrence, which):
+    ins = dict(x=torch.randn(2, 4, 3), g=torch.zeros(2, 4, 3), initial_state=torch.zeros(2, 3))
+    with fwAD.dual_level():
+        ins[which] = fwAD.make_dual(ins[which], torch.ones_like(ins[which]))
+        with pytest.raises(NotImplementedError):
+            gated_scan(**ins)
