@@ -17,8 +17,9 @@ passed in. No decode cache for the nested layers.
 Beyond the reference, the embedding may scale its rows (``embed_tokens``), and
 the layers named in ``recurrent_layers`` mix tokens with the channel-wise
 gated recurrence (``gated_scan``) instead of the nested op. A model of such
-layers only decodes token by token (``NestedGDN2ForCausalLM.step``). Everything
-is differentiable, so the same module trains (see ``optim.Muon``).
+layers only decodes token by token (``NestedGDN2ForCausalLM.step``). The forward
+is differentiable, so the same module trains (see ``optim.Muon``); ``step`` is
+not.
 """
 
 from __future__ import annotations
@@ -219,8 +220,9 @@ class GatedRecurrence(nn.Module):
         h, state = gated_scan(v, g, initial_state, output_final_state=True)
         return self._output(h, x), state
 
+    @torch.no_grad()
     def step(self, x, state):
-        """One token: x [B, d], state [B, value_dim] (updated in place) -> [B, d]."""
+        """One token, without gradients: x [B, d], state [B, value_dim] (updated in place) -> [B, d]."""
         v, g = self._inputs(x)
         h, _ = step_gated_scan(v, g, state, out_state=state)
         return self._output(h, x)
@@ -257,6 +259,7 @@ class NestedGDN2Block(nn.Module):
         h = h + a
         return h + self.mlp(self.mlp_norm(h))
 
+    @torch.no_grad()
     def step(self, h, state):
         h = h + self.attn.step(self.attn_norm(h), state)
         return h + self.mlp(self.mlp_norm(h))
@@ -300,9 +303,10 @@ class NestedGDN2ForCausalLM(nn.Module):
             h = h + layer.mlp(layer.mlp_norm(h))
         return self.lm_head(self.norm(h)), states
 
+    @torch.no_grad()
     def step(self, input_ids, states):
-        """One decode token for every row: [B] ids -> logits [B, V]; the states
-        (from ``prefill``) are updated in place."""
+        """One decode token for every row: [B] ids -> logits [B, V], without
+        gradients; the states (from ``prefill``) are updated in place."""
         self._require_recurrent()
         h = self.embeddings(input_ids)
         for layer, state in zip(self.layers, states, strict=True):

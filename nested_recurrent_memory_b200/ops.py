@@ -220,8 +220,12 @@ def _differentiated(*ts):
     """Whether autograd follows any of them (None passes): in reverse, or by a
     forward-mode tangent, of which ``requires_grad`` says nothing."""
     reverse = torch.is_grad_enabled()
-    return any(t is not None and (reverse and t.requires_grad
-                                  or forward_ad.unpack_dual(t).tangent is not None) for t in ts)
+    forward = getattr(forward_ad, "_current_level", 0) >= 0  # (asking each tensor takes 0.7 us)
+    for t in ts:
+        if t is not None and (reverse and t.requires_grad
+                              or forward and forward_ad.unpack_dual(t).tangent is not None):
+            return True
+    return False
 
 
 def _require_same_device(t, *others):

@@ -171,9 +171,13 @@ def gated_scan(x, g, initial_state=None, output_final_state=False):
 def step_gated_scan(x, g, state, *, out_state=None):
     """One decode token: x, g [B, D], state [B, D]. Returns ``(h, state)``,
     h [B, D] in x's dtype and the new state float32; ``out_state`` may be
-    ``state`` itself to update in place."""
+    ``state`` itself to update in place. Not differentiable: raises where
+    autograd would follow an input (``gated_scan`` has gradients)."""
     if x.dim() != 2 or x.shape != g.shape:
         raise ValueError(f"x and g must both be [B, D], got {tuple(x.shape)} and {tuple(g.shape)}")
+    if _differentiated(x, g, state):
+        raise RuntimeError("step_gated_scan is not differentiable: call it under torch.no_grad(), "
+                           "or gated_scan for gradients")
     dev = _require_same_device(x, g, state, out_state)
     B, D = x.shape
     state = _check_state(state, B, D, "state")

@@ -8,7 +8,8 @@ import torch
 import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
 
-from nested_recurrent_memory_b200 import embedding, gated_scan, recurrence
+from nested_recurrent_memory_b200 import (embedding, gated_scan, model, recurrence,
+                                          step_gated_scan)
 from nested_recurrent_memory_b200.embedding import embed_tokens
 
 V, D, SCALE = 7, 3, 1.5
@@ -144,3 +145,41 @@ def test_recurrence_refuses_forward_mode(plain_recurrence, which):
         ins[which] = fwAD.make_dual(ins[which], torch.ones_like(ins[which]))
         with pytest.raises(NotImplementedError):
             gated_scan(**ins)
+
+
+@pytest.mark.parametrize("which", ["x", "g", "state"])
+def test_step_refuses_gradients_that_it_would_drop(which):
+    """Refused before anything else is looked at."""
+    ins = dict(x=torch.randn(2, 3), g=torch.zeros(2, 3), state=torch.zeros(2, 3))
+    with fwAD.dual_level():
+        dual = {**ins, which: fwAD.make_dual(ins[which], torch.ones(2, 3))}
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            step_gated_scan(**dual)
+    ins[which].requires_grad_()
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        step_gated_scan(**ins)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+        step_gated_scan(**ins)
+
+
+def test_decoding_takes_no_part_in_autograd(monkeypatch):
+    """The model's step, with the states of a prefill that autograd follows."""
+    def scan(x, g, initial_state=None, output_final_state=False):
+        return x * 1.0, x[:, -1].float()
+
+    def step(x, g, state, out_state=None):
+        assert not torch.is_grad_enabled()
+        out_state.copy_(state + x)
+        return x * 1.0, out_state
+
+    monkeypatch.setattr(model, "gated_scan", scan)
+    monkeypatch.setattr(model, "step_gated_scan", step)
+    lm = model.NestedGDN2ForCausalLM(model.ModelConfig(
+        vocab_size=20, hidden_size=16, num_hidden_layers=2, num_heads=2, head_dim=8,
+        recurrent_layers=(0, 1)))
+    logits, states = lm.prefill(torch.zeros(1, 4, dtype=torch.long))
+    assert logits.requires_grad and states[0].requires_grad
+    assert not lm.step(torch.zeros(1, dtype=torch.long), states).requires_grad
+    block = lm.layers[0]
+    assert not block.step(torch.zeros(1, 16), states[0]).requires_grad
+    assert not block.attn.step(torch.zeros(1, 16), states[0]).requires_grad
