@@ -32,11 +32,15 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .embedding import embed_tokens
-from .ops import chunk_nested_gdn2
+from .ops import _DTYPES, chunk_nested_gdn2
 from .recurrence import gated_scan, step_gated_scan
 
 __all__ = ["ModelConfig", "NestedGDN2Attention", "GatedRecurrence", "ScaledEmbedding",
            "NestedGDN2Block", "NestedGDN2ForCausalLM"]
+
+
+# Whether a tensor is torch.func's stand-in for one, without memory of its own.
+_is_transformed = torch._C._functorch.is_functorch_wrapped_tensor
 
 
 @dataclass
@@ -230,14 +234,16 @@ class GatedRecurrence(nn.Module):
 
 class ScaledEmbedding(nn.Embedding):
     """Token embedding times a constant: ``embed_tokens`` on a GPU, torch's
-    lookup elsewhere (for models whose op runs there)."""
+    lookup for what that does not take (a model with another op may run on the
+    host, in float64 or under torch.func's transforms)."""
 
     def __init__(self, num_embeddings: int, dim: int, scale: float = 1.0):
         super().__init__(num_embeddings, dim)
         self.scale = scale
 
     def forward(self, input_ids):
-        if self.weight.is_cuda:
+        if self.weight.is_cuda and self.weight.dtype in _DTYPES and not (
+                _is_transformed(self.weight) or _is_transformed(input_ids)):
             return embed_tokens(input_ids, self.weight, self.scale, self.padding_idx)
         y = super().forward(input_ids)
         return y if self.scale == 1.0 else y * self.scale

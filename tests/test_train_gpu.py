@@ -126,3 +126,26 @@ def test_split_parameters_keeps_vectors_embeddings_and_head_apart():
     assert all("conv1d" in n or "norm" in n or "bias" in n or "log" in n or "head" in n or "embed" in n
                for n in kept)
     assert any("key_projections" in names[id(p)] for p in matrices)
+
+
+def test_the_models_embedding_takes_what_torchs_takes():
+    """float64 tables (of a model with another op), and torch.func's transforms."""
+    gen = torch.Generator().manual_seed(3)
+    w, ids = torch.randn(12, 5, generator=gen).cuda(), torch.randint(0, 12, (4, 6), generator=gen).cuda()
+    emb = model_module.ScaledEmbedding(12, 5, scale=4.0).cuda()
+    with torch.no_grad():
+        emb.weight.copy_(w)
+    double = model_module.ScaledEmbedding(12, 5, scale=4.0).cuda().double()
+    y = double(ids)
+    assert y.dtype == torch.float64 and torch.equal(y, F.embedding(ids, double.weight) * 4.0)
+    y.sin().sum().backward()
+    assert double.weight.grad.dtype == torch.float64
+
+    def loss(weight, one):
+        return torch.func.functional_call(emb, {"weight": weight}, (one,)).sin().sum()
+
+    each = torch.func.vmap(torch.func.grad(loss), in_dims=(None, 0))(emb.weight.detach(), ids)
+    for i in range(4):
+        x = emb.weight.detach().clone().requires_grad_()
+        (ref,) = torch.autograd.grad((F.embedding(ids[i], x) * 4.0).sin().sum(), x)
+        assert torch.allclose(each[i], ref, rtol=1e-5, atol=1e-5)
