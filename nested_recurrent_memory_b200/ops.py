@@ -55,10 +55,10 @@ class KernelStatusError(RuntimeError):
 def _status_message(bits: int) -> str:
     parts = []
     if bits & _lib.STATUS_WAIT_TIMEOUT:
-        parts.append("a bounded pipeline wait timed out (outputs invalid; treat the CUDA "
-                     "context as suspect)")
+        parts.append("nested GDN-2 forward, gated recurrence or orthogonalisation: a bounded wait "
+                     "timed out (outputs invalid; treat the CUDA context as suspect)")
     if bits & _lib.STATUS_GATE_TIMEOUT:
-        parts.append("the start gate stayed closed (nothing was computed)")
+        parts.append("nested GDN-2 forward: the start gate stayed closed (nothing was computed)")
     if bits & _lib.STATUS_BAD_INDEX:
         parts.append("embedding: a token id outside [0, V) (its output row is NaN, its gradient "
                      "left out)")
@@ -66,9 +66,10 @@ def _status_message(bits: int) -> str:
 
 
 class _DeviceStatus:
-    """The sticky status word every forward on one device reports into.
+    """The sticky status word that every forward, embedding, recurrence and
+    orthogonalisation on one device reports into.
 
-    Kernels only OR bits into the device word. After each launch a 4-byte
+    Kernels only OR bits into the device word. After each forward a 4-byte
     copy of it goes to pinned host memory on the launching stream, and an
     event marks that copy; the next launch on the device (or ``check``)
     reads the copy once its event has completed and raises
@@ -100,8 +101,7 @@ class _DeviceStatus:
         if bits:
             self.word.zero_()
             self.host.zero_()
-            what = "nested GDN-2 forward: " if bits != _lib.STATUS_BAD_INDEX else ""
-            raise KernelStatusError(what + _status_message(bits))
+            raise KernelStatusError(_status_message(bits))
 
     def poll(self):
         """Raise for a status copied back by an earlier launch, if its copy is done."""
@@ -132,7 +132,7 @@ _SYNC_CHECK = __import__("os").environ.get("NGDN2_SYNC_CHECK", "0") not in ("", 
 
 
 def check_status(device=None, sync: bool = True):
-    """Raise ``KernelStatusError`` if a forward on ``device`` (default: the
+    """Raise ``KernelStatusError`` if a call on ``device`` (default: the
     current CUDA device) reported a device status since the last check, then
     clear it. ``sync=True`` waits for the device's queued work first."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)

@@ -166,3 +166,20 @@ def test_scratch_memory_is_checked():
     for bad in (own.to("meta"), own[::2], torch.empty(1, dtype=torch.uint8).expand(200)):
         with pytest.raises(ValueError, match="workspace"):
             _scratch(need, bad, cpu)
+
+
+@pytest.mark.parametrize(("bits", "named", "not_named"), [
+    (_lib.STATUS_WAIT_TIMEOUT, ("recurrence", "orthogonalisation", "nested GDN-2 forward", "wait"), ("embedding",)),
+    (_lib.STATUS_GATE_TIMEOUT, ("nested GDN-2 forward", "start gate"), ("recurrence", "embedding")),
+    (_lib.STATUS_BAD_INDEX, ("embedding", "token id"), ("nested", "wait"))])
+def test_status_errors_name_the_calls_that_can_set_them(bits, named, not_named):
+    """The word is shared: an error does not blame a forward that did not run."""
+    from nested_recurrent_memory_b200 import KernelStatusError
+    from nested_recurrent_memory_b200.ops import _DeviceStatus
+
+    st = _DeviceStatus.__new__(_DeviceStatus)
+    st.word = st.host = torch.full((1,), bits, dtype=torch.int32)
+    with pytest.raises(KernelStatusError) as e:
+        st._raise_if_set(bits)
+    assert all(n in str(e.value) for n in named) and not any(n in str(e.value) for n in not_named)
+    assert int(st.word) == 0
