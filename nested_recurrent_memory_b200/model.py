@@ -212,7 +212,10 @@ class GatedRecurrence(nn.Module):
     def _inputs(self, x):
         g = -self.A_log.float().exp() * F.softplus(self.f_proj(x).float() + self.dt_bias)
         v = self.v_proj(x)
-        return (v * torch.sqrt(-torch.expm1(2.0 * g))).to(v.dtype), g
+        kept = -torch.expm1(2.0 * g)
+        shut = kept == 0  # (where the root's slope is infinite, and softplus' slope zero)
+        gain = kept.masked_fill(shut, 1.0).sqrt().masked_fill(shut, 0.0)
+        return (v * gain).to(v.dtype), g
 
     def _output(self, h, x):
         heads = (*h.shape[:-1], self.H, self.V)

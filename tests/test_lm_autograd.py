@@ -183,3 +183,21 @@ def test_decoding_takes_no_part_in_autograd(monkeypatch):
     block = lm.layers[0]
     assert not block.step(torch.zeros(1, 16), states[0]).requires_grad
     assert not block.attn.step(torch.zeros(1, 16), states[0]).requires_grad
+
+
+def test_recurrent_layer_gradients_where_nothing_decays():
+    """A gate so far shut that softplus gives zero: no input, no gradient, no NaN."""
+    layer = model.GatedRecurrence(model.ModelConfig(hidden_size=16, num_heads=2, head_dim=8))
+    with torch.no_grad():
+        layer.f_proj[1].weight.zero_()
+        layer.dt_bias[:4] = -200.0
+        layer.dt_bias[4:8] = -100.0
+        layer.v_proj.weight.normal_()
+    x = torch.randn(2, 3, 16, requires_grad=True)
+    v, g = layer._inputs(x)
+    assert bool((v[..., :4] == 0).all()) and bool((g[..., :4] == 0).all())
+    want = layer.v_proj(x) * torch.sqrt(-torch.expm1(2.0 * g))
+    assert torch.equal(v, want)
+    (v.square().sum() + v.sum() + g.sum()).backward()
+    for t in (x, layer.dt_bias, layer.A_log, layer.f_proj[0].weight, layer.v_proj.weight):
+        assert bool(torch.isfinite(t.grad).all())
