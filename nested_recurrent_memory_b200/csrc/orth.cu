@@ -8,20 +8,20 @@
 // Gaussian updates, fp16) to 3e-1 (a strong direction over a weak remainder,
 // bf16). So every operand is held as two fp16 planes, hi + lo (22 bits; X,
 // A and B scaled to the middle of fp16's range), and a product is three MMAs,
-// hi hi + hi lo + lo hi, summed in fp32 in tensor memory: the accuracy of fp32
-// arithmetic (about 1e-6 .. 1e-5 on the same updates) at a third of the
-// tensor cores' rate. A 16-bit update fits its hi plane, so the first step
-// needs one product for A and two for X. That holds for the last step too,
-// whatever the result's type: a 16-bit result is the fp32 one rounded once.
-// (Its hi planes alone would take 13/15 of the MMAs, and change bf16 results
-// by as much as their rounding does.)
+// hi hi + hi lo + lo hi, summed in fp32 (in tensor memory, and in registers from
+// 512 terms on): the error of fp32 arithmetic within a factor of ten (4e-6 .. 3e-5
+// after five steps, whatever the size) at a third of the tensor cores' rate. A 16-bit
+// update fits its hi plane, so the first step needs one product for A and two for X.
+// The last step is computed like the others whatever the result's type: a 16-bit
+// result is the fp32 one rounded once. (Its hi planes alone would take 13/15 of the
+// MMAs, and change bf16 results by as much as their rounding does.)
 //
 // Matrices of up to 128 rows and about 1500 columns (more for fewer rows) take one
 // launch, a CTA or a cluster each (orth_small_kernel). Larger ones: the squared
-// norm (partial sums in 64 bits), the conversion to planes, and the products of all steps: A = X X^T, B = a I + b A
-// + c A A (both symmetric: the tiles on and above the diagonal, written twice)
-// and X' = B X, which reads X as it lies, rows along the reduction. The
-// products are cut into tiles, handed out by a counter. For large batches one
+// norm (partial sums in 64 bits), the conversion to planes, and the products of all
+// steps: A = X X^T, B = a I + b A + c A A (both symmetric: the tiles on and above the
+// diagonal, written twice) and X' = B X, which reads X as it lies, rows along the
+// reduction. The products are cut into tiles, handed out by a counter. For large batches one
 // launch does them all, in an order in which every tile's operands come from
 // tiles before it: a tile waits until those of its matrix are done, so one
 // matrix's next product starts while others' last one still runs. Every wait
@@ -309,6 +309,13 @@ enum { kGram = 0, kPoly = 1, kApply = 2 };  // A = X X^T; B = a I + b A + c A A;
 
 constexpr int kRows = 256;            // of a pair's tile
 constexpr int kDepth = 64;            // reduction elements of a stage
+// Stages whose sum stays in the tensor core's accumulator, which cuts every addition
+// off instead of rounding it, so that the error grows with their number; longer sums are
+// added up in fp32 registers. (Relative error of a 4096 x 4096 fp32 result: one sum 7.6e-5,
+// sums of 16, 8 and 4 stages 2.6e-5, 1.4e-5 and 7.2e-6, fp32 arithmetic 6.5e-6. us a call
+// in a row, one sum and sums of 8 stages: 1001 x 345 174 and 177, 1024 x 2816 340 and 354,
+// 12 x 1024 x 2816 1757 and 1773.)
+constexpr int kRun = 8;
 constexpr int kLeft = 128 * kDepth * 2;  // bytes of the left operand's plane in one CTA, a stage
 
 // Tiles of BN columns: a stage holds both operands' planes; as many stages as
@@ -612,14 +619,47 @@ __device__ __forceinline__ void stage_free() {
   __syncwarp();
 }
 
+// A unit whose reduction is longer than kRun stages comes in parts, by turns in both
+// accumulators. A writing warp adds them up in registers and leaves the sum in
+// the last one's place.
+template <int BN>
+__device__ __forceinline__ bool add_parts(Barriers* s, const MulArgs& p, int parts, uint32_t tmem, uint32_t* buf,
+                                          uint32_t* phase) {
+  const int quarter = threadIdx.x >> 5 & 3, half = (threadIdx.x >> 7) - 1;
+  float sum[BN / 2] = {};
+  for (;;) {
+    if (!__all_sync(0xffffffffu, wait_or_die(s, &s->acc_full[*buf], *phase, p))) return false;
+    fence_after_sync();
+    const uint32_t at = taddr(tmem + *buf * BN, quarter * 32, half * (BN / 2));
+#pragma unroll
+    for (int i = 0; i < BN / 2; i += 16) {
+      float v[16];
+      tmem_ld16(at + i, v);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sum[i + j] += v[j];
+    }
+    if (--parts == 0) {
+#pragma unroll
+      for (int i = 0; i < BN / 2; i += 16) tmem_st16(at + i, sum + i);
+      tmem_wait_st();
+      return true;
+    }
+    fence_before_sync();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) arrive_at(in_first(&s->acc_empty[*buf]));
+    *buf ^= 1;
+    if (*buf == 0) *phase ^= 1;
+  }
+}
+
 // A writing warp's part of a unit: 32 rows by BN / 2 columns, sixteen columns at a
 // time in a loop that is not unrolled: a launch that writes few tiles finds its
 // code cold, and 32 columns spelled out took 15000 cycles of a product's 26000
 // (1001 x 345) to be fetched.
 template <int MODE, int BN>
 __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const Unit& u, const CUtensorMap* out,
-                                           unsigned char* mem, uint32_t rank, uint32_t acc, uint64_t* acc_full,
-                                           uint32_t acc_phase) {
+                                           unsigned char* mem, uint32_t rank, uint32_t tmem, uint32_t* buf,
+                                           uint32_t* phase) {
   const int lane = threadIdx.x & 31, quarter = threadIdx.x >> 5 & 3, half = (threadIdx.x >> 7) - 1;
   const int m = int(p.m), cols = int(MODE == kApply ? p.n : p.m), z = int(u.b * 2);
   const int r0 = int(u.tm * kRows + rank * 128 + quarter * 32), r = r0 + lane, c1 = int(u.tn * BN + half * (BN / 2));
@@ -640,15 +680,18 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
         ol[k] = __ldcg(reinterpret_cast<const uint4*>(old + int64_t(m) * p.ld + c + 8 * k));
       }
   };
-  if (MODE == kPoly && !p.wait) ask(c1);
-  bool ok = wait_or_die(s, acc_full, acc_phase, p);
+  const bool early = BN < 256 && !p.wait;  // (else the registers are for the sum)
+  if (MODE == kPoly && early) ask(c1);
+  const int parts = (u.blocks + kRun - 1) / kRun;
+  bool ok = parts > 1 ? add_parts<BN>(s, p, parts, tmem, buf, phase) : wait_or_die(s, &s->acc_full[*buf], *phase, p);
+  const uint32_t acc = tmem + *buf * BN;
   // (The product is there, so A is. Only now: eight warps of every CTA that
   // polled for it would hold up those that announce it.)
   if (MODE == kPoly && p.wait && lane == 0) ok = ok && wait_operands(s, p, u);
   if (!__all_sync(0xffffffffu, ok)) return false;
   __syncwarp();
   fence_after_sync();
-  if (MODE == kPoly && p.wait) ask(c1);
+  if (MODE == kPoly && !early) ask(c1);
   // Below the diagonal lanes are neighbours: two lanes swap values so that each
   // stores two of them, of every other column. (Through the stage as well,
   // each store would wait for the one before.)
@@ -853,37 +896,41 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
       const uint64_t left_desc = desc_sw128(base, 1024), right_step = (down ? Shape<BN>::kBoxCols * 32 : 32) >> 4;
       const uint64_t right_desc = down ? desc_down<Shape<BN>::kBoxCols>(base + 2 * kLeft, Shape<BN>::kBox)
                                        : desc_sw128(base + 2 * kLeft, 1024);
-      ok = wait_or_die(s, &s->acc_empty[buf], acc_phase ^ 1, p);
-      const uint32_t d = tmem + buf * BN;
-      for (int k = 0; ok && k < u.blocks; ++k) {
-        ok = wait_or_die(s, &s->full[st], phase, p);
-        if (!ok) break;
-        fence_after_sync();
-        // Descriptors count 16 bytes: the lo planes and the next 16 of the
-        // reduction (32 bytes of a row, or 16 rows) are additions away. One thread
-        // issues everything, so what it computes for an MMA must not take
-        // longer than the MMA (64 cycles for 128 columns).
-        uint64_t dl = left_desc + ((st * kStage) >> 4), dr = right_desc + ((st * kStage) >> 4);
+      for (int left = u.blocks; ok && left > 0; left -= kRun) {
+        ok = wait_or_die(s, &s->acc_empty[buf], acc_phase ^ 1, p);
+        const uint32_t d = tmem + buf * BN;
+        const int stages = left < kRun ? left : kRun;
+        for (int k = 0; ok && k < stages; ++k) {
+          ok = wait_or_die(s, &s->full[st], phase, p);
+          if (!ok) break;
+          fence_after_sync();
+          // Descriptors count 16 bytes: the lo planes and the next 16 of the
+          // reduction (32 bytes of a row, or 16 rows) are additions away. One thread
+          // issues everything, so what it computes for an MMA must not take
+          // longer than the MMA (64 cycles for 128 columns).
+          uint64_t dl = left_desc + ((st * kStage) >> 4), dr = right_desc + ((st * kStage) >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kDepth / 16; ++kk) {
-          mma_pair(d, dl, dr, idesc, (k | kk) != 0);
-          if (u.lo_right) mma_pair(d, dl, dr + (kRight >> 4), idesc, 1);
-          if (u.lo_left) mma_pair(d, dl + (kLeft >> 4), dr, idesc, 1);
-          dl += 32 >> 4;
-          dr += right_step;
+          for (int kk = 0; kk < kDepth / 16; ++kk) {
+            mma_pair(d, dl, dr, idesc, (k | kk) != 0);
+            if (u.lo_right) mma_pair(d, dl, dr + (kRight >> 4), idesc, 1);
+            if (u.lo_left) mma_pair(d, dl + (kLeft >> 4), dr, idesc, 1);
+            dl += 32 >> 4;
+            dr += right_step;
+          }
+          commit_pair(&s->empty[st]);
+          last = &s->empty[st];
+          last_phase = phase;
+          if (++st == kStages) {
+            st = 0;
+            phase ^= 1;
+          }
         }
-        commit_pair(&s->empty[st]);
-        last = &s->empty[st];
-        last_phase = phase;
-        if (++st == kStages) {
-          st = 0;
-          phase ^= 1;
-        }
+        if (!ok) break;
+        commit_pair(&s->acc_full[buf]);
+        buf ^= 1;
+        if (buf == 0) acc_phase ^= 1;
       }
       if (!ok) break;
-      commit_pair(&s->acc_full[buf]);
-      buf ^= 1;
-      if (buf == 0) acc_phase ^= 1;
     }
     // (The loads' thread waits for the same, unless it has left early.)
     if (last) drain(last, last_phase, kPolls);
@@ -897,10 +944,9 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
       t = __shfl_sync(0xffffffffu, t, 0);
       if (t >= p.end) break;
       const Unit u = unit_at<BN>(p, plan, t);
-      const uint32_t acc = tmem + buf * BN;
       after_previous();
       auto write = [&](auto mode, const CUtensorMap* out) {
-        return write_unit<decltype(mode)::value, BN>(s, p, u, out, mem, rank, acc, &s->acc_full[buf], acc_phase);
+        return write_unit<decltype(mode)::value, BN>(s, p, u, out, mem, rank, tmem, &buf, &acc_phase);
       };
       if constexpr (SYM)
         if (u.mode == kGram) ok = write(std::integral_constant<int, kGram>{}, &maps.a_out);
