@@ -195,3 +195,31 @@ def test_another_stream_and_graph_capture():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, ref) and torch.equal(dw, dref)
+
+
+@pytest.mark.parametrize("N", [1, 700, 9000, 16385, 300001])
+@pytest.mark.parametrize("V", [(1 << 18) - 1, 1 << 18, 1 << 20])
+def test_tables_whose_tokens_take_three_passes(N, V):
+    """Two sorting passes end at 2^18 - 1 rows; lists sorted by one cluster and in
+    tiles of either size."""
+    D = 8
+    for zipf in (True, False):
+        ids, _, d = _inputs(N, V, D, torch.float32, seed=11, zipf=zipf)
+        ids[0] = V - 1
+        dw = embed_tokens_bwd(ids, d, V, scale=3.0, padding_idx=5)
+        _check_grad(dw, ids, d, 3.0, pad=5)
+        assert torch.equal(embed_tokens_bwd(ids, d, V, scale=3.0, padding_idx=5), dw)
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 72, 1000])
+def test_gradients_of_another_type(dtype, out, D):
+    """Rows read 16 bytes at a time, written in the gradient's own type."""
+    ids, _, d = _inputs(3000, 200, D, dtype, seed=12)
+    dw = embed_tokens_bwd(ids, d, 200, scale=2.0, dtype=out)
+    assert dw.dtype == out
+    _check_grad(dw, ids, d, 2.0)
+    off = torch.empty(3000 * D + 1, dtype=dtype, device="cuda")[1:].view(3000, D)
+    off.copy_(d)  # rows off every 16-byte boundary: element by element, the same sums
+    assert torch.equal(embed_tokens_bwd(ids, off, 200, scale=2.0, dtype=out), dw)
