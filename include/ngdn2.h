@@ -290,7 +290,8 @@ typedef struct ngdn2_embed_args {
 /* Arguments of ngdn2_embed_bwd:
  * dweight[v] = scale * sum over {n : ids[n] = v} of d_out[n], every row
  * written (zeros where no token points, and for padding_idx). Summed in
- * fp32 in the order of n, so the result is reproducible. */
+ * fp32 in an order that follows from ids and N alone, so the result is
+ * reproducible. */
 typedef struct ngdn2_embed_bwd_args {
   int32_t abi_version;
   int32_t dtype;         /* of d_out */
@@ -312,8 +313,10 @@ typedef struct ngdn2_embed_bwd_args {
 #define NGDN2_SCAN_CHUNK 128
 
 /* Arguments of ngdn2_scan: h_t = e^(g_t) h_{t-1} + x_t for each (batch row,
- * channel), the state in fp32. g = -inf drops the state (a packed sequence
- * starts); strides are in elements, 0 included. */
+ * channel), the state in fp32. g = -inf drops a finite state (a packed sequence
+ * starts); g may be positive as long as the factors of 128 consecutive steps
+ * multiply to less than fp32's largest number. Strides are in elements, 0
+ * included. */
 typedef struct ngdn2_scan_args {
   int32_t abi_version;
   int32_t B;
@@ -361,8 +364,8 @@ typedef struct ngdn2_scan_step_args {
 
 /* Arguments of ngdn2_orth: X_0 = G / (|G|_F + eps), then ``steps`` times
  * X <- a X + (b A + c A A) X with A = X X^T taken over the smaller side,
- * for each of ``batch`` matrices. Products to fp32's accuracy, whatever the
- * element types. */
+ * for each of ``batch`` matrices. Operands hold 22 bits and sums are fp32,
+ * whatever the element types: a 16-bit result is the fp32 one rounded once. */
 typedef struct ngdn2_orth_args {
   int32_t abi_version;
   int32_t dtype;               /* of update */

@@ -6,13 +6,14 @@
 // d_out once and writes every row of dweight once.
 //
 // The gradient sorts (token, position) pairs by token with a stable radix
-// sort, so that a row's terms are added in the order of their positions and
-// the result is reproducible (in one launch by a cluster up to 16384 tokens). The
-// sorted list is then cut into chunks of
+// sort (in one launch by a cluster up to 16384 tokens), so that a row's terms lie
+// in the order of their positions. The sorted list is then cut into chunks of
 // equal length, however often a token occurs: a CTA adds up the runs of
-// equal tokens in its chunk; a run that lies within the chunk is its row's
+// equal tokens in its chunk, in order; a run that lies within the chunk is its row's
 // gradient, the parts of one that crosses into other chunks are left in
-// fp32 and joined in order afterwards. A short list's sort keeps few multiprocessors
+// fp32 and joined afterwards: every fourth part by one of four warps, then the
+// warps' sums. So the order of a row's additions follows from the tokens and N alone,
+// and the result is reproducible. A short list's sort keeps few multiprocessors
 // busy; the others meanwhile zero dweight's last rows, whether they have
 // tokens or not, as far as its time goes. Other rows without a token are
 // zeroed by CTAs of the launch that sums.

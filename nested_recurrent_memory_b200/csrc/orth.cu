@@ -762,8 +762,7 @@ __device__ __forceinline__ bool write_unit(Barriers* s, const MulArgs& p, const 
 // also fetches unit numbers for both) and eight warps write; in the first CTA a
 // thread issues the MMAs for both.
 // SYM, APP: whether the launch has units of A or B, and of X' (a kernel for all
-// takes longer to start: all steps of 512 x 4096 take 298 us with it, 291 with
-// one for each).
+// takes longer to start: a call of 512 x 4096 321 us with it, 313 with one for each).
 template <int BN, bool SYM, bool APP>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kMulThreads, 1)
 orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Plan<BN> plan,
@@ -809,8 +808,8 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
     // Loads of this CTA's halves: 128 rows of the left operand, BN / 2 rows (or
     // columns, kApply) of the right one, hi and lo. The first CTA's thread also
     // fetches the next unit's number, with its last load of a unit: earlier,
-    // and units would wait here while other pairs go idle (2048 x 2048, two
-    // units ahead in one launch: 1031 us against 662).
+    // and units would wait here while other pairs go idle (2048 x 2048 in one
+    // launch took 1.6 times as long with two units fetched ahead).
     uint32_t st = 0, phase = 0;
     auto fetch = [&](uint32_t* next) {
       *next = atomicAdd(&p.sync->units, 1u);
@@ -995,7 +994,7 @@ orth_steps_kernel(const __grid_constant__ MulArgs p, const __grid_constant__ Pla
 // operand with the reduction down the columns. A's slices are summed through
 // distributed shared memory: every CTA adds up a part of A's rows and gives its
 // planes to all. What bounds it is the chain of a step's three
-// products, 2.3 us each (16 matrices 128 x 128: 40.7 us), most of it not the
+// products, 2.7 us each (16 matrices 128 x 128: 43 us a call in a row), most of it not the
 // MMAs but getting the results out of tensor memory and back as operands.
 // ---------------------------------------------------------------------------
 
@@ -1091,7 +1090,7 @@ __global__ void __launch_bounds__(kSmallThreads, 1) orth_small_kernel(const __gr
     *reinterpret_cast<uint4*>(mem + i) = make_uint4(0, 0, 0, 0);
   // The slice, in registers: four neighbours along the dimension with the
   // smaller stride are a piece, all pieces' loads are in flight together (16
-  // matrices 128 x 128: 46.2 us where the planes' values were read again after
+  // matrices 128 x 128: 5 us more where the planes' values were read again after
   // the norm).
   const bool along_c = p.sc <= p.sr;
   const int outer = along_c ? m : n, inner = along_c ? n : m;
@@ -1422,17 +1421,18 @@ cudaError_t launch_product(const MulArgs& p, const Maps& maps, int step, int mod
 }
 
 // The tiles' width goes by the rounds that the pairs of CTAs take: one of 128
-// columns takes 0.6 of the time of one of 256, one of 64 0.5 (all steps, one round
-// either way, 64 columns against 128: 1001 x 345 159.5 and 179.4 us, 256 x 512
-// 112.4 and 130.6, 8 x 256 x 512 123.2 and 136.2). An element's sum has the same
+// columns takes 0.6 of the time of one of 256, one of 64 0.5 (us a call, calls in a
+// row, with tiles of 64 columns and without: 1001 x 345 176 and 199, 256 x 512 130 and 149,
+// 8 x 256 x 512 141 and 158, 1024 x 2816 355 and 384). An element's sum has the same
 // order in all.
 constexpr double kTime128 = 0.6, kTime64 = 0.5;
 
 // One launch for all steps where a product of all matrices fills the pairs more
 // than once, so that there is always a unit whose operands are ready; otherwise
 // a launch for each product, whose start costs less than the signals between
-// units (us, one launch against one a product: 12 x 1024 x 2816 1394 and 1556, 12 x
-// 1024 x 1024 818 and 877; 1024 x 2816 423 and 394).
+// units (us a call, calls in a row, one launch against one a product: 12 x 1024 x 1024 741
+// and 881, 80 x 200 x 264 301 and 372, 26 x 300 x 400 240 and 258; 1024 x 2816 396 and 355,
+// 1001 x 345 210 and 176).
 cudaError_t launch_steps(MulArgs p, const Maps& maps, const Maps& thin_rows, const Maps& thin_down, uint32_t pairs,
                          cudaStream_t st) {
   const Plan<256> wide(p);

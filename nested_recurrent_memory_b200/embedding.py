@@ -4,8 +4,8 @@
     y[..., :] = scale * weight[ids[...], :]
     dweight[v] = scale * sum over the tokens of v of d_out
 
-The gradient sums in fp32 in the order of the tokens, so the same inputs
-give the same bits, and writes every row of ``dweight`` once.
+The gradient sums in fp32 in an order that follows from the tokens alone, so
+the same inputs give the same bits, and writes every row of ``dweight`` once.
 """
 
 from __future__ import annotations

@@ -26,7 +26,8 @@ def orthogonalize(update, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1
     bfloat16 or float16; leading dimensions are a batch of matrices treated
     each on its own (layers stacked, or promotion parameters
     [L - 1, H, rows, cols]). Returns the same shape in ``dtype`` (default
-    update's). Products and sums keep fp32's accuracy whatever the types.
+    update's). Operands hold 22 bits and sums are fp32 whatever the types: a
+    16-bit result is the fp32 one rounded once.
 
     ``coefficients`` (a, b, c) must keep every singular value that starts in
     [0, 1] within [0, 4] over ``steps`` steps, else ValueError. A zero update

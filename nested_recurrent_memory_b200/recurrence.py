@@ -4,8 +4,10 @@
     h_t = e^{g_t} h_{t-1} + x_t        for every channel, t = 1 .. T
 
 The state is fp32 throughout. ``g`` are log-decays, as in the nested op
-(``<= 0`` for a decay); ``g = -inf`` drops the state, so packed sequences of
-different lengths are one call with -inf at each sequence's first token.
+(``<= 0`` for a decay); ``g = -inf`` drops a finite state, so packed sequences of
+different lengths are one call with -inf at each sequence's first token. ``g`` may
+be positive as long as the factors of 128 consecutive steps multiply to less
+than fp32's largest number.
 """
 
 from __future__ import annotations
