@@ -208,26 +208,31 @@ def test_sixteen_bit_results_are_the_fp32_ones_rounded(shape, dtype):
         assert torch.equal(orthogonalize(G, dtype=out), full.to(out))
 
 
-def _stop_word(ws, batch, m, n):
+def _stop_word(ws, batch, m, n, steps):
     """Where a call's kernels note in its workspace that a wait gave up: the
     second word after the planes of X (twice), A and B, the sums and scales."""
     up = lambda x, k: (x + k - 1) // k * k  # noqa: E731
     at = 2 * up(batch * 2 * m * up(n, 8) * 2, 256) + 2 * up(batch * 2 * m * up(m, 8) * 2, 256)
-    at += up(batch * 128 * 8, 256) + up(batch * 4, 256)
+    at += up(batch * 128 * 8, 256) + up(batch * steps * 8, 256)
     assert ws.data_ptr() % 256 == 0
     return ws[at + 4:at + 8].view(torch.int32)
 
 
-def _stopped_call(n=2048, steps=24):
+def _stopped_call(n=2048, steps=64):
     """A call of many launches during which another stream sets that word, as
     a wait that gives up does."""
     G = _update((n, n), torch.float32, seed=13)
     ws = torch.empty(32 * n * n, dtype=torch.uint8, device="cuda")
-    stop = _stop_word(ws, 1, n, n)
-    side = torch.cuda.Stream()
+    stop = _stop_word(ws, 1, n, n, steps)
+    main, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    start = torch.cuda.Event()
     torch.cuda.synchronize()
+    torch.cuda._sleep(10 ** 8)  # all of this is queued before any of it runs
+    start.record(main)
     out = orthogonalize(G, steps=steps, coefficients=(1.5, -0.5, 0.0), workspace=ws)
     with torch.cuda.stream(side):
+        side.wait_event(start)
+        torch.cuda._sleep(10 ** 6)  # half a millisecond into the call
         stop.fill_(1)
     torch.cuda.synchronize()
     assert int(stop) == 1
